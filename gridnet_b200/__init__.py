@@ -8,13 +8,15 @@ native extension module. Everything runs through ``libgridnet_b200.so`` (C ABI i
 """
 from . import gridnet_cuda
 from ._lib import LIB_PATH, GridnetB200Error
-from .backend_cuda import (FusedGatedLoopTrainOp, FusedLoopResidualTrainOp, FusedLoopSeparateTrainOp, FusedLoopTrainOp, fused_loop_forward, GatedGridnetCudaOp, GridnetCudaOp, GridNormOp, HostPipelinedForward, device_status, fused_step,
+from .backend_cuda import (FusedGatedLoopTrainOp, FusedLoopResidualTrainOp, FusedLoopSeparateTrainOp, FusedLoopTrainOp, fused_loop_forward, GatedGridnetCudaOp, GridnetCudaOp, GridNormOp, HostPipelinedForward, PackedGridNormOp, device_status, fused_step,
                            keep_forward_stash, norm_apply,
                            norm_finalize, outer_forward, outer_forward_failed, outer_forward_workspace,
                            step_stats_partials)
 
 from .modules import (GatedGridnet, Gridnet, GridnetModel, GridNorm, Readout, gated_gridnet_step,
                       gridnet_step)
+from .packed import PackedActivations, keep_packed, pack_activations, unpack_activations
+from .scan import GatedRecurrence, GatedScanOp, gated_scan, gated_scan_step
 from .script_models import ImageNetModel, MnistModel
 from .web_checkpoint import read_web_checkpoint, write_web_checkpoint
 
@@ -31,6 +33,15 @@ __all__ = [
     "GridnetCudaOp",
     "GatedGridnetCudaOp",
     "GridNormOp",
+    "PackedGridNormOp",
+    "PackedActivations",
+    "pack_activations",
+    "unpack_activations",
+    "keep_packed",
+    "GatedScanOp",
+    "gated_scan",
+    "gated_scan_step",
+    "GatedRecurrence",
     "FusedLoopResidualTrainOp",
     "FusedLoopSeparateTrainOp",
     "FusedLoopTrainOp",

@@ -96,6 +96,15 @@ SIGNATURES = {
     "gn_outer_forward_error_flag_offset": (c_size_t, [c_int] * 5),
     "gn_outer_forward_f32": (c_int, [_P] * 7 + _geom + [c_int, c_int, c_int, c_float, c_int, _P, c_size_t, _P]),
     "gn_outer_forward_flags_f32": (c_int, [_P] * 7 + _geom + [c_int, c_int, c_int, c_float, c_int, _P, c_size_t, c_int, _P]),
+    "gn_pack8": (c_int, [_P] * 3 + [c_longlong] * 2 + [c_int, _P]),
+    "gn_unpack8": (c_int, [_P] * 3 + [c_longlong] * 2 + [c_int, _P]),
+    "gn_norm_packed_workspace_bytes": (c_size_t, [c_int, c_longlong]),
+    "gn_norm_forward_packed_f32": (c_int, [_P] * 7 + [c_int, c_longlong, c_float, _P, c_size_t, _P]),
+    "gn_norm_backward_packed_f32": (c_int, [_P] * 8 + [c_int, c_longlong, _P, c_size_t, _P]),
+    "gn_gated_scan_bounds_bytes": (c_size_t, [c_int, c_longlong, c_longlong, c_int, c_int, c_int]),
+    "gn_gated_scan_forward": (c_int, [_P] * 11 + [c_int, c_longlong, c_longlong, c_int] + [c_longlong] * 4 + [c_int, _P]),
+    "gn_gated_scan_backward": (c_int, [_P] * 12 + [c_int, c_longlong, c_longlong, c_int] + [c_longlong] * 4 + [c_int, _P]),
+    "gn_gated_scan_step": (c_int, [_P] * 5 + [c_longlong, c_int, c_longlong, c_longlong, c_int, _P]),
 }
 
 

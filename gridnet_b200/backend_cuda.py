@@ -18,9 +18,11 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import gridnet_cuda, patch_loop
 from ._lib import activation_id, check, lib
+from .packed import empty_packed, stream_of
 
 
 def _assert_step_args(weight, bias, residual_scale, init_activations, block_size, gated):
@@ -264,6 +266,46 @@ class GridNormOp(torch.autograd.Function):
             check(lib.gn_norm_backward_f32(x.data_ptr(), gamma.data_ptr(), grad_y.data_ptr(), gx.data_ptr(),
                                            gg.data_ptr(), gb.data_ptr(), B, P, ctx.eps, ws.data_ptr(), ws.numel(),
                                            torch.cuda.current_stream().cuda_stream))
+        return gx, gg, gb, None
+
+
+class PackedGridNormOp(_Op):
+    """:class:`GridNormOp` whose backward pass reads x from 8 bits (:func:`pack_activations`, groups along the grid of a sample): a
+    quarter of the memory between the passes. The output is that of :class:`GridNormOp`; mean and deviation in the gradients are
+    those of x itself.
+
+    ``PackedGridNormOp.apply(x, gamma, beta, eps)``."""
+
+    @staticmethod
+    def forward(ctx, x, gamma, beta, eps: float = 1e-5):
+        assert x.shape[1:] == gamma.shape == beta.shape, f"{gamma.shape=} {beta.shape=} invalid for {x.shape=}"
+        _require_f32_cuda(x=x, gamma=gamma, beta=beta)
+        if not any(ctx.needs_input_grad[:3]):
+            return GridNormOp.apply(x, gamma, beta, eps)
+        B, P = x.shape[0], gamma.numel()
+        y = torch.empty_like(x)
+        packed = empty_packed(x.shape, 1, x.dtype, x.device)
+        stats = torch.empty(B, 2, dtype=torch.float32, device=x.device)
+        ws = _workspace(lib.gn_norm_packed_workspace_bytes(B, P), x.device)
+        with torch.cuda.device(x.device):
+            check(lib.gn_norm_forward_packed_f32(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), stats.data_ptr(),
+                                                 packed.codes.data_ptr(), packed.scales.data_ptr(), B, P, float(eps), ws.data_ptr(), ws.numel(),
+                                                 stream_of(x)))
+        ctx.save_for_backward(packed.codes, packed.scales, stats, gamma)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        codes, scales, stats, gamma = ctx.saved_tensors
+        grad_y = grad_y.contiguous()
+        B, P = codes.shape[0], gamma.numel()
+        gx, gg, gb = torch.empty_like(grad_y), torch.empty_like(gamma), torch.empty_like(gamma)
+        ws = _workspace(lib.gn_norm_packed_workspace_bytes(B, P), grad_y.device)
+        with torch.cuda.device(grad_y.device):
+            check(lib.gn_norm_backward_packed_f32(codes.data_ptr(), scales.data_ptr(), stats.data_ptr(), gamma.data_ptr(), grad_y.data_ptr(),
+                                                  gx.data_ptr(), gg.data_ptr(), gb.data_ptr(), B, P, ws.data_ptr(), ws.numel(),
+                                                  stream_of(grad_y)))
         return gx, gg, gb, None
 
 

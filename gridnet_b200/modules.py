@@ -13,7 +13,8 @@ from typing import Tuple
 import torch
 import torch.nn as nn
 
-from .backend_cuda import FusedGatedLoopTrainOp, FusedLoopTrainOp, GatedGridnetCudaOp, GridnetCudaOp, GridNormOp, outer_forward
+from .backend_cuda import FusedGatedLoopTrainOp, FusedLoopTrainOp, GatedGridnetCudaOp, GridnetCudaOp, GridNormOp, PackedGridNormOp, outer_forward
+from .packed import keeps_packed
 
 
 def _need_cuda(t: torch.Tensor, what: str) -> None:
@@ -69,7 +70,8 @@ class GatedGridnet(nn.Module):
 
 
 class GridNorm(nn.Module):
-    """``nn.LayerNorm(shape)`` over the whole grid with the same parameter names (weight, bias)."""
+    """``nn.LayerNorm(shape)`` over the whole grid with the same parameter names (weight, bias). Keeps its input in 8 bits for the
+    backward pass where :func:`keep_packed` says so."""
 
     def __init__(self, shape: Tuple[int, int, int], device, eps: float = 1e-5):
         super().__init__()
@@ -78,7 +80,8 @@ class GridNorm(nn.Module):
         self.bias = nn.Parameter(torch.zeros(*shape, device=device))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return GridNormOp.apply(x, self.weight, self.bias, self.eps)
+        op = PackedGridNormOp if keeps_packed() else GridNormOp
+        return op.apply(x, self.weight, self.bias, self.eps)
 
 
 class Readout(nn.Module):

@@ -1,0 +1,111 @@
+"""Activations in 8 bits: what a backward pass needs, kept in a quarter (float32) or half (16 bits) of the memory.
+
+Groups of 32 values of a row share a power of two 2^e, the smallest with ``|x| <= 125 * 2^e`` (e >= -126); a value is held as
+``x / 2^e`` rounded to a whole number, half to even, in a signed byte. 127, -127 and -128 are +inf, -inf and NaN, so what is not finite
+stays what it is and does not touch its neighbours. 33 bytes hold 32 values, and a value is off by at most half a 2^e. The
+reference has no counterpart: it keeps float32 between the passes.
+
+:func:`pack_activations` / :func:`unpack_activations` are the two directions; :func:`keep_packed` has the norms, scans, steps and loops of this
+package keep packed copies for their backward passes.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from ._lib import GridnetB200Error, check, lib
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # gn_dtype
+GROUP = 32
+
+_keep_packed = False
+
+
+def keep_packed(enabled: bool) -> bool:
+    """Whether differentiated calls keep 8-bit copies of activations for their backward pass, and compute their gradients at those copies:
+    the input of :class:`GridNorm`; gate and value of :func:`gated_scan`. Outputs are the
+    same with and without. Off by default. Holds for forward passes that start afterwards; a backward pass goes by what its forward
+    pass kept. Returns the previous setting."""
+    global _keep_packed
+    previous, _keep_packed = _keep_packed, bool(enabled)
+    return previous
+
+
+def keeps_packed() -> bool:
+    return _keep_packed
+
+
+class PackedActivations(NamedTuple):
+    """``codes``: a signed byte per value, in the shape of the tensor; ``scales``: a byte per group, the row dimensions and the groups of a
+    row; ``dtype``: the tensor's type."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    dtype: torch.dtype
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+
+def dtype_id(t: torch.Tensor, name: str) -> int:
+    if t.dtype not in DTYPES:
+        raise GridnetB200Error(f"unsupported dtype {t.dtype} of {name}: float32, bfloat16 and float16 only")
+    return DTYPES[t.dtype]
+
+
+def stream_of(t: torch.Tensor) -> int:
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def empty_packed(shape, rows: int, dtype: torch.dtype, device) -> PackedActivations:
+    """Room for the packed copy of a tensor of this shape, groups along what is behind its first ``rows`` dimensions."""
+    cols = 1
+    for n in shape[rows:]:
+        cols *= n
+    return PackedActivations(torch.empty(shape, dtype=torch.int8, device=device),
+                             torch.empty(*shape[:rows], (cols + GROUP - 1) // GROUP, dtype=torch.uint8, device=device), dtype)
+
+
+@torch.no_grad()
+def pack_activations(x: torch.Tensor, rows: int = 1) -> PackedActivations:
+    """The packed copy of ``x`` (float32, bfloat16 or float16, on a CUDA device). The first ``rows`` dimensions count rows (a sample, a
+    step of a sequence); groups of 32 run along the others taken together and never across a row's end."""
+    if not x.is_cuda:
+        raise GridnetB200Error("x must be a CUDA tensor")
+    dtype = dtype_id(x, "x")
+    assert 0 <= rows <= x.dim(), f"{rows=} invalid for {x.shape=}"
+    x = x.contiguous()
+    packed = empty_packed(x.shape, rows, x.dtype, x.device)
+    nrows = x.shape[:rows].numel()
+    with torch.cuda.device(x.device):
+        check(lib.gn_pack8(x.data_ptr(), packed.codes.data_ptr(), packed.scales.data_ptr(), nrows, x.numel() // nrows if nrows else 0, dtype,
+                           stream_of(x)))
+    return packed
+
+
+@torch.no_grad()
+def unpack_activations(packed: PackedActivations, out: torch.Tensor | None = None) -> torch.Tensor:
+    """What the packed copy stands for, in the tensor's own type or in ``out``'s (contiguous, any of the three types)."""
+    codes, scales, dtype = packed
+    for name, t in (("codes", codes), ("scales", scales)):
+        if not t.is_cuda:
+            raise GridnetB200Error(f"{name} must be a CUDA tensor")
+        if not t.is_contiguous():
+            raise GridnetB200Error(f"{name} must be contiguous")
+    assert codes.dtype == torch.int8 and scales.dtype == torch.uint8, f"{codes.dtype=} {scales.dtype=}: int8 and uint8"
+    assert codes.device == scales.device, f"mismatching devices: {codes.device=} {scales.device=}"
+    rows = scales.dim() - 1
+    nrows = codes.shape[:rows].numel()
+    cols = codes.shape[rows:].numel()
+    assert 0 <= rows <= codes.dim() and scales.shape == (*codes.shape[:rows], (cols + GROUP - 1) // GROUP), (
+        f"{scales.shape=} invalid for {codes.shape=}")
+    if out is None:
+        out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    assert out.shape == codes.shape, f"{out.shape=} invalid for {codes.shape=}"
+    assert out.device == codes.device, f"mismatching devices: {codes.device=} {out.device=}"
+    if not out.is_contiguous():
+        raise GridnetB200Error("out must be contiguous")
+    with torch.cuda.device(codes.device):
+        check(lib.gn_unpack8(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), nrows, cols, dtype_id(out, "out"), stream_of(codes)))
+    return out

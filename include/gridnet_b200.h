@@ -526,6 +526,56 @@ GN_API int gn_gated_loop_backward_f32(const float *weight, const float *bias, co
                                       float *ggamma, float *gbeta, float *gx, int B, int M, int N, int K, int inner, int outer, int act,
                                       void *workspace, size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------ activations in 8 bits
+ * No counterpart in the reference, which keeps nothing but float32 between a forward and a backward pass.
+ * Groups of 32 values of a row share a power of two 2^e: e the smallest whole number >= -126 with |x| <= 125 * 2^e for every finite x
+ * of the group. codes [rows][cols]: x / 2^e rounded to a whole number (half to even) as a signed byte in [-125, 125]; 127, -127 and -128
+ * are +inf, -inf and NaN (at e = 122 codes end at 63: what is finite stays so). scales [rows][ceil(cols / 32)]: e + 127 as a byte. A value is off by at most 2^(e-1). */
+typedef enum gn_dtype { GN_F32 = 0, GN_BF16 = 1, GN_F16 = 2 } gn_dtype;
+GN_API int gn_pack8(const void *x, void *codes, void *scales, long long rows, long long cols, int dtype, void *stream);
+/* A half that the codes put at 65536 comes out as 65504. */
+GN_API int gn_unpack8(const void *codes, const void *scales, void *x, long long rows, long long cols, int dtype, void *stream);
+
+/* gn_norm_forward_f32 that leaves what its backward pass needs in 8 bits: codes [B][P], scales [B][ceil(P / 32)] of x, and
+ * mean_rstd [B][2] (8-byte aligned) of x itself. The backward call computes the gradients with x as the codes give it. B = 0:
+ * zeros in ggamma and gbeta. workspace: 16-byte aligned. */
+GN_API size_t gn_norm_packed_workspace_bytes(int B, long long P);
+GN_API int gn_norm_forward_packed_f32(const float *x, const float *gamma, const float *beta, float *y, float *mean_rstd, void *codes,
+                                      void *scales, int B, long long P, float eps, void *workspace, size_t workspace_bytes, void *stream);
+GN_API int gn_norm_backward_packed_f32(const void *codes, const void *scales, const float *mean_rstd, const float *gamma, const float *gy,
+                                       float *gx, float *ggamma, float *gbeta, int B, long long P, void *workspace,
+                                       size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------ gated scan
+ * The update of the gated cell (gridnet/backend_torch.py:241-265) along a sequence, gate z and value u given, s the logistic function:
+ *     h_t = s(z_t) h_{t-1} + s(-z_t) u_t,   h_0 = state (NULL: zeros)
+ * in float32 whatever the type (gn_dtype) of gate, value and h. A step whose s(-z) is 0 does not look at its value, one whose s(z)
+ * is 0 not at the state.
+ *   dense    offsets NULL: n sequences of `steps` steps, total = n * steps;
+ *   ragged   offsets [n + 1] (device, not decreasing): sequence i is rows offsets[i] .. offsets[i + 1] - 1 of `total` rows. Rows of no
+ *            sequence get zeros, in h and in the gradients. Offsets outside of 0 .. total are taken as the nearest of the two.
+ * gate and value: `width` values side by side, any distance between steps and (dense) sequences, in elements; h, grad_h and the gradients
+ * [total][width]; state, last and their gradients [n][width] float32. last (may be NULL): the state behind the last step.
+ *
+ * For the backward pass either keep gate, value, state and `bounds` (gn_gated_scan_bounds_bytes; 0: none needed), or pass
+ * gate_codes, gate_scales, value_codes, value_scales ([total][width] and [total][ceil(width / 32)] bytes, format as above) to the
+ * forward call and keep those: the gradients are then those of the same recurrence at the unpacked gate and value, gate and value of the
+ * backward call are the codes, their strides are not looked at, and bounds is scratch of the same size. Without a backward pass all five may be NULL. grad_last,
+ * grad_state and state may be NULL. All gradients are overwritten. */
+GN_API size_t gn_gated_scan_bounds_bytes(int n, long long steps, long long total, int width, int dtype, int ragged);
+GN_API int gn_gated_scan_forward(const void *gate, const void *value, const float *state, const long long *offsets, void *h, float *last,
+                                 void *gate_codes, void *gate_scales, void *value_codes, void *value_scales, float *bounds, int n,
+                                 long long steps, long long total, int width, long long gate_seq, long long gate_step,
+                                 long long value_seq, long long value_step, int dtype, void *stream);
+GN_API int gn_gated_scan_backward(const void *gate, const void *value, const void *gate_scales, const void *value_scales,
+                                  const float *state, const long long *offsets, float *bounds, const void *grad_h,
+                                  const float *grad_last, void *grad_gate, void *grad_value, float *grad_state, int n, long long steps,
+                                  long long total, int width, long long gate_seq, long long gate_step, long long value_seq,
+                                  long long value_step, int dtype, void *stream);
+/* One step of `rows` sequences: h and out_state [rows][width]; out_state may be state. gate_row, value_row: distance of rows in elements. */
+GN_API int gn_gated_scan_step(const void *gate, const void *value, const float *state, void *h, float *out_state, long long rows, int width,
+                              long long gate_row, long long value_row, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
