@@ -2,8 +2,8 @@
 // function - the update of the gated grid's cell (gridnet/backend_torch.py:241-265) with gate z and value u given.
 //
 // Every step is an affine map of the state, and so is every run of steps: (A, H) stands for h -> A h + H, and
-// (A2, H2) after (A1, H1) is (A1 A2, A2 H1 + H2). A thread composes the steps it holds in registers, lanes compose by shuffles,
-// warps through shared memory, the CTAs of a cluster through each other's shared memory; then each thread knows the state ahead of its first step
+// (A2, H2) after (A1, H1) is (A1 A2, A2 H1 + H2). A thread composes the steps it holds in registers, warps compose through shared memory,
+// the CTAs of a cluster through each other's shared memory; then each thread knows the state ahead of its first step
 // and runs its steps again from registers. So gate and value are read once and h is written once, however long the sequence.
 //
 // Backward: c_t = gradient of h_{t-1} = a_t (g_t + c_{t+1}) is affine in c_{t+1}, from the end to the start, with the same A;
@@ -12,8 +12,12 @@
 // sequence is longer than what a CTA or cluster holds at a time, the forward pass has left the state at each such boundary.
 //
 // Steps whose n_t is 0 (gates from about 104 up, and +inf) do not look at their value, which may be NaN; steps whose a_t is 0 do not look
-// at the state. Anything else that is not finite stays in the state.
-// A product of many a_t must not become 0 by underflow, or it would hide such a state: it ends at the smallest normal number.
+// at the state. Anything else that is not finite stays in the state. Threads that hold such a step (the smaller of a_t and n_t is 0) go
+// through the steps with selections, all others with products and sums alone. A run with a reset has the sign bit in A (-0): an A that became
+// +0 by underflow still passes on a state that is not finite.
+//
+// A thread has two channels, so that a row is read 64 channels at a time and arithmetic is on pairs (f32x2); a warp has a run of steps
+// of its own, no lane has to know another lane's.
 #include <cooperative_groups.h>
 
 #include "kernels.h"
@@ -24,16 +28,9 @@ namespace gn {
 namespace cg = cooperative_groups;
 
 constexpr int kScanThreads = 256, kScanWarps = 8, kMaxCluster = 16;
-constexpr int kFwdSteps = 8, kBwdSteps = 4;  // steps that a thread holds
-
-// A row of a tile is 128 bytes: 8 lanes x 4 floats, 16 lanes x 4 values of 16 bits
-template <typename T>
-struct Lay {
-    static constexpr int kLanes = sizeof(T) == 4 ? 8 : 16;
-    static constexpr int kWidth = 4 * kLanes;        // channels of a slab
-    static constexpr int kRuns = 32 / kLanes;        // runs of steps side by side in a warp
-    static constexpr int kFwd = kScanWarps * kRuns * kFwdSteps, kBwd = kScanWarps * kRuns * kBwdSteps;  // steps of a CTA's tile
-};
+constexpr int kSlab = 64;                    // channels of a CTA
+constexpr int kSteps = 8;                    // steps that a thread holds
+constexpr int kTile = kScanWarps * kSteps;   // steps of a CTA
 
 struct Scan {
     const void *gate, *value;  // or codes
@@ -44,8 +41,8 @@ struct Scan {
     void *h;
     float *last;
     unsigned char *pack_gate, *pack_value, *pack_gate_scales, *pack_value_scales;
-    float *bounds;  // state ahead of every interval-th step
-    int interval;
+    float *bounds;  // state ahead of every interval-th step of a sequence
+    int interval;   // a power of two
     const void *gh;
     const float *glast;
     void *dgate, *dvalue;
@@ -76,88 +73,283 @@ __device__ __forceinline__ long long bound_row(const Scan &p, int seq, const Pla
     return s.first / p.interval + seq + k;  // a sequence has at most one boundary more than its rows have multiples of the interval
 }
 
-// logistic function of z and of -z, both to a few units in the last place
-__device__ __forceinline__ void gates(float z, float &a, float &n)
+// ---- pairs
+__device__ __forceinline__ unsigned long long bits2(float2 v)
+{
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+    return r;
+}
+__device__ __forceinline__ float2 pair2(unsigned long long v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b)
+{
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+    return pair2(r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b)
+{
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
+    return pair2(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
+{
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
+    return pair2(r);
+}
+__device__ __forceinline__ float2 two(float v) { return make_float2(v, v); }
+
+__device__ __forceinline__ float2 load2v(const float *p) { return *reinterpret_cast<const float2 *>(p); }
+__device__ __forceinline__ float2 load2v(const __nv_bfloat16 *p)
+{
+    const unsigned q = *reinterpret_cast<const unsigned *>(p);
+    return make_float2(__uint_as_float(q << 16), __uint_as_float(q & 0xffff0000u));
+}
+__device__ __forceinline__ float2 load2v(const __half *p) { return __half22float2(*reinterpret_cast<const __half2 *>(p)); }
+__device__ __forceinline__ void store2v(float *p, float2 v) { *reinterpret_cast<float2 *>(p) = v; }
+__device__ __forceinline__ void store2v(__nv_bfloat16 *p, float2 v) { *reinterpret_cast<__nv_bfloat162 *>(p) = __float22bfloat162_rn(v); }
+__device__ __forceinline__ void store2v(__half *p, float2 v) { *reinterpret_cast<__half2 *>(p) = __float22half2_rn(v); }
+// n: how many of the two are there (what is not reads as 0); vec: pairs lie on whole pairs' addresses
+template <typename T>
+__device__ __forceinline__ float2 load2(const T *p, bool vec, int n)
+{
+    if (vec && n == 2) return load2v(p);
+    return make_float2(n > 0 ? to_float<T>(p[0]) : 0.0f, n > 1 ? to_float<T>(p[1]) : 0.0f);
+}
+template <typename T>
+__device__ __forceinline__ void store2(T *p, bool vec, int n, float2 v)
+{
+    if (vec && n == 2) {
+        store2v(p, v);
+        return;
+    }
+    if (n > 0) p[0] = from_float<T>(v.x);
+    if (n > 1) p[1] = from_float<T>(v.y);
+}
+
+// e = exp(-z) for |z| < 80, as 2^t with what t lost by rounding put back: about three units in the last place
+__device__ __forceinline__ float2 exp_of_minus(float2 z)
+{
+    const float2 t = mul2(z, two(-1.4426950408889634f));
+    float2 e;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    // -z - t ln 2, with ln 2 in two parts: 0.693147182 - 1.90465421e-9
+    const float2 lost = fma2(t, two(1.90465421e-9f), fma2(t, two(-0.693147182f), mul2(z, two(-1.0f))));
+    return fma2(e, lost, e);
+}
+// 1 / w for 1 <= w <= 2^120: the approximation and a Newton step. Its error has a sign that is not even, which a memory of thousands of steps
+// would add up (8 x 2048 x 4096 without the step, gradient of the state: 1.4e-6 off in the 2-norm; the plain form is 2.7e-7 off).
+__device__ __forceinline__ float2 reciprocal(float2 w)
+{
+    float2 r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(w.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(w.y));
+    return fma2(r, fma2(mul2(w, two(-1.0f)), r, two(1.0f)), r);
+}
+// s(z) and s(-z). Gates from kFar on, and what is behind the end, go through gates_any.
+constexpr float kFar = 80.0f;
+__device__ __forceinline__ void gates(float2 z, float2 &a, float2 &n)
+{
+    const float2 e = exp_of_minus(z);
+    a = reciprocal(add2(e, two(1.0f)));
+    n = mul2(e, a);
+}
+// For every z: the smaller from exp(-|z|), which is 0 from |z| = 104 on, the larger as 1 less it
+__device__ __forceinline__ float2 gate_any(float z)  // (s(z), s(-z))
 {
     const float e = expf(-fabsf(z));
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    const float q = e * r;
-    a = z < 0.0f ? q : r;
-    n = z < 0.0f ? r : q;
+    const float q = e / (1.0f + e), p = 1.0f - q;
+    return z < 0.0f ? make_float2(q, p) : make_float2(p, q);
 }
-__device__ __forceinline__ float through(float a, float h, float b) { return a == 0.0f ? b : fmaf(a, h, b); }
+__device__ __forceinline__ void gates_any(float2 z, float2 &a, float2 &n)
+{
+    const float2 x = gate_any(z.x), y = gate_any(z.y);
+    a = make_float2(x.x, y.x);
+    n = make_float2(x.y, y.y);
+}
+
+// ---- maps of runs. The sign bit of A: the run has a reset, what was before it does not show
+__device__ __forceinline__ bool resets(float a) { return __float_as_int(a) < 0; }
+__device__ __forceinline__ float through(float a, float h, float b) { return resets(a) ? b : fmaf(a, h, b); }
+__device__ __forceinline__ float2 through(float2 a, float2 h, float2 b) { return make_float2(through(a.x, h.x, b.x), through(a.y, h.y, b.y)); }
 __device__ __forceinline__ float product(float a, float b)
 {
-    const float p = a * b;
-    return a == 0.0f || b == 0.0f ? 0.0f : (p < FLT_MIN ? FLT_MIN : p);  // NaN stays
+    return __uint_as_float(__float_as_uint(a * b) | ((__float_as_uint(a) | __float_as_uint(b)) & 0x80000000u));
 }
+__device__ __forceinline__ float2 product(float2 a, float2 b) { return make_float2(product(a.x, b.x), product(a.y, b.y)); }
+// one step with a_t = 0 or n_t = 0 among those of the thread
+__device__ __forceinline__ float after(float a, float h, float b) { return a == 0.0f ? b : fmaf(a, h, b); }
+__device__ __forceinline__ float2 after(float2 a, float2 h, float2 b) { return make_float2(after(a.x, h.x, b.x), after(a.y, h.y, b.y)); }
+__device__ __forceinline__ float2 more(float2 A, float2 a)
+{
+    return make_float2(a.x == 0.0f ? -0.0f : product(A.x, a.x), a.y == 0.0f ? -0.0f : product(A.y, a.y));
+}
+__device__ __forceinline__ float2 looked_at(float2 n, float2 v) { return make_float2(n.x == 0.0f ? 0.0f : v.x, n.y == 0.0f ? 0.0f : v.y); }
 
 // Rows outside of every sequence of a ragged call: zeros
 template <typename T>
 __device__ void clear_rows(const Scan &p, T *x, int slab, int rank)
 {
-    using L = Lay<T>;
     const long long lo = min(max(p.offsets[0], 0LL), p.total), hi = min(max(p.offsets[p.n], lo), p.total);
-    const int lr = threadIdx.x % L::kLanes, ch = slab * L::kWidth + lr * 4, nch = min(4, max(0, p.width - ch));
-    const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int rows = kScanThreads / L::kLanes;
-    for (long long i = (long long)rank * rows + threadIdx.x / L::kLanes; i < lo + p.total - hi; i += (long long)rows * p.cluster) {
+    const int ch = slab * kSlab + (threadIdx.x & 31) * 2, nch = min(2, max(0, p.width - ch));
+    for (long long i = (long long)rank * kScanWarps + (threadIdx.x >> 5); i < lo + p.total - hi; i += (long long)kScanWarps * p.cluster) {
         const long long row = i < lo ? i : i - lo + hi;
-        store4(x + row * p.width + ch, p.vec, nch, zero);
+        store2(x + row * p.width + ch, p.vec, nch, two(0.0f));
     }
 }
 
-template <typename T, int S>
-__device__ __forceinline__ void load_rows(const T *x, long long step, bool vec, int cnt, int nch, float (&v)[S][4])
+// Rows behind the end have `end`. Every load stands without a condition of its own (rows behind the end read the last one again): loads under
+// conditions are waited for one by one, 600 cycles each.
+template <typename T>
+__device__ __forceinline__ void load_rows(const T *x, long long step, bool vec, int cnt, int nch, float end, float2 (&v)[kSteps])
 {
-    if (vec && nch == 4) {
+    if (cnt == kSteps && vec && nch == 2) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            if (s < cnt)
-                load4v(x + s * step, v[s]);
-            else
-                v[s][0] = v[s][1] = v[s][2] = v[s][3] = 0.0f;
+        for (int s = 0; s < kSteps; ++s) v[s] = load2v(x + s * step);
+        return;
+    }
+    if (cnt > 0 && nch > 0) {
+        T one[kSteps], other[kSteps];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const T *const at = x + min(s, cnt - 1) * step;
+            one[s] = at[0];
+            other[s] = at[nch - 1];
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) v[s] = s < cnt ? make_float2(to_float<T>(one[s]), nch > 1 ? to_float<T>(other[s]) : 0.0f) : two(end);
+    } else {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) v[s] = s < cnt ? two(0.0f) : two(end);
+    }
+}
+
+__device__ __forceinline__ void load_packed(const unsigned char *codes, const unsigned char *scales, long long row, int width, int ch, bool vec,
+                                            int cnt, int nch, float end, float2 (&v)[kSteps])
+{
+    if (cnt <= 0 || nch <= 0) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) v[s] = s < cnt ? two(0.0f) : two(end);
+        return;
+    }
+    const int per_row = (width + kPackGroup - 1) / kPackGroup;
+    const unsigned char *const c = codes + row * width + ch, *const g = scales + row * per_row + ch / kPackGroup;
+    unsigned w[kSteps], sc[kSteps];
+    if (vec && nch == 2) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const long long i = min(s, cnt - 1);
+            w[s] = *reinterpret_cast<const unsigned short *>(c + i * width);
+            sc[s] = g[i * per_row];
         }
     } else {
 #pragma unroll
-        for (int s = 0; s < S; ++s) load4(x + s * step, false, s < cnt ? nch : 0, v[s]);
+        for (int s = 0; s < kSteps; ++s) {
+            const long long i = min(s, cnt - 1);
+            w[s] = c[i * width] | (nch > 1 ? (unsigned)c[i * width + 1] << 8 : 0u);
+            sc[s] = g[i * per_row];
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; s += 2) {  // the codes of two steps in a word
+        float f[4];
+        unpack4(w[s] | w[s + 1] << 16, 1.0f, f);
+        v[s] = s < cnt ? make_float2(f[0] * pack_step(sc[s]), f[1] * pack_step(sc[s])) : two(end);
+        v[s + 1] = s + 1 < cnt ? make_float2(f[2] * pack_step(sc[s + 1]), f[3] * pack_step(sc[s + 1])) : two(end);
     }
 }
 
-template <int S>
-__device__ __forceinline__ void load_packed(const unsigned char *codes, const unsigned char *scales, long long row, int width, int ch, bool vec,
-                                            int cnt, int nch, float (&v)[S][4])
+// Packs the rows that a warp holds, 8 of them, 64 channels each: two groups a row, a half of the warp's lanes a group. The largest
+// of a group is found for all rows at a time, halving the rows that a lane still looks at: lane l of a half ends up with row l & 7.
+__device__ __forceinline__ void pack_rows(const float2 (&v)[kSteps], unsigned char *codes, unsigned char *scales, long long row, int width, int ch,
+                                          bool vec, int cnt, int nch)
 {
-    const int per_row = (width + kPackGroup - 1) / kPackGroup;
-    unsigned w[S], sc[S];
+    const int lane = threadIdx.x & 31;
+    unsigned m[kSteps];
+    bool again = false;
+    for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-        const bool there = s < cnt && nch > 0;
-        w[s] = there ? load_codes(codes + (row + s) * width + ch, vec, nch) : 0u;
-        sc[s] = there ? scales[(row + s) * per_row + ch / kPackGroup] : 127u;
+        for (int s = 0; s < kSteps; ++s) {
+            const unsigned x = magnitude_bits(v[s].x), y = magnitude_bits(v[s].y);
+            m[s] = pass ? max(bits_finite(x) ? x : 0u, bits_finite(y) ? y : 0u) : max(x, y);
+            if (s >= cnt) m[s] = 0u;
+        }
+#pragma unroll
+        for (int h = kSteps / 2; h > 0; h >>= 1)
+#pragma unroll
+            for (int s = 0; s < h; ++s) {
+                const bool upper = lane & h;
+                const unsigned give = upper ? m[s] : m[s + h], keep = upper ? m[s + h] : m[s];
+                m[s] = max(keep, __shfl_xor_sync(0xffffffffu, give, h));
+            }
+        m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], 8));
+        if (pass == 0) {
+            again = __any_sync(0xffffffffu, m[0] > kPackLargest);
+            if (!again) break;
+        }
     }
+    const unsigned scale = pack_scale(m[0]);
+    const int per_row = (width + kPackGroup - 1) / kPackGroup, group = ch / kPackGroup;
+    if ((lane & 15) < cnt && group < per_row) scales[(row + (lane & 15)) * per_row + group] = (unsigned char)scale;
+    unsigned char *at = codes + row * width + ch;
 #pragma unroll
-    for (int s = 0; s < S; ++s) unpack4(w[s], pack_step(sc[s]), v[s]);
+    for (int s = 0; s < kSteps; ++s, at += width) {
+        const unsigned sc = __shfl_sync(0xffffffffu, scale, (lane & 16) | s);
+        unsigned a, b;
+        if (again) {
+            a = pack_code_any(v[s].x, sc);
+            b = pack_code_any(v[s].y, sc);
+        } else {
+            const float inv = pack_inverse(sc);
+            a = pack_code(v[s].x, inv);
+            b = pack_code(v[s].y, inv);
+        }
+        if (s < cnt) {
+            if (vec && nch == 2) {
+                *reinterpret_cast<unsigned short *>(at) = (unsigned short)__byte_perm(a, b, 0x0040);
+            } else {
+                if (nch > 0) at[0] = (unsigned char)a;
+                if (nch > 1) at[1] = (unsigned char)b;
+            }
+        }
+    }
 }
 
-// What a warp's, a CTA's steps amount to, per channel; two copies, so that one barrier lies between writing and writing again
-template <typename T, int VALUES>
-struct Exchange {
-    float warp[2][kScanWarps][VALUES][Lay<T>::kWidth];
-    float rank[2][kMaxCluster][VALUES][Lay<T>::kWidth];
-};
+__device__ __forceinline__ float farthest(const float2 (&z)[kSteps])  // |z|; NaN does not count
+{
+    float m = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) m = fmaxf(m, fmaxf(fabsf(z[s].x), fabsf(z[s].y)));
+    return m;
+}
 
-__device__ __forceinline__ void get4(const float *p, float (&v)[4]) { load4v(p, v); }
+// What a warp's, a CTA's steps amount to: (A, H) and, backward, (A, C) of a channel pair; two copies, so that one barrier lies between
+// writing and writing again
+__device__ __forceinline__ float4 map_of(float2 A, float2 H) { return make_float4(A.x, A.y, H.x, H.y); }
+__device__ __forceinline__ float2 factor(float4 m) { return make_float2(m.x, m.y); }
+__device__ __forceinline__ float2 term(float4 m) { return make_float2(m.z, m.w); }
+__device__ __forceinline__ float2 through(float4 m, float2 h) { return through(factor(m), h, term(m)); }
+__device__ __forceinline__ float2 straight(float4 m, float2 h) { return fma2(factor(m), h, term(m)); }  // no resets
+template <int WAYS>
+struct Exchange {
+    float4 warp[2][WAYS][kScanWarps][32];
+    float4 rank[2][WAYS][kMaxCluster][32];
+};
 
 // ------------------------------------------------------------------ forward
 // PACKED: gate and value are codes, and only the states at the boundaries are wanted. KEEP: packs gate and value.
 template <typename T, bool PACKED, bool KEEP>
-__global__ void __launch_bounds__(kScanThreads, 2) scan_forward_k(const Scan p)
+__global__ void __launch_bounds__(kScanThreads, sizeof(T) == 2 && !KEEP ? 3 : 2) scan_forward_k(const Scan p)
 {
-    using L = Lay<T>;
-    constexpr int S = kFwdSteps;
-    __shared__ __align__(16) Exchange<T, 2> ex;
+    __shared__ __align__(16) Exchange<1> ex;
     const int rank = blockIdx.x % p.cluster, id = blockIdx.x / p.cluster;
     const int slab = id % p.slabs, seq = id / p.slabs;
     if (seq >= p.n) {
@@ -165,147 +357,138 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_forward_k(const Scan p)
         return;
     }
     const Place q = sequence(p, seq);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lr = lane % L::kLanes, run = lane / L::kLanes;
-    const int ch = slab * L::kWidth + lr * 4, nch = min(4, max(0, p.width - ch));
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int ch = slab * kSlab + lane * 2, nch = min(2, max(0, p.width - ch));
     const bool vec = p.vec;
-    float carry[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (p.state) load4(p.state + (long long)seq * p.width + ch, vec, nch, carry);
+    const long long state_at = (long long)seq * p.width + ch;
+    float2 carry = two(0.0f);
+    if (p.state) carry = load2(p.state + state_at, vec, nch);
     if (q.len == 0) {
-        if (!PACKED && p.last && rank == 0 && threadIdx.x < L::kLanes) store4(p.last + (long long)seq * p.width + ch, vec, nch, carry);
+        if (!PACKED && p.last && rank == 0 && warp == 0) store2(p.last + state_at, vec, nch, carry);
         return;
     }
     if (PACKED && q.len <= p.interval) return;  // the whole cluster
-    const long long gate_at = p.offsets ? q.first * p.gate_step : seq * p.gate_seq;
-    const long long value_at = p.offsets ? q.first * p.value_step : seq * p.value_seq;
+    const long long held = (long long)kTile * p.cluster;
+    long long t0 = (long long)rank * kTile + warp * kSteps;
+    const T *gate = (const T *)p.gate + (p.offsets ? q.first * p.gate_step : seq * p.gate_seq) + t0 * p.gate_step + ch;
+    const T *value = (const T *)p.value + (p.offsets ? q.first * p.value_step : seq * p.value_seq) + t0 * p.value_step + ch;
     // a CTA's shared memory may be written to by others once it runs: waited for ahead of the first such store
     if (p.cluster > 1) cg::this_cluster().sync();
-    int par = 0;
-    for (long long base = 0; base < q.len; base += (long long)L::kFwd * p.cluster, par ^= 1) {
-        const long long t0 = base + (long long)rank * L::kFwd + (warp * L::kRuns + run) * S;
-        const int cnt = (int)min((long long)S, max(0LL, q.len - t0));
-        float a[S][4], b[S][4];
+    const float inf = __uint_as_float(0x7f800000u);
+    const bool pairs = vec && nch == 2;
+    bool asked = false;  // the steps in hand have been asked for a tile ahead
+    float2 za[kSteps], ua[kSteps];
+    for (int par = 0; t0 - (long long)rank * kTile - warp * kSteps < q.len; t0 += held, par ^= 1) {
+        const int cnt = (int)min((long long)kSteps, max(0LL, q.len - t0));
+        // a step behind the end holds the state
+        float2 a[kSteps], b[kSteps];
         if (PACKED) {
-            load_packed<S>((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, a);
-            load_packed<S>((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, b);
+            load_packed((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, inf, a);
+            load_packed((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, 0.0f, b);
         } else {
-            load_rows<T, S>((const T *)p.gate + gate_at + t0 * p.gate_step + ch, p.gate_step, vec, cnt, nch, a);
-            load_rows<T, S>((const T *)p.value + value_at + t0 * p.value_step + ch, p.value_step, vec, cnt, nch, b);
-        }
-        if (KEEP) {
-            const int per_row = (p.width + kPackGroup - 1) / kPackGroup;
+            if (!asked) {
+                load_rows<T>(gate, p.gate_step, vec, cnt, nch, inf, za);
+                load_rows<T>(value, p.value_step, vec, cnt, nch, 0.0f, ua);
+            }
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-                unsigned sg, sv;
-                const unsigned wg = pack_group(a[s], sg), wv = pack_group(b[s], sv);
-                if (s < cnt) {
-                    const long long row = q.first + t0 + s, at = row * p.width + ch;
-                    store_codes(p.pack_gate + at, vec, nch, wg);
-                    store_codes(p.pack_value + at, vec, nch, wv);
-                    if ((lr & 7) == 0 && nch > 0) {
-                        p.pack_gate_scales[row * per_row + ch / kPackGroup] = (unsigned char)sg;
-                        p.pack_value_scales[row * per_row + ch / kPackGroup] = (unsigned char)sv;
-                    }
+            for (int s = 0; s < kSteps; ++s) {
+                a[s] = za[s];
+                b[s] = ua[s];
+            }
+        }
+        if constexpr (KEEP) {
+            pack_rows(a, p.pack_gate, p.pack_gate_scales, q.first + t0, p.width, ch, vec, cnt, nch);
+            pack_rows(b, p.pack_value, p.pack_value_scales, q.first + t0, p.width, ch, vec, cnt, nch);
+        }
+        const bool special = farthest(a) >= kFar;
+        float2 A = two(1.0f), H = two(0.0f);
+        if (!special) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                float2 w, n;
+                gates(a[s], w, n);
+                a[s] = w;
+                b[s] = mul2(n, b[s]);
+                H = fma2(w, H, b[s]);
+                A = mul2(A, w);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                float2 w, n;
+                gates_any(a[s], w, n);
+                a[s] = w;
+                b[s] = mul2(n, looked_at(n, b[s]));
+                H = after(w, H, b[s]);
+                A = more(A, w);
+            }
+        }
+        if (!PACKED) {
+            gate += held * p.gate_step;
+            value += held * p.value_step;
+            asked = pairs && t0 + held + kSteps <= q.len;
+            if (asked) {
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) {
+                    za[s] = load2v(gate + s * p.gate_step);
+                    ua[s] = load2v(value + s * p.value_step);
                 }
             }
         }
-        float A[4], H[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            A[i] = 1.0f;
-            H[i] = 0.0f;
-#pragma unroll
-            for (int s = 0; s < S; ++s) {
-                float w, n;
-                gates(a[s][i], w, n);
-                a[s][i] = s < cnt ? w : 1.0f;
-                b[s][i] = s < cnt && n != 0.0f ? n * b[s][i] : 0.0f;
-                H[i] = through(a[s][i], H[i], b[s][i]);
-                A[i] = product(A[i], a[s][i]);
-            }
-        }
-        // runs before this one in the warp
-#pragma unroll
-        for (int d = 1; d < L::kRuns; d *= 2)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float pa = __shfl_up_sync(0xffffffffu, A[i], d * L::kLanes), ph = __shfl_up_sync(0xffffffffu, H[i], d * L::kLanes);
-                if (run >= d) {
-                    H[i] = through(A[i], ph, H[i]);
-                    A[i] = product(pa, A[i]);
-                }
-            }
-        if (run == L::kRuns - 1) {
-            store4v(&ex.warp[par][warp][0][lr * 4], A);
-            store4v(&ex.warp[par][warp][1][lr * 4], H);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            A[i] = __shfl_up_sync(0xffffffffu, A[i], L::kLanes);
-            H[i] = __shfl_up_sync(0xffffffffu, H[i], L::kLanes);
-            if (run == 0) {
-                A[i] = 1.0f;
-                H[i] = 0.0f;
-            }
-        }
-        __syncthreads();
-        float h[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = carry[i];
+        ex.warp[par][0][warp][lane] = map_of(A, H);
+        const bool any = __syncthreads_or(special);
+        float2 h = carry;
         if (p.cluster > 1) {
             cg::cluster_group cluster = cg::this_cluster();
-            if (warp < 1 && run == 0) {
-                float ta[4] = {1.0f, 1.0f, 1.0f, 1.0f}, th[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                for (int w = 0; w < kScanWarps; ++w) {
-                    float wa[4], wh[4];
-                    get4(&ex.warp[par][w][0][lr * 4], wa);
-                    get4(&ex.warp[par][w][1][lr * 4], wh);
+            // every warp composes the CTA's steps and tells every eighth CTA
+            float2 ta = two(1.0f), th = two(0.0f);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        th[i] = through(wa[i], th[i], wh[i]);
-                        ta[i] = product(ta[i], wa[i]);
-                    }
-                }
-                for (int r = 0; r < p.cluster; ++r) {
-                    store4v(cluster.map_shared_rank(&ex.rank[par][rank][0][lr * 4], r), ta);
-                    store4v(cluster.map_shared_rank(&ex.rank[par][rank][1][lr * 4], r), th);
-                }
+            for (int w = 0; w < kScanWarps; ++w) {
+                const float4 m = ex.warp[par][0][w][lane];
+                th = through(m, th);
+                ta = product(ta, factor(m));
             }
+            for (int r = warp; r < p.cluster; r += kScanWarps) *cluster.map_shared_rank(&ex.rank[par][0][rank][lane], r) = map_of(ta, th);
             cluster.sync();
             for (int r = 0; r < p.cluster; ++r) {
-                float ra[4], rh[4];
-                get4(&ex.rank[par][r][0][lr * 4], ra);
-                get4(&ex.rank[par][r][1][lr * 4], rh);
+                if (r == rank) h = carry;
+                carry = through(ex.rank[par][0][r][lane], carry);
+            }
+            for (int w = 0; w < warp; ++w) h = through(ex.warp[par][0][w][lane], h);
+        } else if (!any) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (r == rank) h[i] = carry[i];
-                    carry[i] = through(ra[i], carry[i], rh[i]);
-                }
+            for (int w = 0; w < kScanWarps; ++w) {
+                if (w == warp) h = carry;
+                carry = straight(ex.warp[par][0][w][lane], carry);
+            }
+        } else {
+#pragma unroll
+            for (int w = 0; w < kScanWarps; ++w) {
+                if (w == warp) h = carry;
+                carry = through(ex.warp[par][0][w][lane], carry);
             }
         }
-        for (int w = 0; w < kScanWarps; ++w) {
-            float wa[4], wh[4];
-            if (p.cluster > 1 && w >= warp) break;
-            get4(&ex.warp[par][w][0][lr * 4], wa);
-            get4(&ex.warp[par][w][1][lr * 4], wh);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (w < warp) h[i] = through(wa[i], h[i], wh[i]);
-                if (p.cluster == 1) carry[i] = through(wa[i], carry[i], wh[i]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = through(A[i], h[i], H[i]);
-        if (p.bounds && cnt > 0 && t0 > 0 && t0 % p.interval == 0)
-            store4(p.bounds + bound_row(p, seq, q, t0 / p.interval) * p.width + ch, vec, nch, h);
+        // intervals are multiples of 64 steps: boundaries lie at the start of a thread's steps
+        if (p.bounds && cnt > 0 && t0 > 0 && (t0 & (p.interval - 1)) == 0)
+            store2(p.bounds + bound_row(p, seq, q, t0 / p.interval) * p.width + ch, vec, nch, h);
         if (!PACKED) {
-            T *out = (T *)p.h + (q.first + t0) * p.width + ch;
+            T *const out = (T *)p.h + (q.first + t0) * p.width + ch;
+            if (!special) {
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
+                for (int s = 0; s < kSteps; ++s) a[s] = h = fma2(a[s], h, b[s]);
+            } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) h[i] = through(a[s][i], h[i], b[s][i]);
-                if (s < cnt) store4(out + (long long)s * p.width, vec, nch, h);
+                for (int s = 0; s < kSteps; ++s) a[s] = h = after(a[s], h, b[s]);
             }
-            if (p.last && cnt > 0 && t0 + cnt == q.len) store4(p.last + (long long)seq * p.width + ch, vec, nch, h);
+            if (pairs && cnt == kSteps) {
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) store2v(out + (long long)s * p.width, a[s]);
+            } else {
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s)
+                    if (s < cnt) store2(out + (long long)s * p.width, vec, nch, a[s]);
+            }
+            if (p.last && cnt > 0 && t0 + cnt == q.len) store2(p.last + state_at, vec, nch, h);
         }
     }
 }
@@ -314,9 +497,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_forward_k(const Scan p)
 template <typename T, bool PACKED>
 __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
 {
-    using L = Lay<T>;
-    constexpr int S = kBwdSteps;
-    __shared__ __align__(16) Exchange<T, 3> ex;
+    __shared__ __align__(16) Exchange<2> ex;
     const int rank = blockIdx.x % p.cluster, id = blockIdx.x / p.cluster;
     const int slab = id % p.slabs, seq = id / p.slabs;
     if (seq >= p.n) {
@@ -325,185 +506,151 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
         return;
     }
     const Place q = sequence(p, seq);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, lr = lane % L::kLanes, run = lane / L::kLanes;
-    const int ch = slab * L::kWidth + lr * 4, nch = min(4, max(0, p.width - ch));
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int ch = slab * kSlab + lane * 2, nch = min(2, max(0, p.width - ch));
     const bool vec = p.vec;
     const long long state_at = (long long)seq * p.width + ch;
-    float carry[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // gradient of the state behind the steps in hand
-    if (p.glast) load4(p.glast + state_at, vec, nch, carry);
-    const long long gate_at = p.offsets ? q.first * p.gate_step : seq * p.gate_seq;
-    const long long value_at = p.offsets ? q.first * p.value_step : seq * p.value_seq;
-    const long long held = (long long)L::kBwd * p.cluster;  // == p.interval
+    float2 carry = two(0.0f);  // gradient of the state behind the steps in hand
+    if (p.glast) carry = load2(p.glast + state_at, vec, nch);
+    const T *const gate = (const T *)p.gate + (p.offsets ? q.first * p.gate_step : seq * p.gate_seq) + ch;
+    const T *const value = (const T *)p.value + (p.offsets ? q.first * p.value_step : seq * p.value_seq) + ch;
+    const long long held = (long long)kTile * p.cluster;  // == p.interval
+    int par = 0;
     // a CTA's shared memory may be written to by others once it runs: waited for ahead of the first such store
     if (p.cluster > 1) cg::this_cluster().sync();
-    int par = 0;
+    const float inf = __uint_as_float(0x7f800000u);
     for (long long k = (q.len + held - 1) / held - 1; k >= 0; --k, par ^= 1) {
-        const long long t0 = k * held + (long long)rank * L::kBwd + (warp * L::kRuns + run) * S;
-        const int cnt = (int)min((long long)S, max(0LL, q.len - t0));
-        float z[S][4], u[S][4], g[S][4], h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const long long t0 = k * held + (long long)rank * kTile + warp * kSteps;
+        const int cnt = (int)min((long long)kSteps, max(0LL, q.len - t0));
+        // a step behind the end holds the state and has no gradient of its own
+        float2 a[kSteps], n[kSteps], u[kSteps], g[kSteps], h = two(0.0f);
         if (PACKED) {
-            load_packed<S>((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, z);
-            load_packed<S>((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, u);
+            load_packed((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, inf, a);
+            load_packed((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, 0.0f, u);
         } else {
-            load_rows<T, S>((const T *)p.gate + gate_at + t0 * p.gate_step + ch, p.gate_step, vec, cnt, nch, z);
-            load_rows<T, S>((const T *)p.value + value_at + t0 * p.value_step + ch, p.value_step, vec, cnt, nch, u);
+            load_rows<T>(gate + t0 * p.gate_step, p.gate_step, vec, cnt, nch, inf, a);
+            load_rows<T>(value + t0 * p.value_step, p.value_step, vec, cnt, nch, 0.0f, u);
         }
-        load_rows<T, S>((const T *)p.gh + (q.first + t0) * p.width + ch, p.width, vec, cnt, nch, g);
+        load_rows<T>((const T *)p.gh + (q.first + t0) * p.width + ch, p.width, vec, cnt, nch, 0.0f, g);
         if (k > 0)
-            load4(p.bounds + bound_row(p, seq, q, k) * p.width + ch, vec, nch, h);
+            h = load2(p.bounds + bound_row(p, seq, q, k) * p.width + ch, vec, nch);
         else if (p.state)
-            load4(p.state + state_at, vec, nch, h);
-        float A[4], H[4], C[4], a[S][4], n[S][4];
+            h = load2(p.state + state_at, vec, nch);
+        float2 A = two(1.0f), H = two(0.0f), C = two(0.0f);
+        const bool special = farthest(a) >= kFar;
+        if (!special) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            A[i] = 1.0f;
-            H[i] = C[i] = 0.0f;
-#pragma unroll
-            for (int s = 0; s < S; ++s) {
-                gates(z[s][i], a[s][i], n[s][i]);
-                if (s >= cnt) {
-                    a[s][i] = 1.0f;
-                    n[s][i] = 0.0f;
-                }
-                H[i] = through(a[s][i], H[i], n[s][i] == 0.0f ? 0.0f : n[s][i] * u[s][i]);
-                A[i] = product(A[i], a[s][i]);
+            for (int s = 0; s < kSteps; ++s) {
+                float2 w;
+                gates(a[s], w, n[s]);
+                a[s] = w;
+                H = fma2(w, H, mul2(n[s], u[s]));
+                A = mul2(A, w);
             }
 #pragma unroll
-            for (int s = S - 1; s >= 0; --s) C[i] = a[s][i] == 0.0f ? 0.0f : a[s][i] * (g[s][i] + C[i]);
+            for (int s = kSteps - 1; s >= 0; --s) C = mul2(a[s], add2(g[s], C));
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                float2 w;
+                gates_any(a[s], w, n[s]);
+                a[s] = w;
+                u[s] = looked_at(n[s], u[s]);
+                H = after(w, H, mul2(n[s], u[s]));
+                A = more(A, w);
+            }
+#pragma unroll
+            for (int s = kSteps - 1; s >= 0; --s) C = looked_at(a[s], mul2(a[s], add2(g[s], C)));
         }
-        // exclusive, before (A, H) and behind (B, C) this run in the warp
-        float B[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) B[i] = A[i];
-#pragma unroll
-        for (int d = 1; d < L::kRuns; d *= 2)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float pa = __shfl_up_sync(0xffffffffu, A[i], d * L::kLanes), ph = __shfl_up_sync(0xffffffffu, H[i], d * L::kLanes);
-                const float nb = __shfl_down_sync(0xffffffffu, B[i], d * L::kLanes), nc = __shfl_down_sync(0xffffffffu, C[i], d * L::kLanes);
-                if (run >= d) {
-                    H[i] = through(A[i], ph, H[i]);
-                    A[i] = product(pa, A[i]);
-                }
-                if (run + d < L::kRuns) {
-                    C[i] = through(B[i], nc, C[i]);
-                    B[i] = product(nb, B[i]);
-                }
-            }
-        if (run == L::kRuns - 1) {
-            store4v(&ex.warp[par][warp][0][lr * 4], A);
-            store4v(&ex.warp[par][warp][1][lr * 4], H);
-        }
-        if (run == 0) store4v(&ex.warp[par][warp][2][lr * 4], C);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            A[i] = __shfl_up_sync(0xffffffffu, A[i], L::kLanes);
-            H[i] = __shfl_up_sync(0xffffffffu, H[i], L::kLanes);
-            B[i] = __shfl_down_sync(0xffffffffu, B[i], L::kLanes);
-            C[i] = __shfl_down_sync(0xffffffffu, C[i], L::kLanes);
-            if (run == 0) {
-                A[i] = 1.0f;
-                H[i] = 0.0f;
-            }
-            if (run == L::kRuns - 1) {
-                B[i] = 1.0f;
-                C[i] = 0.0f;
-            }
-        }
-        __syncthreads();
-        float c[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = carry[i];
+        ex.warp[par][0][warp][lane] = map_of(A, H);
+        ex.warp[par][1][warp][lane] = map_of(A, C);
+        const bool any = __syncthreads_or(special);
+        float2 c = carry;
         if (p.cluster > 1) {
             cg::cluster_group cluster = cg::this_cluster();
-            if (warp == 0 && run == 0) {
-                float ta[4] = {1.0f, 1.0f, 1.0f, 1.0f}, th[4] = {0.0f, 0.0f, 0.0f, 0.0f}, tc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                for (int w = 0; w < kScanWarps; ++w) {
-                    float wa[4], wh[4], wc[4], va[4];
-                    get4(&ex.warp[par][w][0][lr * 4], wa);
-                    get4(&ex.warp[par][w][1][lr * 4], wh);
-                    get4(&ex.warp[par][kScanWarps - 1 - w][0][lr * 4], va);
-                    get4(&ex.warp[par][kScanWarps - 1 - w][2][lr * 4], wc);
+            float2 ta = two(1.0f), th = two(0.0f), tc = two(0.0f);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        th[i] = through(wa[i], th[i], wh[i]);
-                        ta[i] = product(ta[i], wa[i]);
-                        tc[i] = through(va[i], tc[i], wc[i]);
-                    }
-                }
-                for (int r = 0; r < p.cluster; ++r) {
-                    store4v(cluster.map_shared_rank(&ex.rank[par][rank][0][lr * 4], r), ta);
-                    store4v(cluster.map_shared_rank(&ex.rank[par][rank][1][lr * 4], r), th);
-                    store4v(cluster.map_shared_rank(&ex.rank[par][rank][2][lr * 4], r), tc);
-                }
+            for (int w = 0; w < kScanWarps; ++w) {
+                const float4 m = ex.warp[par][0][w][lane];
+                th = through(m, th);
+                ta = product(ta, factor(m));
+                tc = through(ex.warp[par][1][kScanWarps - 1 - w][lane], tc);
+            }
+            for (int r = warp; r < p.cluster; r += kScanWarps) {
+                *cluster.map_shared_rank(&ex.rank[par][0][rank][lane], r) = map_of(ta, th);
+                *cluster.map_shared_rank(&ex.rank[par][1][rank][lane], r) = map_of(ta, tc);
             }
             cluster.sync();
-            for (int r = 0; r < rank; ++r) {
-                float ra[4], rh[4];
-                get4(&ex.rank[par][r][0][lr * 4], ra);
-                get4(&ex.rank[par][r][1][lr * 4], rh);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) h[i] = through(ra[i], h[i], rh[i]);
-            }
+            for (int r = 0; r < rank; ++r) h = through(ex.rank[par][0][r][lane], h);
             for (int r = p.cluster - 1; r >= 0; --r) {
-                float ra[4], rc[4];
-                get4(&ex.rank[par][r][0][lr * 4], ra);
-                get4(&ex.rank[par][r][2][lr * 4], rc);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (r == rank) c[i] = carry[i];
-                    carry[i] = through(ra[i], carry[i], rc[i]);
-                }
+                if (r == rank) c = carry;
+                carry = through(ex.rank[par][1][r][lane], carry);
             }
-        }
-        for (int w = 0; w < warp; ++w) {
-            float wa[4], wh[4];
-            get4(&ex.warp[par][w][0][lr * 4], wa);
-            get4(&ex.warp[par][w][1][lr * 4], wh);
+            for (int w = kScanWarps - 1; w > warp; --w) c = through(ex.warp[par][1][w][lane], c);
+            for (int w = 0; w < warp; ++w) h = through(ex.warp[par][0][w][lane], h);
+        } else if (!any) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) h[i] = through(wa[i], h[i], wh[i]);
-        }
-        for (int w = kScanWarps - 1; w >= 0; --w) {
-            float wa[4], wc[4];
-            if (p.cluster > 1 && w <= warp) break;
-            get4(&ex.warp[par][w][0][lr * 4], wa);
-            get4(&ex.warp[par][w][2][lr * 4], wc);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (w > warp) c[i] = through(wa[i], c[i], wc[i]);
-                if (p.cluster == 1) carry[i] = through(wa[i], carry[i], wc[i]);
+            for (int w = kScanWarps - 1; w >= 0; --w) {
+                if (w == warp) c = carry;
+                carry = straight(ex.warp[par][1][w][lane], carry);
             }
+            for (int w = 0; w < warp; ++w) h = straight(ex.warp[par][0][w][lane], h);
+        } else {
+#pragma unroll
+            for (int w = kScanWarps - 1; w >= 0; --w) {
+                if (w == warp) c = carry;
+                carry = through(ex.warp[par][1][w][lane], carry);
+            }
+            for (int w = 0; w < warp; ++w) h = through(ex.warp[par][0][w][lane], h);
         }
+        // u becomes a n (h before the step - u), then both gradients in place of g and u
+        if (!special) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            h[i] = through(A[i], h[i], H[i]);
-            c[i] = through(B[i], c[i], C[i]);
+            for (int s = 0; s < kSteps; ++s) {
+                const float2 d = fma2(u[s], two(-1.0f), h);
+                h = fma2(a[s], h, mul2(n[s], u[s]));
+                u[s] = mul2(mul2(a[s], n[s]), d);
+            }
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-                const float w = a[s][i] * n[s][i], d = h[i] - u[s][i];
-                h[i] = through(a[s][i], h[i], n[s][i] == 0.0f ? 0.0f : n[s][i] * u[s][i]);
-                z[s][i] = w == 0.0f ? 0.0f : w * d;
+            for (int s = kSteps - 1; s >= 0; --s) {
+                const float2 dh = add2(g[s], c);
+                u[s] = mul2(u[s], dh);
+                g[s] = mul2(n[s], dh);
+                c = mul2(a[s], dh);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const float2 d = fma2(u[s], two(-1.0f), h), w = mul2(a[s], n[s]);
+                h = after(a[s], h, mul2(n[s], u[s]));
+                u[s] = looked_at(w, mul2(w, d));
+            }
+#pragma unroll
+            for (int s = kSteps - 1; s >= 0; --s) {
+                const float2 dh = add2(g[s], c);
+                u[s] = mul2(u[s], dh);
+                g[s] = mul2(n[s], dh);
+                c = looked_at(a[s], mul2(a[s], dh));
             }
         }
         const long long at = (q.first + t0) * p.width + ch;
+        T *const dz = (T *)p.dgate + at, *const du = (T *)p.dvalue + at;
+        if (vec && nch == 2 && cnt == kSteps) {
 #pragma unroll
-        for (int s = S - 1; s >= 0; --s) {
-            float dz[4], du[4];
+            for (int s = 0; s < kSteps; ++s) {
+                store2v(dz + (long long)s * p.width, u[s]);
+                store2v(du + (long long)s * p.width, g[s]);
+            }
+        } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float dh = g[s][i] + c[i];
-                du[i] = n[s][i] * dh;
-                dz[i] = z[s][i] * dh;
-                // a step behind the end has a = 1 and g = 0
-                c[i] = a[s][i] == 0.0f ? 0.0f : a[s][i] * dh;
-            }
-            if (s < cnt) {
-                store4((T *)p.dgate + at + (long long)s * p.width, vec, nch, dz);
-                store4((T *)p.dvalue + at + (long long)s * p.width, vec, nch, du);
-            }
+            for (int s = 0; s < kSteps; ++s)
+                if (s < cnt) {
+                    store2(dz + (long long)s * p.width, vec, nch, u[s]);
+                    store2(du + (long long)s * p.width, vec, nch, g[s]);
+                }
         }
     }
-    if (p.dstate && rank == 0 && threadIdx.x < L::kLanes) store4(p.dstate + state_at, vec, nch, carry);
+    if (p.dstate && rank == 0 && warp == 0) store2(p.dstate + state_at, vec, nch, carry);
 }
 
 // ------------------------------------------------------------------ one step
@@ -511,23 +658,17 @@ template <typename T>
 __global__ void __launch_bounds__(256) scan_step_k(const T *__restrict__ gate, const T *__restrict__ value, const float *state, T *__restrict__ h,
                                                    float *out_state, long long rows, int width, long long gate_row, long long value_row, int vec)
 {
-    const int quads = (width + 3) / 4;
+    const int pairs = (width + 1) / 2;
     const long long stride = (long long)gridDim.x * blockDim.x;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < rows * quads; i += stride) {
-        const long long row = i / quads;
-        const int ch = (int)(i - row * quads) * 4, nch = min(4, width - ch);
-        float z[4], u[4], s[4];
-        load4(gate + row * gate_row + ch, vec, nch, z);
-        load4(value + row * value_row + ch, vec, nch, u);
-        load4(state + row * width + ch, vec, nch, s);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float a, n;
-            gates(z[k], a, n);
-            s[k] = through(a, s[k], n == 0.0f ? 0.0f : n * u[k]);
-        }
-        store4(h + row * width + ch, vec, nch, s);
-        store4(out_state + row * width + ch, vec, nch, s);
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < rows * pairs; i += stride) {
+        const long long row = i / pairs;
+        const int ch = (int)(i - row * pairs) * 2, nch = min(2, width - ch);
+        float2 a, n;
+        gates_any(load2(gate + row * gate_row + ch, vec, nch), a, n);
+        const float2 u = looked_at(n, load2(value + row * value_row + ch, vec, nch));
+        const float2 s = after(a, load2(state + row * width + ch, vec, nch), mul2(n, u));
+        store2(h + row * width + ch, vec, nch, s);
+        store2(out_state + row * width + ch, vec, nch, s);
     }
 }
 
@@ -540,8 +681,6 @@ static int scan_cluster(int n, long long steps, int width, int size, bool backwa
     (void)n; (void)steps; (void)width; (void)size; (void)backward;
     return 1;
 }
-static int slab_width(int dtype) { return dtype == GN_F32 ? Lay<float>::kWidth : Lay<__half>::kWidth; }
-static int held_steps(int dtype) { return dtype == GN_F32 ? Lay<float>::kBwd : Lay<__half>::kBwd; }
 
 static int scan_check(int n, long long steps, long long total, int width, int dtype, bool ragged)
 {
@@ -549,7 +688,7 @@ static int scan_check(int n, long long steps, long long total, int width, int dt
     if (!ragged && total != n * steps) return GN_ERR_BAD_SHAPE;
     if (dtype < GN_F32 || dtype > GN_F16) return GN_ERR_UNSUPPORTED;
     if (total > (1LL << 48) / width) return GN_ERR_TOO_LARGE;
-    const long long slabs = (width + slab_width(dtype) - 1) / slab_width(dtype);
+    const long long slabs = (width + kSlab - 1) / kSlab;
     if ((n + 1LL) * slabs * kMaxCluster > 0x7fffffffLL) return GN_ERR_TOO_LARGE;
     return GN_OK;
 }
@@ -557,7 +696,7 @@ static int scan_check(int n, long long steps, long long total, int width, int dt
 static int scan_interval(int n, long long steps, long long total, int width, int dtype, bool ragged)
 {
     const long long mean = ragged ? total / (n > 0 ? n : 1) : steps;
-    return held_steps(dtype) * scan_cluster(n, mean, width, dtype == GN_F32 ? 4 : 2, true);
+    return kTile * scan_cluster(n, mean, width, dtype == GN_F32 ? 4 : 2, true);
 }
 
 static int launch_scan(void (*kern)(const Scan), const Scan &p, const char *what, cudaStream_t st)
@@ -572,7 +711,9 @@ static int launch_scan(void (*kern)(const Scan), const Scan &p, const char *what
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
+    cudaError_t e = cudaSuccess;
+    if (p.cluster > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kern, p);
     if (e != cudaSuccess) {
         record_cuda_error(e, what);
         (void)cudaGetLastError();
@@ -584,14 +725,14 @@ static int launch_scan(void (*kern)(const Scan), const Scan &p, const char *what
 template <typename T>
 static int scan_forward(Scan &p, cudaStream_t st)
 {
-    p.slabs = (p.width + Lay<T>::kWidth - 1) / Lay<T>::kWidth;
+    p.slabs = (p.width + kSlab - 1) / kSlab;
     return launch_scan(p.pack_gate ? scan_forward_k<T, false, true> : scan_forward_k<T, false, false>, p, "gated_scan", st);
 }
 
 template <typename T>
 static int scan_backward(Scan &p, bool packed, bool long_sequences, cudaStream_t st)
 {
-    p.slabs = (p.width + Lay<T>::kWidth - 1) / Lay<T>::kWidth;
+    p.slabs = (p.width + kSlab - 1) / kSlab;
     if (packed && long_sequences) {  // the states that the codes lead to
         const int rc = launch_scan(scan_forward_k<T, true, false>, p, "gated_scan states", st);
         if (rc != GN_OK) return rc;
@@ -634,9 +775,9 @@ GN_API int gn_gated_scan_forward(const void *gate, const void *value, const floa
     p.n = n; p.steps = steps; p.total = total; p.width = width;
     const int size = dtype == GN_F32 ? 4 : 2;
     p.cluster = scan_cluster(n, offsets ? total / (n > 0 ? n : 1) : steps, width, size, false);
-    p.vec = width % 4 == 0 && gate_seq % 4 == 0 && gate_step % 4 == 0 && value_seq % 4 == 0 && value_step % 4 == 0 && aligned(gate, 4 * size) &&
-            aligned(value, 4 * size) && aligned(h, 4 * size) && aligned(state, 16) && aligned(last, 16) && aligned(bounds, 16) &&
-            aligned(gate_codes, 4) && aligned(value_codes, 4);
+    p.vec = width % 2 == 0 && gate_seq % 2 == 0 && gate_step % 2 == 0 && value_seq % 2 == 0 && value_step % 2 == 0 && aligned(gate, 2 * size) &&
+            aligned(value, 2 * size) && aligned(h, 2 * size) && aligned(state, 8) && aligned(last, 8) && aligned(bounds, 8) &&
+            aligned(gate_codes, 2) && aligned(value_codes, 2);
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == GN_F32) return scan_forward<float>(p, st);
     if (dtype == GN_BF16) return scan_forward<__nv_bfloat16>(p, st);
@@ -662,11 +803,11 @@ GN_API int gn_gated_scan_backward(const void *gate, const void *value, const voi
     p.interval = scan_interval(n, steps, total, width, dtype, offsets != nullptr);
     p.gate_seq = gate_seq; p.gate_step = gate_step; p.value_seq = value_seq; p.value_step = value_step;
     p.n = n; p.steps = steps; p.total = total; p.width = width;
-    p.cluster = p.interval / held_steps(dtype);
+    p.cluster = p.interval / kTile;
     const int size = dtype == GN_F32 ? 4 : 2, in = gate_scales ? 1 : size;
-    p.vec = width % 4 == 0 && gate_seq % 4 == 0 && gate_step % 4 == 0 && value_seq % 4 == 0 && value_step % 4 == 0 && aligned(gate, 4 * in) &&
-            aligned(value, 4 * in) && aligned(grad_h, 4 * size) && aligned(grad_gate, 4 * size) && aligned(grad_value, 4 * size) &&
-            aligned(state, 16) && aligned(grad_last, 16) && aligned(grad_state, 16) && aligned(bounds, 16);
+    p.vec = width % 2 == 0 && gate_seq % 2 == 0 && gate_step % 2 == 0 && value_seq % 2 == 0 && value_step % 2 == 0 && aligned(gate, 2 * in) &&
+            aligned(value, 2 * in) && aligned(grad_h, 2 * size) && aligned(grad_gate, 2 * size) && aligned(grad_value, 2 * size) &&
+            aligned(state, 8) && aligned(grad_last, 8) && aligned(grad_state, 8) && aligned(bounds, 8);
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == GN_F32) return scan_backward<float>(p, gate_scales != nullptr, long_sequences, st);
     if (dtype == GN_BF16) return scan_backward<__nv_bfloat16>(p, gate_scales != nullptr, long_sequences, st);
@@ -681,9 +822,9 @@ GN_API int gn_gated_scan_step(const void *gate, const void *value, const float *
     if (rows == 0) return GN_OK;
     if (!gate || !value || !state || !h || !out_state) return GN_ERR_NULL_POINTER;
     const int size = dtype == GN_F32 ? 4 : 2;
-    const int vec = width % 4 == 0 && gate_row % 4 == 0 && value_row % 4 == 0 && aligned(gate, 4 * size) && aligned(value, 4 * size) &&
-                    aligned(h, 4 * size) && aligned(state, 16) && aligned(out_state, 16);
-    const long long want = (rows * ((width + 3) / 4) + 255) / 256, most = 16LL * sm_count();
+    const int vec = width % 2 == 0 && gate_row % 2 == 0 && value_row % 2 == 0 && aligned(gate, 2 * size) && aligned(value, 2 * size) &&
+                    aligned(h, 2 * size) && aligned(state, 8) && aligned(out_state, 8);
+    const long long want = (rows * ((width + 1) / 2) + 255) / 256, most = 16LL * sm_count();
     const unsigned blocks = (unsigned)(want < most ? want : most);
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == GN_F32)
