@@ -20,6 +20,8 @@
 // of its own, no lane has to know another lane's.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "kernels.h"
 #include "packed8.cuh"
 
@@ -27,7 +29,7 @@ namespace gn {
 
 namespace cg = cooperative_groups;
 
-constexpr int kScanThreads = 256, kScanWarps = 8, kMaxCluster = 16;
+constexpr int kScanThreads = 256, kScanWarps = 8, kMaxCluster = 8;
 constexpr int kSlab = 64;                    // channels of a CTA
 constexpr int kSteps = 8;                    // steps that a thread holds
 constexpr int kTile = kScanWarps * kSteps;   // steps of a CTA
@@ -47,7 +49,9 @@ struct Scan {
     const float *glast;
     void *dgate, *dvalue;
     float *dstate;
-    int n, width, slabs, cluster, vec;
+    int n, width, slabs, cluster;
+    int vec;   // pairs of channels lie on whole pairs' addresses
+    int wide;  // 16 bytes of a row on multiples of 16
     long long steps, total;  // steps of a sequence; rows of everything
 };
 
@@ -74,36 +78,9 @@ __device__ __forceinline__ long long bound_row(const Scan &p, int seq, const Pla
 }
 
 // ---- pairs
-__device__ __forceinline__ unsigned long long bits2(float2 v)
-{
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
-    return r;
-}
-__device__ __forceinline__ float2 pair2(unsigned long long v)
-{
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b)
-{
-    unsigned long long r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
-    return pair2(r);
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b)
-{
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)));
-    return pair2(r);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c)
-{
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits2(a)), "l"(bits2(b)), "l"(bits2(c)));
-    return pair2(r);
-}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 two(float v) { return make_float2(v, v); }
 
 __device__ __forceinline__ float2 load2v(const float *p) { return *reinterpret_cast<const float2 *>(p); }
@@ -134,32 +111,22 @@ __device__ __forceinline__ void store2(T *p, bool vec, int n, float2 v)
     if (n > 1) p[1] = from_float<T>(v.y);
 }
 
-// e = exp(-z) for |z| < 80, as 2^t with what t lost by rounding put back: about three units in the last place
-__device__ __forceinline__ float2 exp_of_minus(float2 z)
-{
-    const float2 t = mul2(z, two(-1.4426950408889634f));
-    float2 e;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
-    asm("ex2.approx.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
-    // -z - t ln 2, with ln 2 in two parts: 0.693147182 - 1.90465421e-9
-    const float2 lost = fma2(t, two(1.90465421e-9f), fma2(t, two(-0.693147182f), mul2(z, two(-1.0f))));
-    return fma2(e, lost, e);
-}
-// 1 / w for 1 <= w <= 2^120: the approximation and a Newton step. Its error has a sign that is not even, which a memory of thousands of steps
-// would add up (8 x 2048 x 4096 without the step, gradient of the state: 1.4e-6 off in the 2-norm; the plain form is 2.7e-7 off).
-__device__ __forceinline__ float2 reciprocal(float2 w)
-{
-    float2 r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(w.x));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(w.y));
-    return fma2(r, fma2(mul2(w, two(-1.0f)), r, two(1.0f)), r);
-}
-// s(z) and s(-z). Gates from kFar on, and what is behind the end, go through gates_any.
+// s(z) and s(-z) for |z| < kFar; everything else, and what is behind the end, goes through gates_any.
+// e = exp(-z) as 2^t: t is rounded, which is as if z were another number 1.3 half steps of float32 away, about as far as z has been rounded
+// to begin with. a = 1 / (1 + e) by the approximation and a Newton step r (2 - (1 + e) r), all with signs turned so that no operand has
+// to be negated: the approximation's error has a sign that is not even, which a memory of thousands of steps would add up
+// (8 x 2048 x 4096 without the step, gradient of the state: 1.4e-6 off in the 2-norm; the plain form is 2.7e-7 off).
 constexpr float kFar = 80.0f;
 __device__ __forceinline__ void gates(float2 z, float2 &a, float2 &n)
 {
-    const float2 e = exp_of_minus(z);
-    a = reciprocal(add2(e, two(1.0f)));
+    const float2 t = mul2(z, two(-1.4426950408889634f));
+    float2 e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    const float2 w = fma2(e, two(-1.0f), two(-1.0f));  // -(1 + e)
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(w.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(w.y));
+    a = mul2(r, fma2(w, r, two(-2.0f)));
     n = mul2(e, a);
 }
 // For every z: the smaller from exp(-|z|), which is 0 from |z| = 104 on, the larger as 1 less it
@@ -269,8 +236,9 @@ __device__ __forceinline__ void load_packed(const unsigned char *codes, const un
 
 // Packs the rows that a warp holds, 8 of them, 64 channels each: two groups a row, a half of the warp's lanes a group. The largest
 // of a group is found for all rows at a time, halving the rows that a lane still looks at: lane l of a half ends up with row l & 7.
+// whole: all rows and channels are there, and pairs of codes lie on even addresses
 __device__ __forceinline__ void pack_rows(const float2 (&v)[kSteps], unsigned char *codes, unsigned char *scales, long long row, int width, int ch,
-                                          bool vec, int cnt, int nch)
+                                          bool whole, int cnt, int nch)
 {
     const int lane = threadIdx.x & 31;
     unsigned m[kSteps];
@@ -300,6 +268,15 @@ __device__ __forceinline__ void pack_rows(const float2 (&v)[kSteps], unsigned ch
     const int per_row = (width + kPackGroup - 1) / kPackGroup, group = ch / kPackGroup;
     if ((lane & 15) < cnt && group < per_row) scales[(row + (lane & 15)) * per_row + group] = (unsigned char)scale;
     unsigned char *at = codes + row * width + ch;
+    if (!again && whole) {
+        const float inverse = pack_inverse(scale);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s, at += width) {
+            const float2 c = fma2(v[s], two(__shfl_sync(0xffffffffu, inverse, (lane & 16) | s)), two(12582912.0f));
+            *reinterpret_cast<unsigned short *>(at) = (unsigned short)__byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x0040);
+        }
+        return;
+    }
 #pragma unroll
     for (int s = 0; s < kSteps; ++s, at += width) {
         const unsigned sc = __shfl_sync(0xffffffffu, scale, (lane & 16) | s);
@@ -313,12 +290,8 @@ __device__ __forceinline__ void pack_rows(const float2 (&v)[kSteps], unsigned ch
             b = pack_code(v[s].y, inv);
         }
         if (s < cnt) {
-            if (vec && nch == 2) {
-                *reinterpret_cast<unsigned short *>(at) = (unsigned short)__byte_perm(a, b, 0x0040);
-            } else {
-                if (nch > 0) at[0] = (unsigned char)a;
-                if (nch > 1) at[1] = (unsigned char)b;
-            }
+            if (nch > 0) at[0] = (unsigned char)a;
+            if (nch > 1) at[1] = (unsigned char)b;
         }
     }
 }
@@ -329,6 +302,78 @@ __device__ __forceinline__ float farthest(const float2 (&z)[kSteps])  // |z|; Na
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) m = fmaxf(m, fmaxf(fabsf(z[s].x), fabsf(z[s].y)));
     return m;
+}
+
+// ---- a warp's next steps on their way to shared memory while the ones in hand are worked on: 8 rows of 64 values each
+__device__ __forceinline__ void copy16(void *to, const void *from)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_on_their_way() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_there()  // all lanes' of the warp
+{
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+}
+template <typename V>
+struct Rows {
+    V v[kSteps][kSlab];
+};
+// from: first value of the slab in the first row; left: values of a row from there on
+template <typename V>
+__device__ __forceinline__ void ask(Rows<V> &to, const V *from, long long step, int cnt, int left)
+{
+    constexpr int kPer = 16 / sizeof(V), kChunks = kSlab / kPer;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < kSteps * kChunks; i += 32) {
+        const int at = i + lane, row = at / kChunks, col = at % kChunks * kPer;
+        if (at < kSteps * kChunks && row < cnt && col < left) copy16(&to.v[row][col], from + row * step + col);
+    }
+}
+// What has been asked for, as load_rows gives it
+template <typename T>
+__device__ __forceinline__ void take(const Rows<T> &from, int cnt, int nch, float end, float2 (&v)[kSteps])
+{
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) v[s] = load2v(&from.v[s][lane * 2]);
+    if (cnt < kSteps || nch == 0)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) v[s] = s >= cnt ? two(end) : nch == 0 ? two(0.0f) : v[s];
+}
+// The scale bytes of a warp's steps: lane 2 r + g has those of row r, group g of the slab
+__device__ __forceinline__ unsigned ask_scales(const unsigned char *scales, long long row, int per_row, int slab, int cnt)
+{
+    const int lane = threadIdx.x & 31, r = lane >> 1, g = slab * (kSlab / kPackGroup) + (lane & 1);
+    return r < cnt && r < kSteps && g < per_row ? scales[(row + r) * per_row + g] : 127u;
+}
+__device__ __forceinline__ void take_packed(const Rows<unsigned char> &from, unsigned scales, int cnt, int nch, float end, float2 (&v)[kSteps])
+{
+    const int lane = threadIdx.x & 31;
+    unsigned w[kSteps / 2], odd = 0;
+#pragma unroll
+    for (int s = 0; s < kSteps; s += 2) {  // the codes of two steps in a word
+        w[s / 2] = __byte_perm(*reinterpret_cast<const unsigned short *>(&from.v[s][lane * 2]),
+                               *reinterpret_cast<const unsigned short *>(&from.v[s + 1][lane * 2]), 0x5410);
+        odd |= unpack_odd(w[s / 2]);
+        float f[4];
+        unpack4_finite(w[s / 2], f);
+        v[s] = make_float2(f[0], f[1]);
+        v[s + 1] = make_float2(f[2], f[3]);
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) v[s] = mul2(v[s], two(pack_step(__shfl_sync(0xffffffffu, scales, 2 * s + (lane >> 4)))));
+    if (odd) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const unsigned c = w[s / 2] >> (s % 2 * 16);
+            v[s] = make_float2(unpack_special(v[s].x, c & 0xffu), unpack_special(v[s].y, (c >> 8) & 0xffu));
+        }
+    }
+    if (cnt < kSteps || nch == 0)
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) v[s] = s >= cnt ? two(end) : nch == 0 ? two(0.0f) : v[s];
 }
 
 // What a warp's, a CTA's steps amount to: (A, H) and, backward, (A, C) of a channel pair; two copies, so that one barrier lies between
@@ -347,8 +392,10 @@ struct Exchange {
 // ------------------------------------------------------------------ forward
 // PACKED: gate and value are codes, and only the states at the boundaries are wanted. KEEP: packs gate and value.
 template <typename T, bool PACKED, bool KEEP>
-__global__ void __launch_bounds__(kScanThreads, sizeof(T) == 2 && !KEEP ? 3 : 2) scan_forward_k(const Scan p)
+__global__ void __launch_bounds__(kScanThreads, KEEP ? 2 : 3) scan_forward_k(const Scan p)
 {
+    using V = std::conditional_t<PACKED, unsigned char, T>;
+    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) Exchange<1> ex;
     const int rank = blockIdx.x % p.cluster, id = blockIdx.x / p.cluster;
     const int slab = id % p.slabs, seq = id / p.slabs;
@@ -370,35 +417,57 @@ __global__ void __launch_bounds__(kScanThreads, sizeof(T) == 2 && !KEEP ? 3 : 2)
     if (PACKED && q.len <= p.interval) return;  // the whole cluster
     const long long held = (long long)kTile * p.cluster;
     long long t0 = (long long)rank * kTile + warp * kSteps;
-    const T *gate = (const T *)p.gate + (p.offsets ? q.first * p.gate_step : seq * p.gate_seq) + t0 * p.gate_step + ch;
-    const T *value = (const T *)p.value + (p.offsets ? q.first * p.value_step : seq * p.value_seq) + t0 * p.value_step + ch;
+    // codes lie in rows of width, one after the other
+    const long long gate_step = PACKED ? p.width : p.gate_step, value_step = PACKED ? p.width : p.value_step;
+    const V *gate = (const V *)p.gate + (PACKED || p.offsets ? q.first * gate_step : seq * p.gate_seq) + t0 * gate_step + slab * kSlab;
+    const V *value = (const V *)p.value + (PACKED || p.offsets ? q.first * value_step : seq * p.value_seq) + t0 * value_step + slab * kSlab;
+    const int per_row = (p.width + kPackGroup - 1) / kPackGroup, left = p.width - slab * kSlab;
+    Rows<V> &zs = reinterpret_cast<Rows<V> *>(dynamic)[warp], &us = reinterpret_cast<Rows<V> *>(dynamic)[kScanWarps + warp];
+    unsigned zsc = 0, usc = 0;
+    const bool wide = p.wide;
+    auto ask_all = [&](long long t) {
+        const int cnt = (int)min((long long)kSteps, max(0LL, q.len - t));
+        ask(zs, gate, gate_step, cnt, left);
+        ask(us, value, value_step, cnt, left);
+        copies_on_their_way();
+        if (PACKED) {
+            zsc = ask_scales(p.gate_scales, q.first + t, per_row, slab, cnt);
+            usc = ask_scales(p.value_scales, q.first + t, per_row, slab, cnt);
+        }
+    };
+    if (wide) ask_all(t0);
     // a CTA's shared memory may be written to by others once it runs: waited for ahead of the first such store
     if (p.cluster > 1) cg::this_cluster().sync();
     const float inf = __uint_as_float(0x7f800000u);
-    const bool pairs = vec && nch == 2;
-    bool asked = false;  // the steps in hand have been asked for a tile ahead
-    float2 za[kSteps], ua[kSteps];
     for (int par = 0; t0 - (long long)rank * kTile - warp * kSteps < q.len; t0 += held, par ^= 1) {
         const int cnt = (int)min((long long)kSteps, max(0LL, q.len - t0));
         // a step behind the end holds the state
         float2 a[kSteps], b[kSteps];
-        if (PACKED) {
+        if (wide) {
+            copies_there();
+            if constexpr (PACKED) {
+                take_packed(zs, zsc, cnt, nch, inf, a);
+                take_packed(us, usc, cnt, nch, 0.0f, b);
+            } else {
+                take(zs, cnt, nch, inf, a);
+                take(us, cnt, nch, 0.0f, b);
+            }
+            __syncwarp();
+            gate += held * gate_step;
+            value += held * value_step;
+            ask_all(t0 + held);
+        } else if constexpr (PACKED) {
             load_packed((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, inf, a);
             load_packed((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, 0.0f, b);
         } else {
-            if (!asked) {
-                load_rows<T>(gate, p.gate_step, vec, cnt, nch, inf, za);
-                load_rows<T>(value, p.value_step, vec, cnt, nch, 0.0f, ua);
-            }
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                a[s] = za[s];
-                b[s] = ua[s];
-            }
+            load_rows<T>(gate + lane * 2, gate_step, vec, cnt, nch, inf, a);
+            load_rows<T>(value + lane * 2, value_step, vec, cnt, nch, 0.0f, b);
+            gate += held * gate_step;
+            value += held * value_step;
         }
         if constexpr (KEEP) {
-            pack_rows(a, p.pack_gate, p.pack_gate_scales, q.first + t0, p.width, ch, vec, cnt, nch);
-            pack_rows(b, p.pack_value, p.pack_value_scales, q.first + t0, p.width, ch, vec, cnt, nch);
+            pack_rows(a, p.pack_gate, p.pack_gate_scales, q.first + t0, p.width, ch, vec && left >= kSlab && cnt == kSteps, cnt, nch);
+            pack_rows(b, p.pack_value, p.pack_value_scales, q.first + t0, p.width, ch, vec && left >= kSlab && cnt == kSteps, cnt, nch);
         }
         const bool special = farthest(a) >= kFar;
         float2 A = two(1.0f), H = two(0.0f);
@@ -421,18 +490,6 @@ __global__ void __launch_bounds__(kScanThreads, sizeof(T) == 2 && !KEEP ? 3 : 2)
                 b[s] = mul2(n, looked_at(n, b[s]));
                 H = after(w, H, b[s]);
                 A = more(A, w);
-            }
-        }
-        if (!PACKED) {
-            gate += held * p.gate_step;
-            value += held * p.value_step;
-            asked = pairs && t0 + held + kSteps <= q.len;
-            if (asked) {
-#pragma unroll
-                for (int s = 0; s < kSteps; ++s) {
-                    za[s] = load2v(gate + s * p.gate_step);
-                    ua[s] = load2v(value + s * p.value_step);
-                }
             }
         }
         ex.warp[par][0][warp][lane] = map_of(A, H);
@@ -480,7 +537,7 @@ __global__ void __launch_bounds__(kScanThreads, sizeof(T) == 2 && !KEEP ? 3 : 2)
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) a[s] = h = after(a[s], h, b[s]);
             }
-            if (pairs && cnt == kSteps) {
+            if (vec && nch == 2 && cnt == kSteps) {
 #pragma unroll
                 for (int s = 0; s < kSteps; ++s) store2v(out + (long long)s * p.width, a[s]);
             } else {
@@ -497,6 +554,8 @@ __global__ void __launch_bounds__(kScanThreads, sizeof(T) == 2 && !KEEP ? 3 : 2)
 template <typename T, bool PACKED>
 __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
 {
+    using V = std::conditional_t<PACKED, unsigned char, T>;
+    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) Exchange<2> ex;
     const int rank = blockIdx.x % p.cluster, id = blockIdx.x / p.cluster;
     const int slab = id % p.slabs, seq = id / p.slabs;
@@ -512,26 +571,63 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
     const long long state_at = (long long)seq * p.width + ch;
     float2 carry = two(0.0f);  // gradient of the state behind the steps in hand
     if (p.glast) carry = load2(p.glast + state_at, vec, nch);
-    const T *const gate = (const T *)p.gate + (p.offsets ? q.first * p.gate_step : seq * p.gate_seq) + ch;
-    const T *const value = (const T *)p.value + (p.offsets ? q.first * p.value_step : seq * p.value_seq) + ch;
+    // codes lie in rows of width, one after the other
+    const long long gate_step = PACKED ? p.width : p.gate_step, value_step = PACKED ? p.width : p.value_step;
+    const V *const gate = (const V *)p.gate + (PACKED || p.offsets ? q.first * gate_step : seq * p.gate_seq) + slab * kSlab;
+    const V *const value = (const V *)p.value + (PACKED || p.offsets ? q.first * value_step : seq * p.value_seq) + slab * kSlab;
+    const T *const grad = (const T *)p.gh + q.first * p.width + slab * kSlab;
     const long long held = (long long)kTile * p.cluster;  // == p.interval
+    const int per_row = (p.width + kPackGroup - 1) / kPackGroup, left = p.width - slab * kSlab;
+    Rows<T> &gs = reinterpret_cast<Rows<T> *>(dynamic)[warp];
+    Rows<V> *const inputs = reinterpret_cast<Rows<V> *>(dynamic + kScanWarps * sizeof(Rows<T>));
+    Rows<V> &zs = inputs[warp], &us = inputs[kScanWarps + warp];
+    unsigned zsc = 0, usc = 0;
+    const bool wide = p.wide;
+    auto ask_all = [&](long long t) {
+        const int cnt = (int)min((long long)kSteps, max(0LL, q.len - t));
+        if (cnt <= 0) return;
+        ask(zs, gate + t * gate_step, gate_step, cnt, left);
+        ask(us, value + t * value_step, value_step, cnt, left);
+        ask(gs, grad + t * p.width, p.width, cnt, left);
+        copies_on_their_way();
+        if (PACKED) {
+            zsc = ask_scales(p.gate_scales, q.first + t, per_row, slab, cnt);
+            usc = ask_scales(p.value_scales, q.first + t, per_row, slab, cnt);
+        }
+    };
     int par = 0;
+    const long long last = (q.len + held - 1) / held - 1, mine = (long long)rank * kTile + warp * kSteps;
+    if (wide && last >= 0) ask_all(last * held + mine);
     // a CTA's shared memory may be written to by others once it runs: waited for ahead of the first such store
     if (p.cluster > 1) cg::this_cluster().sync();
     const float inf = __uint_as_float(0x7f800000u);
-    for (long long k = (q.len + held - 1) / held - 1; k >= 0; --k, par ^= 1) {
-        const long long t0 = k * held + (long long)rank * kTile + warp * kSteps;
+    for (long long k = last; k >= 0; --k, par ^= 1) {
+        const long long t0 = k * held + mine;
         const int cnt = (int)min((long long)kSteps, max(0LL, q.len - t0));
         // a step behind the end holds the state and has no gradient of its own
         float2 a[kSteps], n[kSteps], u[kSteps], g[kSteps], h = two(0.0f);
-        if (PACKED) {
-            load_packed((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, inf, a);
-            load_packed((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, 0.0f, u);
+        if (wide) {
+            copies_there();
+            if constexpr (PACKED) {
+                take_packed(zs, zsc, cnt, nch, inf, a);
+                take_packed(us, usc, cnt, nch, 0.0f, u);
+            } else {
+                take(zs, cnt, nch, inf, a);
+                take(us, cnt, nch, 0.0f, u);
+            }
+            take(gs, cnt, nch, 0.0f, g);
+            __syncwarp();
+            if (k > 0) ask_all(t0 - held);
         } else {
-            load_rows<T>(gate + t0 * p.gate_step, p.gate_step, vec, cnt, nch, inf, a);
-            load_rows<T>(value + t0 * p.value_step, p.value_step, vec, cnt, nch, 0.0f, u);
+            if constexpr (PACKED) {
+                load_packed((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, inf, a);
+                load_packed((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, 0.0f, u);
+            } else {
+                load_rows<T>(gate + lane * 2 + t0 * gate_step, gate_step, vec, cnt, nch, inf, a);
+                load_rows<T>(value + lane * 2 + t0 * value_step, value_step, vec, cnt, nch, 0.0f, u);
+            }
+            load_rows<T>(grad + lane * 2 + t0 * p.width, p.width, vec, cnt, nch, 0.0f, g);
         }
-        load_rows<T>((const T *)p.gh + (q.first + t0) * p.width + ch, p.width, vec, cnt, nch, 0.0f, g);
         if (k > 0)
             h = load2(p.bounds + bound_row(p, seq, q, k) * p.width + ch, vec, nch);
         else if (p.state)
@@ -699,11 +795,13 @@ static int scan_interval(int n, long long steps, long long total, int width, int
     return kTile * scan_cluster(n, mean, width, dtype == GN_F32 ? 4 : 2, true);
 }
 
-static int launch_scan(void (*kern)(const Scan), const Scan &p, const char *what, cudaStream_t st)
+static int launch_scan(void (*kern)(const Scan), const Scan &p, size_t value_bytes, const char *what, cudaStream_t st)
 {
+    const size_t smem = p.wide ? value_bytes * kTile * kSlab : 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((p.n + (p.offsets ? 1LL : 0LL)) * p.slabs * p.cluster));
     cfg.blockDim = dim3(kScanThreads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -712,7 +810,7 @@ static int launch_scan(void (*kern)(const Scan), const Scan &p, const char *what
     cfg.attrs = attr;
     cfg.numAttrs = p.cluster > 1 ? 1 : 0;
     cudaError_t e = cudaSuccess;
-    if (p.cluster > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (smem > 0) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kern, p);
     if (e != cudaSuccess) {
         record_cuda_error(e, what);
@@ -726,7 +824,7 @@ template <typename T>
 static int scan_forward(Scan &p, cudaStream_t st)
 {
     p.slabs = (p.width + kSlab - 1) / kSlab;
-    return launch_scan(p.pack_gate ? scan_forward_k<T, false, true> : scan_forward_k<T, false, false>, p, "gated_scan", st);
+    return launch_scan(p.pack_gate ? scan_forward_k<T, false, true> : scan_forward_k<T, false, false>, p, 2 * sizeof(T), "gated_scan", st);
 }
 
 template <typename T>
@@ -734,10 +832,10 @@ static int scan_backward(Scan &p, bool packed, bool long_sequences, cudaStream_t
 {
     p.slabs = (p.width + kSlab - 1) / kSlab;
     if (packed && long_sequences) {  // the states that the codes lead to
-        const int rc = launch_scan(scan_forward_k<T, true, false>, p, "gated_scan states", st);
+        const int rc = launch_scan(scan_forward_k<T, true, false>, p, 2, "gated_scan states", st);
         if (rc != GN_OK) return rc;
     }
-    return launch_scan(packed ? scan_backward_k<T, true> : scan_backward_k<T, false>, p, "gated_scan backward", st);
+    return launch_scan(packed ? scan_backward_k<T, true> : scan_backward_k<T, false>, p, (packed ? 2 : 2 * sizeof(T)) + sizeof(T), "gated_scan backward", st);
 }
 
 }  // namespace gn
@@ -778,6 +876,8 @@ GN_API int gn_gated_scan_forward(const void *gate, const void *value, const floa
     p.vec = width % 2 == 0 && gate_seq % 2 == 0 && gate_step % 2 == 0 && value_seq % 2 == 0 && value_step % 2 == 0 && aligned(gate, 2 * size) &&
             aligned(value, 2 * size) && aligned(h, 2 * size) && aligned(state, 8) && aligned(last, 8) && aligned(bounds, 8) &&
             aligned(gate_codes, 2) && aligned(value_codes, 2);
+    p.wide = (long long)width * size % 16 == 0 && gate_seq * size % 16 == 0 && gate_step * size % 16 == 0 && value_seq * size % 16 == 0 &&
+             value_step * size % 16 == 0 && aligned(gate, 16) && aligned(value, 16);
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == GN_F32) return scan_forward<float>(p, st);
     if (dtype == GN_BF16) return scan_forward<__nv_bfloat16>(p, st);
@@ -808,6 +908,8 @@ GN_API int gn_gated_scan_backward(const void *gate, const void *value, const voi
     p.vec = width % 2 == 0 && gate_seq % 2 == 0 && gate_step % 2 == 0 && value_seq % 2 == 0 && value_step % 2 == 0 && aligned(gate, 2 * in) &&
             aligned(value, 2 * in) && aligned(grad_h, 2 * size) && aligned(grad_gate, 2 * size) && aligned(grad_value, 2 * size) &&
             aligned(state, 8) && aligned(grad_last, 8) && aligned(grad_state, 8) && aligned(bounds, 8);
+    p.wide = (long long)width * in % 16 == 0 && (long long)width * size % 16 == 0 && gate_seq * in % 16 == 0 && gate_step * in % 16 == 0 &&
+             value_seq * in % 16 == 0 && value_step * in % 16 == 0 && aligned(gate, 16) && aligned(value, 16) && aligned(grad_h, 16);
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == GN_F32) return scan_backward<float>(p, gate_scales != nullptr, long_sequences, st);
     if (dtype == GN_BF16) return scan_backward<__nv_bfloat16>(p, gate_scales != nullptr, long_sequences, st);

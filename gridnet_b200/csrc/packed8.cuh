@@ -158,16 +158,28 @@ __device__ __forceinline__ float unpack_special(float v, unsigned code)
     return code == 0x7fu ? __uint_as_float(0x7f800000u) : code == 0x81u ? __uint_as_float(0xff800000u)
          : code == 0x80u ? __uint_as_float(0x7fc00000u) : v;
 }
+// four codes, all of them of finite values, as whole numbers
+__device__ __forceinline__ void unpack4_finite(unsigned word, float (&v)[4])
+{
+    const unsigned w = word ^ 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // 2^23 + (code + 128), as a float, less 2^23 + 128: exact
+        v[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)) - 8388736.0f;
+}
+// not 0 where one of the four stands for what is not finite
+__device__ __forceinline__ unsigned unpack_odd(unsigned word)
+{
+    // code + 129 as a byte: 0, 1 and 2 stand for what is not finite, 4 .. 254 for the rest
+    const unsigned w = word ^ 0x80808080u, up = (((w & 0x7f7f7f7fu) + 0x01010101u) ^ (w & 0x80808080u)) & 0xfcfcfcfcu;
+    return (up - 0x01010101u) & ~up & 0x80808080u;  // a byte of 0
+}
 // four codes -> the values they stand for
 __device__ __forceinline__ void unpack4(unsigned word, float step, float (&v)[4])
 {
-    const unsigned w = word ^ 0x80808080u;  // code + 128: 255, 1 and 0 stand for what is not finite, 3 .. 253 for the rest
+    unpack4_finite(word, v);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)  // 2^23 + byte, as a float, less 2^23 + 128: exact
-        v[i] = (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)) - 8388736.0f) * step;
-    // bytes 255, 0, 1 (and 2, which is none): all but the low two bits of byte + 1 are 0
-    const unsigned up = (((w & 0x7f7f7f7fu) + 0x01010101u) ^ (w & 0x80808080u)) & 0xfcfcfcfcu;
-    if ((up - 0x01010101u) & ~up & 0x80808080u) {
+    for (int i = 0; i < 4; ++i) v[i] *= step;
+    if (unpack_odd(word)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = unpack_special(v[i], (word >> (8 * i)) & 0xffu);
     }
