@@ -29,10 +29,10 @@ namespace gn {
 
 namespace cg = cooperative_groups;
 
-constexpr int kScanThreads = 256, kScanWarps = 8, kMaxCluster = 8;
+constexpr int kScanThreads = 128, kScanWarps = 4, kMaxCluster = 8;
 constexpr int kSlab = 64;                    // channels of a CTA
-constexpr int kSteps = 8;                    // steps that a thread holds
-constexpr int kTile = kScanWarps * kSteps;   // steps of a CTA
+constexpr int kFwdSteps = 16, kBwdSteps = 8;  // steps that a thread holds
+constexpr int kFwdTile = kScanWarps * kFwdSteps, kBwdTile = kScanWarps * kBwdSteps;
 
 struct Scan {
     const void *gate, *value;  // or codes
@@ -175,58 +175,59 @@ __device__ void clear_rows(const Scan &p, T *x, int slab, int rank)
 
 // Rows behind the end have `end`. Every load stands without a condition of its own (rows behind the end read the last one again): loads under
 // conditions are waited for one by one, 600 cycles each.
-template <typename T>
-__device__ __forceinline__ void load_rows(const T *x, long long step, bool vec, int cnt, int nch, float end, float2 (&v)[kSteps])
+template <typename T, int S>
+__device__ __forceinline__ void load_rows(const T *x, long long step, bool vec, int cnt, int nch, float end, float2 (&v)[S])
 {
-    if (cnt == kSteps && vec && nch == 2) {
+    if (cnt == S && vec && nch == 2) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) v[s] = load2v(x + s * step);
+        for (int s = 0; s < S; ++s) v[s] = load2v(x + s * step);
         return;
     }
     if (cnt > 0 && nch > 0) {
-        T one[kSteps], other[kSteps];
+        T one[S], other[S];
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
+        for (int s = 0; s < S; ++s) {
             const T *const at = x + min(s, cnt - 1) * step;
             one[s] = at[0];
             other[s] = at[nch - 1];
         }
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) v[s] = s < cnt ? make_float2(to_float<T>(one[s]), nch > 1 ? to_float<T>(other[s]) : 0.0f) : two(end);
+        for (int s = 0; s < S; ++s) v[s] = s < cnt ? make_float2(to_float<T>(one[s]), nch > 1 ? to_float<T>(other[s]) : 0.0f) : two(end);
     } else {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) v[s] = s < cnt ? two(0.0f) : two(end);
+        for (int s = 0; s < S; ++s) v[s] = s < cnt ? two(0.0f) : two(end);
     }
 }
 
+template <int S>
 __device__ __forceinline__ void load_packed(const unsigned char *codes, const unsigned char *scales, long long row, int width, int ch, bool vec,
-                                            int cnt, int nch, float end, float2 (&v)[kSteps])
+                                            int cnt, int nch, float end, float2 (&v)[S])
 {
     if (cnt <= 0 || nch <= 0) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) v[s] = s < cnt ? two(0.0f) : two(end);
+        for (int s = 0; s < S; ++s) v[s] = s < cnt ? two(0.0f) : two(end);
         return;
     }
     const int per_row = (width + kPackGroup - 1) / kPackGroup;
     const unsigned char *const c = codes + row * width + ch, *const g = scales + row * per_row + ch / kPackGroup;
-    unsigned w[kSteps], sc[kSteps];
+    unsigned w[S], sc[S];
     if (vec && nch == 2) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
+        for (int s = 0; s < S; ++s) {
             const long long i = min(s, cnt - 1);
             w[s] = *reinterpret_cast<const unsigned short *>(c + i * width);
             sc[s] = g[i * per_row];
         }
     } else {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
+        for (int s = 0; s < S; ++s) {
             const long long i = min(s, cnt - 1);
             w[s] = c[i * width] | (nch > 1 ? (unsigned)c[i * width + 1] << 8 : 0u);
             sc[s] = g[i * per_row];
         }
     }
 #pragma unroll
-    for (int s = 0; s < kSteps; s += 2) {  // the codes of two steps in a word
+    for (int s = 0; s < S; s += 2) {  // the codes of two steps in a word
         float f[4];
         unpack4(w[s] | w[s + 1] << 16, 1.0f, f);
         v[s] = s < cnt ? make_float2(f[0] * pack_step(sc[s]), f[1] * pack_step(sc[s])) : two(end);
@@ -234,31 +235,30 @@ __device__ __forceinline__ void load_packed(const unsigned char *codes, const un
     }
 }
 
-// Packs the rows that a warp holds, 8 of them, 64 channels each: two groups a row, a half of the warp's lanes a group. The largest
-// of a group is found for all rows at a time, halving the rows that a lane still looks at: lane l of a half ends up with row l & 7.
+// Packs the rows that a warp holds, 16 of them, 64 channels each: two groups a row, a half of the warp's lanes a group. The largest
+// of a group is found for all rows at a time, halving the rows that a lane still looks at: lane l of a half ends up with row l.
 // whole: all rows and channels are there, and pairs of codes lie on even addresses
-__device__ __forceinline__ void pack_rows(const float2 (&v)[kSteps], unsigned char *codes, unsigned char *scales, long long row, int width, int ch,
+__device__ __forceinline__ void pack_rows(const float2 (&v)[kFwdSteps], unsigned char *codes, unsigned char *scales, long long row, int width, int ch,
                                           bool whole, int cnt, int nch)
 {
     const int lane = threadIdx.x & 31;
-    unsigned m[kSteps];
+    unsigned m[kFwdSteps];
     bool again = false;
     for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
+        for (int s = 0; s < kFwdSteps; ++s) {
             const unsigned x = magnitude_bits(v[s].x), y = magnitude_bits(v[s].y);
             m[s] = pass ? max(bits_finite(x) ? x : 0u, bits_finite(y) ? y : 0u) : max(x, y);
             if (s >= cnt) m[s] = 0u;
         }
 #pragma unroll
-        for (int h = kSteps / 2; h > 0; h >>= 1)
+        for (int h = kFwdSteps / 2; h > 0; h >>= 1)
 #pragma unroll
             for (int s = 0; s < h; ++s) {
                 const bool upper = lane & h;
                 const unsigned give = upper ? m[s] : m[s + h], keep = upper ? m[s + h] : m[s];
                 m[s] = max(keep, __shfl_xor_sync(0xffffffffu, give, h));
             }
-        m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], 8));
         if (pass == 0) {
             again = __any_sync(0xffffffffu, m[0] > kPackLargest);
             if (!again) break;
@@ -271,14 +271,14 @@ __device__ __forceinline__ void pack_rows(const float2 (&v)[kSteps], unsigned ch
     if (!again && whole) {
         const float inverse = pack_inverse(scale);
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s, at += width) {
+        for (int s = 0; s < kFwdSteps; ++s, at += width) {
             const float2 c = fma2(v[s], two(__shfl_sync(0xffffffffu, inverse, (lane & 16) | s)), two(12582912.0f));
             *reinterpret_cast<unsigned short *>(at) = (unsigned short)__byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x0040);
         }
         return;
     }
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s, at += width) {
+    for (int s = 0; s < kFwdSteps; ++s, at += width) {
         const unsigned sc = __shfl_sync(0xffffffffu, scale, (lane & 16) | s);
         unsigned a, b;
         if (again) {
@@ -296,15 +296,16 @@ __device__ __forceinline__ void pack_rows(const float2 (&v)[kSteps], unsigned ch
     }
 }
 
-__device__ __forceinline__ float farthest(const float2 (&z)[kSteps])  // |z|; NaN does not count
+template <int S>
+__device__ __forceinline__ float farthest(const float2 (&z)[S])  // |z|; NaN does not count
 {
     float m = 0.0f;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) m = fmaxf(m, fmaxf(fabsf(z[s].x), fabsf(z[s].y)));
+    for (int s = 0; s < S; ++s) m = fmaxf(m, fmaxf(fabsf(z[s].x), fabsf(z[s].y)));
     return m;
 }
 
-// ---- a warp's next steps on their way to shared memory while the ones in hand are worked on: 8 rows of 64 values each
+// ---- a warp's next steps on their way to shared memory while the ones in hand are worked on: S rows of 64 values each
 __device__ __forceinline__ void copy16(void *to, const void *from)
 {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
@@ -315,45 +316,59 @@ __device__ __forceinline__ void copies_there()  // all lanes' of the warp
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
 }
-template <typename V>
+template <typename V, int S>
 struct Rows {
-    V v[kSteps][kSlab];
+    V v[S][kSlab];
+    static constexpr int kPer = 16 / sizeof(V), kChunks = kSlab / kPer, kAtOnce = 32 / kChunks;  // values of a copy, copies of a row, rows of a round
 };
-// from: first value of the slab in the first row; left: values of a row from there on
-template <typename V>
-__device__ __forceinline__ void ask(Rows<V> &to, const V *from, long long step, int cnt, int left)
+// Where a lane's first copy of a tile starts; from: first value of the slab in the first row
+template <typename V, int S>
+__device__ __forceinline__ const V *asks_from(const V *from, long long step)
 {
-    constexpr int kPer = 16 / sizeof(V), kChunks = kSlab / kPer;
+    using R = Rows<V, S>;
     const int lane = threadIdx.x & 31;
+    return from + lane / R::kChunks * step + lane % R::kChunks * R::kPer;
+}
+// left: values of a row from the slab's first on
+template <typename V, int S>
+__device__ __forceinline__ void ask(Rows<V, S> &to, const V *from, long long step, int cnt, int left)
+{
+    using R = Rows<V, S>;
+    const int lane = threadIdx.x & 31;
+    V *const place = &to.v[0][0] + lane * R::kPer;
+    if (cnt == S && left >= kSlab) {
 #pragma unroll
-    for (int i = 0; i < kSteps * kChunks; i += 32) {
-        const int at = i + lane, row = at / kChunks, col = at % kChunks * kPer;
-        if (at < kSteps * kChunks && row < cnt && col < left) copy16(&to.v[row][col], from + row * step + col);
+        for (int i = 0; i < S / R::kAtOnce; ++i, from += R::kAtOnce * step) copy16(place + i * 32 * R::kPer, from);
+    } else {
+        const int row = lane / R::kChunks, col = lane % R::kChunks * R::kPer;
+        for (int i = 0; i < S / R::kAtOnce; ++i, from += R::kAtOnce * step)
+            if (row + i * R::kAtOnce < cnt && col < left) copy16(place + i * 32 * R::kPer, from);
     }
 }
 // What has been asked for, as load_rows gives it
-template <typename T>
-__device__ __forceinline__ void take(const Rows<T> &from, int cnt, int nch, float end, float2 (&v)[kSteps])
+template <typename T, int S>
+__device__ __forceinline__ void take(const Rows<T, S> &from, int cnt, int nch, float end, float2 (&v)[S])
 {
     const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) v[s] = load2v(&from.v[s][lane * 2]);
-    if (cnt < kSteps || nch == 0)
+    for (int s = 0; s < S; ++s) v[s] = load2v(&from.v[s][lane * 2]);
+    if (cnt < S || nch == 0)
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) v[s] = s >= cnt ? two(end) : nch == 0 ? two(0.0f) : v[s];
+        for (int s = 0; s < S; ++s) v[s] = s >= cnt ? two(end) : nch == 0 ? two(0.0f) : v[s];
 }
 // The scale bytes of a warp's steps: lane 2 r + g has those of row r, group g of the slab
 __device__ __forceinline__ unsigned ask_scales(const unsigned char *scales, long long row, int per_row, int slab, int cnt)
 {
     const int lane = threadIdx.x & 31, r = lane >> 1, g = slab * (kSlab / kPackGroup) + (lane & 1);
-    return r < cnt && r < kSteps && g < per_row ? scales[(row + r) * per_row + g] : 127u;
+    return r < cnt && g < per_row ? scales[(row + r) * per_row + g] : 127u;
 }
-__device__ __forceinline__ void take_packed(const Rows<unsigned char> &from, unsigned scales, int cnt, int nch, float end, float2 (&v)[kSteps])
+template <int S>
+__device__ __forceinline__ void take_packed(const Rows<unsigned char, S> &from, unsigned scales, int cnt, int nch, float end, float2 (&v)[S])
 {
     const int lane = threadIdx.x & 31;
-    unsigned w[kSteps / 2], odd = 0;
+    unsigned w[S / 2], odd = 0;
 #pragma unroll
-    for (int s = 0; s < kSteps; s += 2) {  // the codes of two steps in a word
+    for (int s = 0; s < S; s += 2) {  // the codes of two steps in a word
         w[s / 2] = __byte_perm(*reinterpret_cast<const unsigned short *>(&from.v[s][lane * 2]),
                                *reinterpret_cast<const unsigned short *>(&from.v[s + 1][lane * 2]), 0x5410);
         odd |= unpack_odd(w[s / 2]);
@@ -363,17 +378,17 @@ __device__ __forceinline__ void take_packed(const Rows<unsigned char> &from, uns
         v[s + 1] = make_float2(f[2], f[3]);
     }
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) v[s] = mul2(v[s], two(pack_step(__shfl_sync(0xffffffffu, scales, 2 * s + (lane >> 4)))));
+    for (int s = 0; s < S; ++s) v[s] = mul2(v[s], two(pack_step(__shfl_sync(0xffffffffu, scales, 2 * s + (lane >> 4)))));
     if (odd) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
+        for (int s = 0; s < S; ++s) {
             const unsigned c = w[s / 2] >> (s % 2 * 16);
             v[s] = make_float2(unpack_special(v[s].x, c & 0xffu), unpack_special(v[s].y, (c >> 8) & 0xffu));
         }
     }
-    if (cnt < kSteps || nch == 0)
+    if (cnt < S || nch == 0)
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) v[s] = s >= cnt ? two(end) : nch == 0 ? two(0.0f) : v[s];
+        for (int s = 0; s < S; ++s) v[s] = s >= cnt ? two(end) : nch == 0 ? two(0.0f) : v[s];
 }
 
 // What a warp's, a CTA's steps amount to: (A, H) and, backward, (A, C) of a channel pair; two copies, so that one barrier lies between
@@ -392,9 +407,10 @@ struct Exchange {
 // ------------------------------------------------------------------ forward
 // PACKED: gate and value are codes, and only the states at the boundaries are wanted. KEEP: packs gate and value.
 template <typename T, bool PACKED, bool KEEP>
-__global__ void __launch_bounds__(kScanThreads, KEEP ? 2 : 3) scan_forward_k(const Scan p)
+__global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
 {
     using V = std::conditional_t<PACKED, unsigned char, T>;
+    constexpr int S = kFwdSteps;
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) Exchange<1> ex;
     const int rank = blockIdx.x % p.cluster, id = blockIdx.x / p.cluster;
@@ -415,18 +431,18 @@ __global__ void __launch_bounds__(kScanThreads, KEEP ? 2 : 3) scan_forward_k(con
         return;
     }
     if (PACKED && q.len <= p.interval) return;  // the whole cluster
-    const long long held = (long long)kTile * p.cluster;
-    long long t0 = (long long)rank * kTile + warp * kSteps;
+    const long long held = (long long)kFwdTile * p.cluster;
+    long long t0 = (long long)rank * kFwdTile + warp * S;
     // codes lie in rows of width, one after the other
     const long long gate_step = PACKED ? p.width : p.gate_step, value_step = PACKED ? p.width : p.value_step;
     const V *gate = (const V *)p.gate + (PACKED || p.offsets ? q.first * gate_step : seq * p.gate_seq) + t0 * gate_step + slab * kSlab;
     const V *value = (const V *)p.value + (PACKED || p.offsets ? q.first * value_step : seq * p.value_seq) + t0 * value_step + slab * kSlab;
     const int per_row = (p.width + kPackGroup - 1) / kPackGroup, left = p.width - slab * kSlab;
-    Rows<V> &zs = reinterpret_cast<Rows<V> *>(dynamic)[warp], &us = reinterpret_cast<Rows<V> *>(dynamic)[kScanWarps + warp];
+    Rows<V, S> &zs = reinterpret_cast<Rows<V, S> *>(dynamic)[warp], &us = reinterpret_cast<Rows<V, S> *>(dynamic)[kScanWarps + warp];
     unsigned zsc = 0, usc = 0;
     const bool wide = p.wide;
     auto ask_all = [&](long long t) {
-        const int cnt = (int)min((long long)kSteps, max(0LL, q.len - t));
+        const int cnt = (int)min((long long)S, max(0LL, q.len - t));
         ask(zs, gate, gate_step, cnt, left);
         ask(us, value, value_step, cnt, left);
         copies_on_their_way();
@@ -435,19 +451,23 @@ __global__ void __launch_bounds__(kScanThreads, KEEP ? 2 : 3) scan_forward_k(con
             usc = ask_scales(p.value_scales, q.first + t, per_row, slab, cnt);
         }
     };
-    if (wide) ask_all(t0);
+    if (wide) {
+        gate = asks_from<V, S>(gate, gate_step);
+        value = asks_from<V, S>(value, value_step);
+        ask_all(t0);
+    }
     // a CTA's shared memory may be written to by others once it runs: waited for ahead of the first such store
     if (p.cluster > 1) cg::this_cluster().sync();
     const float inf = __uint_as_float(0x7f800000u);
-    for (int par = 0; t0 - (long long)rank * kTile - warp * kSteps < q.len; t0 += held, par ^= 1) {
-        const int cnt = (int)min((long long)kSteps, max(0LL, q.len - t0));
+    for (int par = 0; t0 - (long long)rank * kFwdTile - warp * S < q.len; t0 += held, par ^= 1) {
+        const int cnt = (int)min((long long)S, max(0LL, q.len - t0));
         // a step behind the end holds the state
-        float2 a[kSteps], b[kSteps];
+        float2 a[S], b[S];
         if (wide) {
             copies_there();
             if constexpr (PACKED) {
-                take_packed(zs, zsc, cnt, nch, inf, a);
-                take_packed(us, usc, cnt, nch, 0.0f, b);
+                take_packed<S>(zs, zsc, cnt, nch, inf, a);
+                take_packed<S>(us, usc, cnt, nch, 0.0f, b);
             } else {
                 take(zs, cnt, nch, inf, a);
                 take(us, cnt, nch, 0.0f, b);
@@ -457,23 +477,23 @@ __global__ void __launch_bounds__(kScanThreads, KEEP ? 2 : 3) scan_forward_k(con
             value += held * value_step;
             ask_all(t0 + held);
         } else if constexpr (PACKED) {
-            load_packed((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, inf, a);
-            load_packed((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, 0.0f, b);
+            load_packed<S>((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, inf, a);
+            load_packed<S>((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, 0.0f, b);
         } else {
-            load_rows<T>(gate + lane * 2, gate_step, vec, cnt, nch, inf, a);
-            load_rows<T>(value + lane * 2, value_step, vec, cnt, nch, 0.0f, b);
+            load_rows<T, S>(gate + lane * 2, gate_step, vec, cnt, nch, inf, a);
+            load_rows<T, S>(value + lane * 2, value_step, vec, cnt, nch, 0.0f, b);
             gate += held * gate_step;
             value += held * value_step;
         }
         if constexpr (KEEP) {
-            pack_rows(a, p.pack_gate, p.pack_gate_scales, q.first + t0, p.width, ch, vec && left >= kSlab && cnt == kSteps, cnt, nch);
-            pack_rows(b, p.pack_value, p.pack_value_scales, q.first + t0, p.width, ch, vec && left >= kSlab && cnt == kSteps, cnt, nch);
+            pack_rows(a, p.pack_gate, p.pack_gate_scales, q.first + t0, p.width, ch, vec && left >= kSlab && cnt == S, cnt, nch);
+            pack_rows(b, p.pack_value, p.pack_value_scales, q.first + t0, p.width, ch, vec && left >= kSlab && cnt == S, cnt, nch);
         }
         const bool special = farthest(a) >= kFar;
         float2 A = two(1.0f), H = two(0.0f);
         if (!special) {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
+            for (int s = 0; s < S; ++s) {
                 float2 w, n;
                 gates(a[s], w, n);
                 a[s] = w;
@@ -483,7 +503,7 @@ __global__ void __launch_bounds__(kScanThreads, KEEP ? 2 : 3) scan_forward_k(con
             }
         } else {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
+            for (int s = 0; s < S; ++s) {
                 float2 w, n;
                 gates_any(a[s], w, n);
                 a[s] = w;
@@ -497,7 +517,7 @@ __global__ void __launch_bounds__(kScanThreads, KEEP ? 2 : 3) scan_forward_k(con
         float2 h = carry;
         if (p.cluster > 1) {
             cg::cluster_group cluster = cg::this_cluster();
-            // every warp composes the CTA's steps and tells every eighth CTA
+            // every warp composes the CTA's steps and tells every fourth CTA
             float2 ta = two(1.0f), th = two(0.0f);
 #pragma unroll
             for (int w = 0; w < kScanWarps; ++w) {
@@ -525,24 +545,24 @@ __global__ void __launch_bounds__(kScanThreads, KEEP ? 2 : 3) scan_forward_k(con
                 carry = through(ex.warp[par][0][w][lane], carry);
             }
         }
-        // intervals are multiples of 64 steps: boundaries lie at the start of a thread's steps
+        // intervals are multiples of 32 steps: boundaries lie at the start of a thread's steps
         if (p.bounds && cnt > 0 && t0 > 0 && (t0 & (p.interval - 1)) == 0)
             store2(p.bounds + bound_row(p, seq, q, t0 / p.interval) * p.width + ch, vec, nch, h);
         if (!PACKED) {
-            T *const out = (T *)p.h + (q.first + t0) * p.width + ch;
+            T *out = (T *)p.h + (q.first + t0) * p.width + ch;
             if (!special) {
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s) a[s] = h = fma2(a[s], h, b[s]);
+                for (int s = 0; s < S; ++s) a[s] = h = fma2(a[s], h, b[s]);
             } else {
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s) a[s] = h = after(a[s], h, b[s]);
+                for (int s = 0; s < S; ++s) a[s] = h = after(a[s], h, b[s]);
             }
-            if (vec && nch == 2 && cnt == kSteps) {
+            if (vec && nch == 2 && cnt == S) {
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s) store2v(out + (long long)s * p.width, a[s]);
+                for (int s = 0; s < S; ++s, out += p.width) store2v(out, a[s]);
             } else {
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s)
+                for (int s = 0; s < S; ++s)
                     if (s < cnt) store2(out + (long long)s * p.width, vec, nch, a[s]);
             }
             if (p.last && cnt > 0 && t0 + cnt == q.len) store2(p.last + state_at, vec, nch, h);
@@ -552,9 +572,10 @@ __global__ void __launch_bounds__(kScanThreads, KEEP ? 2 : 3) scan_forward_k(con
 
 // ------------------------------------------------------------------ backward
 template <typename T, bool PACKED>
-__global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
+__global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
 {
     using V = std::conditional_t<PACKED, unsigned char, T>;
+    constexpr int S = kBwdSteps;
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) Exchange<2> ex;
     const int rank = blockIdx.x % p.cluster, id = blockIdx.x / p.cluster;
@@ -576,19 +597,21 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
     const V *const gate = (const V *)p.gate + (PACKED || p.offsets ? q.first * gate_step : seq * p.gate_seq) + slab * kSlab;
     const V *const value = (const V *)p.value + (PACKED || p.offsets ? q.first * value_step : seq * p.value_seq) + slab * kSlab;
     const T *const grad = (const T *)p.gh + q.first * p.width + slab * kSlab;
-    const long long held = (long long)kTile * p.cluster;  // == p.interval
+    const long long held = (long long)kBwdTile * p.cluster;  // == p.interval
     const int per_row = (p.width + kPackGroup - 1) / kPackGroup, left = p.width - slab * kSlab;
-    Rows<T> &gs = reinterpret_cast<Rows<T> *>(dynamic)[warp];
-    Rows<V> *const inputs = reinterpret_cast<Rows<V> *>(dynamic + kScanWarps * sizeof(Rows<T>));
-    Rows<V> &zs = inputs[warp], &us = inputs[kScanWarps + warp];
+    Rows<T, S> &gs = reinterpret_cast<Rows<T, S> *>(dynamic)[warp];
+    Rows<V, S> *const inputs = reinterpret_cast<Rows<V, S> *>(dynamic + kScanWarps * sizeof(Rows<T, S>));
+    Rows<V, S> &zs = inputs[warp], &us = inputs[kScanWarps + warp];
     unsigned zsc = 0, usc = 0;
     const bool wide = p.wide;
+    const V *const gate_from = asks_from<V, S>(gate, gate_step), *const value_from = asks_from<V, S>(value, value_step);
+    const T *const grad_from = asks_from<T, S>(grad, p.width);
     auto ask_all = [&](long long t) {
-        const int cnt = (int)min((long long)kSteps, max(0LL, q.len - t));
+        const int cnt = (int)min((long long)S, max(0LL, q.len - t));
         if (cnt <= 0) return;
-        ask(zs, gate + t * gate_step, gate_step, cnt, left);
-        ask(us, value + t * value_step, value_step, cnt, left);
-        ask(gs, grad + t * p.width, p.width, cnt, left);
+        ask(zs, gate_from + t * gate_step, gate_step, cnt, left);
+        ask(us, value_from + t * value_step, value_step, cnt, left);
+        ask(gs, grad_from + t * p.width, (long long)p.width, cnt, left);
         copies_on_their_way();
         if (PACKED) {
             zsc = ask_scales(p.gate_scales, q.first + t, per_row, slab, cnt);
@@ -596,21 +619,21 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
         }
     };
     int par = 0;
-    const long long last = (q.len + held - 1) / held - 1, mine = (long long)rank * kTile + warp * kSteps;
+    const long long last = (q.len + held - 1) / held - 1, mine = (long long)rank * kBwdTile + warp * S;
     if (wide && last >= 0) ask_all(last * held + mine);
     // a CTA's shared memory may be written to by others once it runs: waited for ahead of the first such store
     if (p.cluster > 1) cg::this_cluster().sync();
     const float inf = __uint_as_float(0x7f800000u);
     for (long long k = last; k >= 0; --k, par ^= 1) {
         const long long t0 = k * held + mine;
-        const int cnt = (int)min((long long)kSteps, max(0LL, q.len - t0));
+        const int cnt = (int)min((long long)S, max(0LL, q.len - t0));
         // a step behind the end holds the state and has no gradient of its own
-        float2 a[kSteps], n[kSteps], u[kSteps], g[kSteps], h = two(0.0f);
+        float2 a[S], n[S], u[S], g[S], h = two(0.0f);
         if (wide) {
             copies_there();
             if constexpr (PACKED) {
-                take_packed(zs, zsc, cnt, nch, inf, a);
-                take_packed(us, usc, cnt, nch, 0.0f, u);
+                take_packed<S>(zs, zsc, cnt, nch, inf, a);
+                take_packed<S>(us, usc, cnt, nch, 0.0f, u);
             } else {
                 take(zs, cnt, nch, inf, a);
                 take(us, cnt, nch, 0.0f, u);
@@ -620,13 +643,13 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
             if (k > 0) ask_all(t0 - held);
         } else {
             if constexpr (PACKED) {
-                load_packed((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, inf, a);
-                load_packed((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, 0.0f, u);
+                load_packed<S>((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, inf, a);
+                load_packed<S>((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, 0.0f, u);
             } else {
-                load_rows<T>(gate + lane * 2 + t0 * gate_step, gate_step, vec, cnt, nch, inf, a);
-                load_rows<T>(value + lane * 2 + t0 * value_step, value_step, vec, cnt, nch, 0.0f, u);
+                load_rows<T, S>(gate + lane * 2 + t0 * gate_step, gate_step, vec, cnt, nch, inf, a);
+                load_rows<T, S>(value + lane * 2 + t0 * value_step, value_step, vec, cnt, nch, 0.0f, u);
             }
-            load_rows<T>(grad + lane * 2 + t0 * p.width, p.width, vec, cnt, nch, 0.0f, g);
+            load_rows<T, S>(grad + lane * 2 + t0 * p.width, p.width, vec, cnt, nch, 0.0f, g);
         }
         if (k > 0)
             h = load2(p.bounds + bound_row(p, seq, q, k) * p.width + ch, vec, nch);
@@ -636,7 +659,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
         const bool special = farthest(a) >= kFar;
         if (!special) {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
+            for (int s = 0; s < S; ++s) {
                 float2 w;
                 gates(a[s], w, n[s]);
                 a[s] = w;
@@ -644,10 +667,10 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
                 A = mul2(A, w);
             }
 #pragma unroll
-            for (int s = kSteps - 1; s >= 0; --s) C = mul2(a[s], add2(g[s], C));
+            for (int s = S - 1; s >= 0; --s) C = mul2(a[s], add2(g[s], C));
         } else {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
+            for (int s = 0; s < S; ++s) {
                 float2 w;
                 gates_any(a[s], w, n[s]);
                 a[s] = w;
@@ -656,7 +679,7 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
                 A = more(A, w);
             }
 #pragma unroll
-            for (int s = kSteps - 1; s >= 0; --s) C = looked_at(a[s], mul2(a[s], add2(g[s], C)));
+            for (int s = S - 1; s >= 0; --s) C = looked_at(a[s], mul2(a[s], add2(g[s], C)));
         }
         ex.warp[par][0][warp][lane] = map_of(A, H);
         ex.warp[par][1][warp][lane] = map_of(A, C);
@@ -702,13 +725,13 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
         // u becomes a n (h before the step - u), then both gradients in place of g and u
         if (!special) {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
+            for (int s = 0; s < S; ++s) {
                 const float2 d = fma2(u[s], two(-1.0f), h);
                 h = fma2(a[s], h, mul2(n[s], u[s]));
                 u[s] = mul2(mul2(a[s], n[s]), d);
             }
 #pragma unroll
-            for (int s = kSteps - 1; s >= 0; --s) {
+            for (int s = S - 1; s >= 0; --s) {
                 const float2 dh = add2(g[s], c);
                 u[s] = mul2(u[s], dh);
                 g[s] = mul2(n[s], dh);
@@ -716,13 +739,13 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
             }
         } else {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
+            for (int s = 0; s < S; ++s) {
                 const float2 d = fma2(u[s], two(-1.0f), h), w = mul2(a[s], n[s]);
                 h = after(a[s], h, mul2(n[s], u[s]));
                 u[s] = looked_at(w, mul2(w, d));
             }
 #pragma unroll
-            for (int s = kSteps - 1; s >= 0; --s) {
+            for (int s = S - 1; s >= 0; --s) {
                 const float2 dh = add2(g[s], c);
                 u[s] = mul2(u[s], dh);
                 g[s] = mul2(n[s], dh);
@@ -730,16 +753,16 @@ __global__ void __launch_bounds__(kScanThreads, 2) scan_backward_k(const Scan p)
             }
         }
         const long long at = (q.first + t0) * p.width + ch;
-        T *const dz = (T *)p.dgate + at, *const du = (T *)p.dvalue + at;
-        if (vec && nch == 2 && cnt == kSteps) {
+        T *dz = (T *)p.dgate + at, *du = (T *)p.dvalue + at;
+        if (vec && nch == 2 && cnt == S) {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                store2v(dz + (long long)s * p.width, u[s]);
-                store2v(du + (long long)s * p.width, g[s]);
+            for (int s = 0; s < S; ++s, dz += p.width, du += p.width) {
+                store2v(dz, u[s]);
+                store2v(du, g[s]);
             }
         } else {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s)
+            for (int s = 0; s < S; ++s)
                 if (s < cnt) {
                     store2(dz + (long long)s * p.width, vec, nch, u[s]);
                     store2(du + (long long)s * p.width, vec, nch, g[s]);
@@ -792,12 +815,12 @@ static int scan_check(int n, long long steps, long long total, int width, int dt
 static int scan_interval(int n, long long steps, long long total, int width, int dtype, bool ragged)
 {
     const long long mean = ragged ? total / (n > 0 ? n : 1) : steps;
-    return kTile * scan_cluster(n, mean, width, dtype == GN_F32 ? 4 : 2, true);
+    return kBwdTile * scan_cluster(n, mean, width, dtype == GN_F32 ? 4 : 2, true);
 }
 
-static int launch_scan(void (*kern)(const Scan), const Scan &p, size_t value_bytes, const char *what, cudaStream_t st)
+static int launch_scan(void (*kern)(const Scan), const Scan &p, size_t tile_bytes, const char *what, cudaStream_t st)
 {
-    const size_t smem = p.wide ? value_bytes * kTile * kSlab : 0;
+    const size_t smem = p.wide ? tile_bytes * kSlab : 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((p.n + (p.offsets ? 1LL : 0LL)) * p.slabs * p.cluster));
     cfg.blockDim = dim3(kScanThreads);
@@ -824,7 +847,7 @@ template <typename T>
 static int scan_forward(Scan &p, cudaStream_t st)
 {
     p.slabs = (p.width + kSlab - 1) / kSlab;
-    return launch_scan(p.pack_gate ? scan_forward_k<T, false, true> : scan_forward_k<T, false, false>, p, 2 * sizeof(T), "gated_scan", st);
+    return launch_scan(p.pack_gate ? scan_forward_k<T, false, true> : scan_forward_k<T, false, false>, p, kFwdTile * 2 * sizeof(T), "gated_scan", st);
 }
 
 template <typename T>
@@ -832,10 +855,10 @@ static int scan_backward(Scan &p, bool packed, bool long_sequences, cudaStream_t
 {
     p.slabs = (p.width + kSlab - 1) / kSlab;
     if (packed && long_sequences) {  // the states that the codes lead to
-        const int rc = launch_scan(scan_forward_k<T, true, false>, p, 2, "gated_scan states", st);
+        const int rc = launch_scan(scan_forward_k<T, true, false>, p, kFwdTile * 2, "gated_scan states", st);
         if (rc != GN_OK) return rc;
     }
-    return launch_scan(packed ? scan_backward_k<T, true> : scan_backward_k<T, false>, p, (packed ? 2 : 2 * sizeof(T)) + sizeof(T), "gated_scan backward", st);
+    return launch_scan(packed ? scan_backward_k<T, true> : scan_backward_k<T, false>, p, kBwdTile * ((packed ? 2 : 2 * sizeof(T)) + sizeof(T)), "gated_scan backward", st);
 }
 
 }  // namespace gn
@@ -903,7 +926,7 @@ GN_API int gn_gated_scan_backward(const void *gate, const void *value, const voi
     p.interval = scan_interval(n, steps, total, width, dtype, offsets != nullptr);
     p.gate_seq = gate_seq; p.gate_step = gate_step; p.value_seq = value_seq; p.value_step = value_step;
     p.n = n; p.steps = steps; p.total = total; p.width = width;
-    p.cluster = p.interval / kTile;
+    p.cluster = p.interval / kBwdTile;
     const int size = dtype == GN_F32 ? 4 : 2, in = gate_scales ? 1 : size;
     p.vec = width % 2 == 0 && gate_seq % 2 == 0 && gate_step % 2 == 0 && value_seq % 2 == 0 && value_step % 2 == 0 && aligned(gate, 2 * in) &&
             aligned(value, 2 * in) && aligned(grad_h, 2 * size) && aligned(grad_gate, 2 * size) && aligned(grad_value, 2 * size) &&
