@@ -43,8 +43,8 @@ struct Scan {
     void *h;
     float *last;
     unsigned char *pack_gate, *pack_value, *pack_gate_scales, *pack_value_scales;
-    float *bounds;  // state ahead of every interval-th step of a sequence
-    int interval;   // a power of two
+    float *bounds;  // state ahead of every 2^interval_log2-th step of a sequence
+    int interval_log2;
     const void *gh;
     const float *glast;
     void *dgate, *dvalue;
@@ -70,11 +70,11 @@ __device__ __forceinline__ Place sequence(const Scan &p, int seq)
     }
     return s;
 }
-// row of p.bounds that holds the state ahead of step interval * k of a sequence, k >= 1
+// row of p.bounds that holds the state ahead of step k << interval_log2 of a sequence, k >= 1
 __device__ __forceinline__ long long bound_row(const Scan &p, int seq, const Place &s, long long k)
 {
-    if (!p.offsets) return seq * ((p.steps + p.interval - 1) / p.interval) + k;
-    return s.first / p.interval + seq + k;  // a sequence has at most one boundary more than its rows have multiples of the interval
+    if (!p.offsets) return seq * ((p.steps + (1LL << p.interval_log2) - 1) >> p.interval_log2) + k;
+    return (s.first >> p.interval_log2) + seq + k;  // a sequence has at most one boundary more than its rows have multiples of the interval
 }
 
 // ---- pairs
@@ -235,63 +235,99 @@ __device__ __forceinline__ void load_packed(const unsigned char *codes, const un
     }
 }
 
-// Packs the rows that a warp holds, 16 of them, 64 channels each: two groups a row, a half of the warp's lanes a group. The largest
-// of a group is found for all rows at a time, halving the rows that a lane still looks at: lane l of a half ends up with row l.
-// whole: all rows and channels are there, and pairs of codes lie on even addresses
-__device__ __forceinline__ void pack_rows(const float2 (&v)[kFwdSteps], unsigned char *codes, unsigned char *scales, long long row, int width, int ch,
-                                          bool whole, int cnt, int nch)
+// ---- packing of the rows that a warp holds, 16 of gate and of value, 64 channels each: two groups a row, half of the warp's lanes a group.
+// The scale of a group follows from the upper 16 bits of its largest magnitude, rounded up (125 / 64 has no more), so that of gate and value are
+// looked for together, as two 16-bit numbers; and for all rows at a time, halving the rows that a lane still looks at: lane l of a
+// half ends up with row l. What is not finite is above kLargestKey, and so is a group that would need 2^122.
+constexpr unsigned kLargestKey = kPackLargest >> 16;
+__device__ __forceinline__ float larger(float2 v)  // magnitude; NaN where one of the two is
+{
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(v.x)), "f"(fabsf(v.y)));
+    return m;
+}
+__device__ __forceinline__ unsigned keys_of(float gate, float value)
+{
+    return __byte_perm(__float_as_uint(gate) + 0xffffu, __float_as_uint(value) + 0xffffu, 0x7632);
+}
+__device__ __forceinline__ unsigned scale_of_key(unsigned key)
+{
+    return (unsigned)max((int)(key >> 7) - 6 + ((key & 0x7fu) > 0x7au ? 1 : 0), 1);
+}
+// the largest of 16 lanes, row by row
+__device__ __forceinline__ unsigned rows_to_lanes(unsigned (&m)[kFwdSteps])
 {
     const int lane = threadIdx.x & 31;
-    unsigned m[kFwdSteps];
-    bool again = false;
-    for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
-        for (int s = 0; s < kFwdSteps; ++s) {
-            const unsigned x = magnitude_bits(v[s].x), y = magnitude_bits(v[s].y);
-            m[s] = pass ? max(bits_finite(x) ? x : 0u, bits_finite(y) ? y : 0u) : max(x, y);
-            if (s >= cnt) m[s] = 0u;
-        }
+    for (int h = kFwdSteps / 2; h > 0; h >>= 1) {
+        const bool upper = lane & h;
 #pragma unroll
-        for (int h = kFwdSteps / 2; h > 0; h >>= 1)
-#pragma unroll
-            for (int s = 0; s < h; ++s) {
-                const bool upper = lane & h;
-                const unsigned give = upper ? m[s] : m[s + h], keep = upper ? m[s + h] : m[s];
-                m[s] = max(keep, __shfl_xor_sync(0xffffffffu, give, h));
-            }
-        if (pass == 0) {
-            again = __any_sync(0xffffffffu, m[0] > kPackLargest);
-            if (!again) break;
+        for (int s = 0; s < h; ++s) {
+            const unsigned give = upper ? m[s] : m[s + h], keep = upper ? m[s + h] : m[s];
+            m[s] = __vmaxu2(keep, __shfl_xor_sync(0xffffffffu, give, h));
         }
     }
-    const unsigned scale = pack_scale(m[0]);
-    const int per_row = (width + kPackGroup - 1) / kPackGroup, group = ch / kPackGroup;
-    if ((lane & 15) < cnt && group < per_row) scales[(row + (lane & 15)) * per_row + group] = (unsigned char)scale;
-    unsigned char *at = codes + row * width + ch;
-    if (!again && whole) {
-        const float inverse = pack_inverse(scale);
+    return m[0];
+}
+struct PackTo {
+    unsigned char *gate, *value, *gate_scales, *value_scales;
+};
+// whole: all rows and channels are there, and pairs of codes lie on even addresses
+__device__ __forceinline__ void pack_rows(const float2 (&z)[kFwdSteps], const float2 (&u)[kFwdSteps], const PackTo &to, long long row, int width, int ch,
+                                          bool whole, int cnt, int nch)
+{
+    const int lane = threadIdx.x & 31, per_row = (width + kPackGroup - 1) / kPackGroup, group = ch / kPackGroup;
+    unsigned m[kFwdSteps];
 #pragma unroll
-        for (int s = 0; s < kFwdSteps; ++s, at += width) {
-            const float2 c = fma2(v[s], two(__shfl_sync(0xffffffffu, inverse, (lane & 16) | s)), two(12582912.0f));
-            *reinterpret_cast<unsigned short *>(at) = (unsigned short)__byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x0040);
+    for (int s = 0; s < kFwdSteps; ++s) m[s] = keys_of(larger(z[s]), larger(u[s]));
+    if (!whole)
+#pragma unroll
+        for (int s = 0; s < kFwdSteps; ++s)
+            if (s >= cnt) m[s] = 0u;
+    unsigned key = rows_to_lanes(m);
+    const bool rare = __any_sync(0xffffffffu, (key & 0xffffu) > kLargestKey || key >> 16 > kLargestKey);
+    if (rare) {  // once more over what is finite
+#pragma unroll
+        for (int s = 0; s < kFwdSteps; ++s) {
+            float2 f = z[s], g = u[s];
+            f.x = bits_finite(magnitude_bits(f.x)) ? f.x : 0.0f;
+            f.y = bits_finite(magnitude_bits(f.y)) ? f.y : 0.0f;
+            g.x = bits_finite(magnitude_bits(g.x)) ? g.x : 0.0f;
+            g.y = bits_finite(magnitude_bits(g.y)) ? g.y : 0.0f;
+            m[s] = s < cnt ? keys_of(larger(f), larger(g)) : 0u;
+        }
+        key = rows_to_lanes(m);
+    }
+    const unsigned zs = scale_of_key(key & 0xffffu), us = scale_of_key(key >> 16);
+    if ((lane & 15) < cnt && group < per_row) {
+        const long long at = (row + (lane & 15)) * per_row + group;
+        to.gate_scales[at] = (unsigned char)zs;
+        to.value_scales[at] = (unsigned char)us;
+    }
+    unsigned char *zc = to.gate + row * width + ch, *uc = to.value + row * width + ch;
+    if (whole && !rare) {
+        // the upper halves of both 2^-e (the lower ones are 0)
+        const unsigned inverses = __byte_perm(__float_as_uint(pack_inverse(zs)), __float_as_uint(pack_inverse(us)), 0x7632);
+        const float2 magic = two(12582912.0f);
+#pragma unroll
+        for (int s = 0; s < kFwdSteps; ++s, zc += width, uc += width) {
+            const unsigned both = __shfl_sync(0xffffffffu, inverses, (lane & 16) | s);
+            const float2 c = fma2(z[s], two(__uint_as_float(both << 16)), magic), d = fma2(u[s], two(__uint_as_float(both & 0xffff0000u)), magic);
+            *reinterpret_cast<unsigned short *>(zc) = (unsigned short)__byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x0040);
+            *reinterpret_cast<unsigned short *>(uc) = (unsigned short)__byte_perm(__float_as_uint(d.x), __float_as_uint(d.y), 0x0040);
         }
         return;
     }
 #pragma unroll
-    for (int s = 0; s < kFwdSteps; ++s, at += width) {
-        const unsigned sc = __shfl_sync(0xffffffffu, scale, (lane & 16) | s);
-        unsigned a, b;
-        if (again) {
-            a = pack_code_any(v[s].x, sc);
-            b = pack_code_any(v[s].y, sc);
-        } else {
-            const float inv = pack_inverse(sc);
-            a = pack_code(v[s].x, inv);
-            b = pack_code(v[s].y, inv);
-        }
-        if (s < cnt) {
-            if (nch > 0) at[0] = (unsigned char)a;
-            if (nch > 1) at[1] = (unsigned char)b;
+    for (int s = 0; s < kFwdSteps; ++s, zc += width, uc += width) {
+        const unsigned both = __shfl_sync(0xffffffffu, zs | us << 16, (lane & 16) | s);
+        if (s < cnt && nch > 0) {
+            zc[0] = (unsigned char)pack_code_any(z[s].x, both & 0xffffu);
+            uc[0] = (unsigned char)pack_code_any(u[s].x, both >> 16);
+            if (nch > 1) {
+                zc[1] = (unsigned char)pack_code_any(z[s].y, both & 0xffffu);
+                uc[1] = (unsigned char)pack_code_any(u[s].y, both >> 16);
+            }
         }
     }
 }
@@ -356,39 +392,59 @@ __device__ __forceinline__ void take(const Rows<T, S> &from, int cnt, int nch, f
 #pragma unroll
         for (int s = 0; s < S; ++s) v[s] = s >= cnt ? two(end) : nch == 0 ? two(0.0f) : v[s];
 }
-// The scale bytes of a warp's steps: lane 2 r + g has those of row r, group g of the slab
-__device__ __forceinline__ unsigned ask_scales(const unsigned char *scales, long long row, int per_row, int slab, int cnt)
+// The scale bytes of gate and of value for a warp's steps: lane 2 r + g has row r, group g of the slab
+__device__ __forceinline__ unsigned ask_scales(const Scan &p, long long row, int per_row, int slab, int cnt)
 {
     const int lane = threadIdx.x & 31, r = lane >> 1, g = slab * (kSlab / kPackGroup) + (lane & 1);
-    return r < cnt && g < per_row ? scales[(row + r) * per_row + g] : 127u;
+    if (r >= cnt || g >= per_row) return 127u | 127u << 16;
+    const long long at = (row + r) * per_row + g;
+    return p.gate_scales[at] | (unsigned)p.value_scales[at] << 16;
 }
+// gate and value as their codes give them
 template <int S>
-__device__ __forceinline__ void take_packed(const Rows<unsigned char, S> &from, unsigned scales, int cnt, int nch, float end, float2 (&v)[S])
+__device__ __forceinline__ void take_packed(const Rows<unsigned char, S> &gates, const Rows<unsigned char, S> &values, unsigned scales, int cnt, int nch,
+                                            float end, float2 (&z)[S], float2 (&u)[S])
 {
     const int lane = threadIdx.x & 31;
-    unsigned w[S / 2], odd = 0;
-#pragma unroll
-    for (int s = 0; s < S; s += 2) {  // the codes of two steps in a word
-        w[s / 2] = __byte_perm(*reinterpret_cast<const unsigned short *>(&from.v[s][lane * 2]),
-                               *reinterpret_cast<const unsigned short *>(&from.v[s + 1][lane * 2]), 0x5410);
-        odd |= unpack_odd(w[s / 2]);
+    unsigned wz[S / 2], wu[S / 2];
+    float far = 0.0f;
+    auto word = [&](const Rows<unsigned char, S> &from, int s) {  // the codes of two steps
+        return __byte_perm(*reinterpret_cast<const unsigned short *>(&from.v[s][lane * 2]), *reinterpret_cast<const unsigned short *>(&from.v[s + 1][lane * 2]),
+                           0x5410);
+    };
+    auto whole = [&](unsigned w, float2 &a, float2 &b) {
         float f[4];
-        unpack4_finite(w[s / 2], f);
-        v[s] = make_float2(f[0], f[1]);
-        v[s + 1] = make_float2(f[2], f[3]);
-    }
+        unpack4_finite(w, f);
+        far = fmaxf(fmaxf(far, fmaxf(fabsf(f[0]), fabsf(f[1]))), fmaxf(fabsf(f[2]), fabsf(f[3])));
+        a = make_float2(f[0], f[1]);
+        b = make_float2(f[2], f[3]);
+    };
 #pragma unroll
-    for (int s = 0; s < S; ++s) v[s] = mul2(v[s], two(pack_step(__shfl_sync(0xffffffffu, scales, 2 * s + (lane >> 4)))));
-    if (odd) {
+    for (int s = 0; s < S; s += 2) {
+        whole(wz[s / 2] = word(gates, s), z[s], z[s + 1]);
+        whole(wu[s / 2] = word(values, s), u[s], u[s + 1]);
+    }
+    const unsigned steps = scales << 7;  // the upper halves of both 2^e (the lower ones are 0)
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const unsigned both = __shfl_sync(0xffffffffu, steps, 2 * s + (lane >> 4));
+        z[s] = mul2(z[s], two(__uint_as_float(both << 16)));
+        u[s] = mul2(u[s], two(__uint_as_float(both & 0xffff0000u)));
+    }
+    if (far > 125.0f) {  // some code stands for what is not finite
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const unsigned c = w[s / 2] >> (s % 2 * 16);
-            v[s] = make_float2(unpack_special(v[s].x, c & 0xffu), unpack_special(v[s].y, (c >> 8) & 0xffu));
+            const unsigned c = wz[s / 2] >> (s % 2 * 16), d = wu[s / 2] >> (s % 2 * 16);
+            z[s] = make_float2(unpack_special(z[s].x, c & 0xffu), unpack_special(z[s].y, (c >> 8) & 0xffu));
+            u[s] = make_float2(unpack_special(u[s].x, d & 0xffu), unpack_special(u[s].y, (d >> 8) & 0xffu));
         }
     }
     if (cnt < S || nch == 0)
 #pragma unroll
-        for (int s = 0; s < S; ++s) v[s] = s >= cnt ? two(end) : nch == 0 ? two(0.0f) : v[s];
+        for (int s = 0; s < S; ++s) {
+            z[s] = s >= cnt ? two(end) : nch == 0 ? two(0.0f) : z[s];
+            u[s] = s >= cnt || nch == 0 ? two(0.0f) : u[s];
+        }
 }
 
 // What a warp's, a CTA's steps amount to: (A, H) and, backward, (A, C) of a channel pair; two copies, so that one barrier lies between
@@ -430,7 +486,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
         if (!PACKED && p.last && rank == 0 && warp == 0) store2(p.last + state_at, vec, nch, carry);
         return;
     }
-    if (PACKED && q.len <= p.interval) return;  // the whole cluster
+    if (PACKED && q.len <= 1LL << p.interval_log2) return;  // the whole cluster
     const long long held = (long long)kFwdTile * p.cluster;
     long long t0 = (long long)rank * kFwdTile + warp * S;
     // codes lie in rows of width, one after the other
@@ -439,7 +495,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
     const V *value = (const V *)p.value + (PACKED || p.offsets ? q.first * value_step : seq * p.value_seq) + t0 * value_step + slab * kSlab;
     const int per_row = (p.width + kPackGroup - 1) / kPackGroup, left = p.width - slab * kSlab;
     Rows<V, S> &zs = reinterpret_cast<Rows<V, S> *>(dynamic)[warp], &us = reinterpret_cast<Rows<V, S> *>(dynamic)[kScanWarps + warp];
-    unsigned zsc = 0, usc = 0;
+    unsigned scales = 0;
     const bool wide = p.wide;
     auto ask_all = [&](long long t) {
         const int cnt = (int)min((long long)S, max(0LL, q.len - t));
@@ -447,8 +503,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
         ask(us, value, value_step, cnt, left);
         copies_on_their_way();
         if (PACKED) {
-            zsc = ask_scales(p.gate_scales, q.first + t, per_row, slab, cnt);
-            usc = ask_scales(p.value_scales, q.first + t, per_row, slab, cnt);
+            scales = ask_scales(p, q.first + t, per_row, slab, cnt);
         }
     };
     if (wide) {
@@ -466,8 +521,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
         if (wide) {
             copies_there();
             if constexpr (PACKED) {
-                take_packed<S>(zs, zsc, cnt, nch, inf, a);
-                take_packed<S>(us, usc, cnt, nch, 0.0f, b);
+                take_packed<S>(zs, us, scales, cnt, nch, inf, a, b);
             } else {
                 take(zs, cnt, nch, inf, a);
                 take(us, cnt, nch, 0.0f, b);
@@ -486,8 +540,8 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
             value += held * value_step;
         }
         if constexpr (KEEP) {
-            pack_rows(a, p.pack_gate, p.pack_gate_scales, q.first + t0, p.width, ch, vec && left >= kSlab && cnt == S, cnt, nch);
-            pack_rows(b, p.pack_value, p.pack_value_scales, q.first + t0, p.width, ch, vec && left >= kSlab && cnt == S, cnt, nch);
+            const PackTo to = {p.pack_gate, p.pack_value, p.pack_gate_scales, p.pack_value_scales};
+            pack_rows(a, b, to, q.first + t0, p.width, ch, vec && left >= kSlab && cnt == S, cnt, nch);
         }
         const bool special = farthest(a) >= kFar;
         float2 A = two(1.0f), H = two(0.0f);
@@ -546,8 +600,8 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
             }
         }
         // intervals are multiples of 32 steps: boundaries lie at the start of a thread's steps
-        if (p.bounds && cnt > 0 && t0 > 0 && (t0 & (p.interval - 1)) == 0)
-            store2(p.bounds + bound_row(p, seq, q, t0 / p.interval) * p.width + ch, vec, nch, h);
+        if (p.bounds && cnt > 0 && t0 > 0 && (t0 & ((1 << p.interval_log2) - 1)) == 0)
+            store2(p.bounds + bound_row(p, seq, q, t0 >> p.interval_log2) * p.width + ch, vec, nch, h);
         if (!PACKED) {
             T *out = (T *)p.h + (q.first + t0) * p.width + ch;
             if (!special) {
@@ -597,12 +651,12 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
     const V *const gate = (const V *)p.gate + (PACKED || p.offsets ? q.first * gate_step : seq * p.gate_seq) + slab * kSlab;
     const V *const value = (const V *)p.value + (PACKED || p.offsets ? q.first * value_step : seq * p.value_seq) + slab * kSlab;
     const T *const grad = (const T *)p.gh + q.first * p.width + slab * kSlab;
-    const long long held = (long long)kBwdTile * p.cluster;  // == p.interval
+    const int held_log2 = p.interval_log2, held = 1 << held_log2;  // kBwdTile * p.cluster
     const int per_row = (p.width + kPackGroup - 1) / kPackGroup, left = p.width - slab * kSlab;
     Rows<T, S> &gs = reinterpret_cast<Rows<T, S> *>(dynamic)[warp];
     Rows<V, S> *const inputs = reinterpret_cast<Rows<V, S> *>(dynamic + kScanWarps * sizeof(Rows<T, S>));
     Rows<V, S> &zs = inputs[warp], &us = inputs[kScanWarps + warp];
-    unsigned zsc = 0, usc = 0;
+    unsigned scales = 0;
     const bool wide = p.wide;
     const V *const gate_from = asks_from<V, S>(gate, gate_step), *const value_from = asks_from<V, S>(value, value_step);
     const T *const grad_from = asks_from<T, S>(grad, p.width);
@@ -614,26 +668,24 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
         ask(gs, grad_from + t * p.width, (long long)p.width, cnt, left);
         copies_on_their_way();
         if (PACKED) {
-            zsc = ask_scales(p.gate_scales, q.first + t, per_row, slab, cnt);
-            usc = ask_scales(p.value_scales, q.first + t, per_row, slab, cnt);
+            scales = ask_scales(p, q.first + t, per_row, slab, cnt);
         }
     };
     int par = 0;
-    const long long last = (q.len + held - 1) / held - 1, mine = (long long)rank * kBwdTile + warp * S;
-    if (wide && last >= 0) ask_all(last * held + mine);
+    const long long last = ((q.len + held - 1) >> held_log2) - 1, mine = (long long)rank * kBwdTile + warp * S;
+    if (wide && last >= 0) ask_all((last << held_log2) + mine);
     // a CTA's shared memory may be written to by others once it runs: waited for ahead of the first such store
     if (p.cluster > 1) cg::this_cluster().sync();
     const float inf = __uint_as_float(0x7f800000u);
     for (long long k = last; k >= 0; --k, par ^= 1) {
-        const long long t0 = k * held + mine;
+        const long long t0 = (k << held_log2) + mine;
         const int cnt = (int)min((long long)S, max(0LL, q.len - t0));
         // a step behind the end holds the state and has no gradient of its own
         float2 a[S], n[S], u[S], g[S], h = two(0.0f);
         if (wide) {
             copies_there();
             if constexpr (PACKED) {
-                take_packed<S>(zs, zsc, cnt, nch, inf, a);
-                take_packed<S>(us, usc, cnt, nch, 0.0f, u);
+                take_packed<S>(zs, us, scales, cnt, nch, inf, a, u);
             } else {
                 take(zs, cnt, nch, inf, a);
                 take(us, cnt, nch, 0.0f, u);
@@ -812,10 +864,13 @@ static int scan_check(int n, long long steps, long long total, int width, int dt
     return GN_OK;
 }
 
-static int scan_interval(int n, long long steps, long long total, int width, int dtype, bool ragged)
+// log2 of the steps between two states that a backward pass starts from: what its CTA or cluster holds
+static int scan_interval_log2(int n, long long steps, long long total, int width, int dtype, bool ragged)
 {
     const long long mean = ragged ? total / (n > 0 ? n : 1) : steps;
-    return kBwdTile * scan_cluster(n, mean, width, dtype == GN_F32 ? 4 : 2, true);
+    int log2 = 0;
+    while ((1 << log2) < kBwdTile * scan_cluster(n, mean, width, dtype == GN_F32 ? 4 : 2, true)) ++log2;
+    return log2;
 }
 
 static int launch_scan(void (*kern)(const Scan), const Scan &p, size_t tile_bytes, const char *what, cudaStream_t st)
@@ -870,7 +925,7 @@ extern "C" {
 GN_API size_t gn_gated_scan_bounds_bytes(int n, long long steps, long long total, int width, int dtype, int ragged)
 {
     if (scan_check(n, steps, total, width, dtype, ragged != 0) != GN_OK || n == 0 || total == 0) return 0;
-    const int interval = scan_interval(n, steps, total, width, dtype, ragged != 0);
+    const int interval = 1 << scan_interval_log2(n, steps, total, width, dtype, ragged != 0);
     if ((ragged ? total : steps) <= interval) return 0;
     const long long rows = ragged ? total / interval + n + 1 : n * ((steps + interval - 1) / interval);
     return sizeof(float) * (size_t)rows * width;
@@ -891,7 +946,7 @@ GN_API int gn_gated_scan_forward(const void *gate, const void *value, const floa
     p.pack_gate = (unsigned char *)gate_codes; p.pack_gate_scales = (unsigned char *)gate_scales;
     p.pack_value = (unsigned char *)value_codes; p.pack_value_scales = (unsigned char *)value_scales;
     p.bounds = gate_codes ? nullptr : bounds;  // those of the codes are found when they are wanted
-    p.interval = scan_interval(n, steps, total, width, dtype, offsets != nullptr);
+    p.interval_log2 = scan_interval_log2(n, steps, total, width, dtype, offsets != nullptr);
     p.gate_seq = gate_seq; p.gate_step = gate_step; p.value_seq = value_seq; p.value_step = value_step;
     p.n = n; p.steps = steps; p.total = total; p.width = width;
     const int size = dtype == GN_F32 ? 4 : 2;
@@ -923,10 +978,10 @@ GN_API int gn_gated_scan_backward(const void *gate, const void *value, const voi
     p.gate = gate; p.value = value; p.state = state; p.offsets = offsets; p.bounds = bounds;
     p.gate_scales = (const unsigned char *)gate_scales; p.value_scales = (const unsigned char *)value_scales;
     p.gh = grad_h; p.glast = grad_last; p.dgate = grad_gate; p.dvalue = grad_value; p.dstate = grad_state;
-    p.interval = scan_interval(n, steps, total, width, dtype, offsets != nullptr);
+    p.interval_log2 = scan_interval_log2(n, steps, total, width, dtype, offsets != nullptr);
     p.gate_seq = gate_seq; p.gate_step = gate_step; p.value_seq = value_seq; p.value_step = value_step;
     p.n = n; p.steps = steps; p.total = total; p.width = width;
-    p.cluster = p.interval / kBwdTile;
+    p.cluster = (1 << p.interval_log2) / kBwdTile;
     const int size = dtype == GN_F32 ? 4 : 2, in = gate_scales ? 1 : size;
     p.vec = width % 2 == 0 && gate_seq % 2 == 0 && gate_step % 2 == 0 && value_seq % 2 == 0 && value_step % 2 == 0 && aligned(gate, 2 * in) &&
             aligned(value, 2 * in) && aligned(grad_h, 2 * size) && aligned(grad_gate, 2 * size) && aligned(grad_value, 2 * size) &&
