@@ -102,8 +102,9 @@ SIGNATURES = {
     "gn_norm_forward_packed_f32": (c_int, [_P] * 7 + [c_int, c_longlong, c_float, _P, c_size_t, _P]),
     "gn_norm_backward_packed_f32": (c_int, [_P] * 8 + [c_int, c_longlong, _P, c_size_t, _P]),
     "gn_gated_scan_bounds_bytes": (c_size_t, [c_int, c_longlong, c_longlong, c_int, c_int, c_int]),
-    "gn_gated_scan_forward": (c_int, [_P] * 11 + [c_int, c_longlong, c_longlong, c_int] + [c_longlong] * 4 + [c_int, _P]),
-    "gn_gated_scan_backward": (c_int, [_P] * 12 + [c_int, c_longlong, c_longlong, c_int] + [c_longlong] * 4 + [c_int, _P]),
+    "gn_gated_scan_workspace_bytes": (c_size_t, [c_int, c_longlong, c_longlong] + [c_int] * 5),
+    "gn_gated_scan_forward": (c_int, [_P] * 11 + [c_int, c_longlong, c_longlong, c_int] + [c_longlong] * 4 + [c_int, _P, c_size_t, _P]),
+    "gn_gated_scan_backward": (c_int, [_P] * 12 + [c_int, c_longlong, c_longlong, c_int] + [c_longlong] * 4 + [c_int, _P, c_size_t, _P]),
     "gn_gated_scan_step": (c_int, [_P] * 5 + [c_longlong, c_int, c_longlong, c_longlong, c_int, _P]),
 }
 

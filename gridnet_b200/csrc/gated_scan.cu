@@ -2,14 +2,21 @@
 // function - the update of the gated grid's cell (gridnet/backend_torch.py:241-265) with gate z and value u given.
 //
 // Every step is an affine map of the state, and so is every run of steps: (A, H) stands for h -> A h + H, and
-// (A2, H2) after (A1, H1) is (A1 A2, A2 H1 + H2). A thread composes the steps it holds in registers, warps compose through shared memory,
-// the CTAs of a cluster through each other's shared memory; then each thread knows the state ahead of its first step
-// and runs its steps again from registers. So gate and value are read once and h is written once, however long the sequence.
+// (A2, H2) after (A1, H1) is (A1 A2, A2 H1 + H2). A thread composes the steps it holds in registers, warps compose through shared memory;
+// then each thread knows the state ahead of its first step and runs its steps again from registers.
 //
 // Backward: c_t = gradient of h_{t-1} = a_t (g_t + c_{t+1}) is affine in c_{t+1}, from the end to the start, with the same A;
 //     dh_t = g_t + c_{t+1},  du_t = n_t dh_t,  dz_t = a_t n_t (h_{t-1} - u_t) dh_t.
-// h is not kept but run again: both directions are composed in the same exchange, from one reading of gate, value and g. Where a
-// sequence is longer than what a CTA or cluster holds at a time, the forward pass has left the state at each such boundary.
+// h is not kept but run again: both directions are composed in the same exchange, from one reading of gate, value and g.
+//
+// Two ways along a sequence:
+//   walk     a CTA has 64 channels of a sequence and goes from tile to tile, everything read once. Backward it needs the state ahead
+//            of each tile, which the forward pass has left. For many sequences or channels.
+//   chunks   every tile is a CTA of its own: one kernel composes each tile's steps, one goes over the tiles and says where
+//            each starts, one does the work. gate and value (and g) are read twice, the second time from L2 where they fit.
+//            For few and long sequences, and for the backward pass from packed copies, where there is no state that could have been left.
+// A cluster of CTAs that walks together and exchanges maps through distributed shared memory was measured as a third way: 1.5 us more for
+// a round of tiles, slower than the chunks (4 x 4097 x 1024 float32, backward from packed copies, 157 us).
 //
 // Steps whose n_t is 0 (gates from about 104 up, and +inf) do not look at their value, which may be NaN; steps whose a_t is 0 do not look
 // at the state. Anything else that is not finite stays in the state. Threads that hold such a step (the smaller of a_t and n_t is 0) go
@@ -18,8 +25,6 @@
 //
 // A thread has two channels, so that a row is read 64 channels at a time and arithmetic is on pairs (f32x2); a warp has a run of steps
 // of its own, no lane has to know another lane's.
-#include <cooperative_groups.h>
-
 #include <type_traits>
 
 #include "kernels.h"
@@ -27,12 +32,14 @@
 
 namespace gn {
 
-namespace cg = cooperative_groups;
-
-constexpr int kScanThreads = 128, kScanWarps = 4, kMaxCluster = 8;
-constexpr int kSlab = 64;                    // channels of a CTA
+constexpr int kScanThreads = 128, kScanWarps = 4;
+constexpr int kSlab = 64;                     // channels of a CTA
 constexpr int kFwdSteps = 16, kBwdSteps = 8;  // steps that a thread holds
-constexpr int kFwdTile = kScanWarps * kFwdSteps, kBwdTile = kScanWarps * kBwdSteps;
+constexpr int kFwdLog2 = 6, kBwdLog2 = 5;     // of a tile's steps
+constexpr int kFwdTile = 1 << kFwdLog2, kBwdTile = 1 << kBwdLog2;
+static_assert(kFwdTile == kScanWarps * kFwdSteps && kBwdTile == kScanWarps * kBwdSteps, "a tile is what a CTA holds");
+constexpr int kSumSteps = 8;                  // steps that a thread composes at a time when a warp has a tile to itself
+constexpr int kStartWarps = 16;
 
 struct Scan {
     const void *gate, *value;  // or codes
@@ -43,13 +50,14 @@ struct Scan {
     void *h;
     float *last;
     unsigned char *pack_gate, *pack_value, *pack_gate_scales, *pack_value_scales;
-    float *bounds;  // state ahead of every 2^interval_log2-th step of a sequence
-    int interval_log2;
+    float *bounds;  // walk: state ahead of each backward tile of a sequence but the first
+    float *maps;    // chunks: A, H and (backward) C of each tile, planes of map_rows x padded; H and C give way to where the tile starts
+    long long map_rows;
     const void *gh;
     const float *glast;
     void *dgate, *dvalue;
     float *dstate;
-    int n, width, slabs, cluster;
+    int n, width, slabs, padded;  // padded: slabs * kSlab
     int vec;   // pairs of channels lie on whole pairs' addresses
     int wide;  // 16 bytes of a row on multiples of 16
     long long steps, total;  // steps of a sequence; rows of everything
@@ -70,11 +78,36 @@ __device__ __forceinline__ Place sequence(const Scan &p, int seq)
     }
     return s;
 }
-// row of p.bounds that holds the state ahead of step k << interval_log2 of a sequence, k >= 1
-__device__ __forceinline__ long long bound_row(const Scan &p, int seq, const Place &s, long long k)
+// Row of p.bounds or p.maps that belongs to tile k of a sequence, tiles of 2^LOG2 steps
+template <int LOG2>
+__device__ __forceinline__ long long tile_row(const Scan &p, int seq, const Place &s, long long k)
 {
-    if (!p.offsets) return seq * ((p.steps + (1LL << p.interval_log2) - 1) >> p.interval_log2) + k;
-    return (s.first >> p.interval_log2) + seq + k;  // a sequence has at most one boundary more than its rows have multiples of the interval
+    if (!p.offsets) return seq * ((p.steps + (1 << LOG2) - 1) >> LOG2) + k;
+    return (s.first >> LOG2) + seq + k;  // a sequence has at most one tile more than its rows have multiples of a tile
+}
+// and the other way round; false where the row belongs to no tile
+template <int LOG2>
+__device__ __forceinline__ bool tile_of_row(const Scan &p, long long row, int &seq, Place &s, long long &k)
+{
+    if (!p.offsets) {
+        const long long tiles = (p.steps + (1 << LOG2) - 1) >> LOG2;
+        seq = (int)(row / tiles);
+        s = sequence(p, seq);
+        k = row - seq * tiles;
+        return true;
+    }
+    int lo = 0, hi = p.n;  // the last sequence that starts at this row or before
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if ((min(max(p.offsets[mid], 0LL), p.total) >> LOG2) + mid <= row)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    seq = lo;
+    s = sequence(p, seq);
+    k = row - ((s.first >> LOG2) + seq);
+    return k >= 0 && k << LOG2 < s.len;
 }
 
 // ---- pairs
@@ -163,11 +196,11 @@ __device__ __forceinline__ float2 looked_at(float2 n, float2 v) { return make_fl
 
 // Rows outside of every sequence of a ragged call: zeros
 template <typename T>
-__device__ void clear_rows(const Scan &p, T *x, int slab, int rank)
+__device__ void clear_rows(const Scan &p, T *x, int slab)
 {
     const long long lo = min(max(p.offsets[0], 0LL), p.total), hi = min(max(p.offsets[p.n], lo), p.total);
     const int ch = slab * kSlab + (threadIdx.x & 31) * 2, nch = min(2, max(0, p.width - ch));
-    for (long long i = (long long)rank * kScanWarps + (threadIdx.x >> 5); i < lo + p.total - hi; i += (long long)kScanWarps * p.cluster) {
+    for (long long i = threadIdx.x >> 5; i < lo + p.total - hi; i += blockDim.x >> 5) {
         const long long row = i < lo ? i : i - lo + hi;
         store2(x + row * p.width + ch, p.vec, nch, two(0.0f));
     }
@@ -392,17 +425,21 @@ __device__ __forceinline__ void take(const Rows<T, S> &from, int cnt, int nch, f
 #pragma unroll
         for (int s = 0; s < S; ++s) v[s] = s >= cnt ? two(end) : nch == 0 ? two(0.0f) : v[s];
 }
-// The scale bytes of gate and of value for a warp's steps: lane 2 r + g has row r, group g of the slab
-__device__ __forceinline__ unsigned ask_scales(const Scan &p, long long row, int per_row, int slab, int cnt)
+// The scale bytes of gate and of value for a warp's steps: lane 2 r + g has row r, group g of the slab. Put together only where they are used:
+// whoever combines them waits for them.
+struct Scales {
+    unsigned char gate, value;
+};
+__device__ __forceinline__ Scales ask_scales(const Scan &p, long long row, int slab, int cnt)
 {
-    const int lane = threadIdx.x & 31, r = lane >> 1, g = slab * (kSlab / kPackGroup) + (lane & 1);
-    if (r >= cnt || g >= per_row) return 127u | 127u << 16;
-    const long long at = (row + r) * per_row + g;
-    return p.gate_scales[at] | (unsigned)p.value_scales[at] << 16;
+    const int lane = threadIdx.x & 31, r = lane >> 1, g = slab * (kSlab / kPackGroup) + (lane & 1), per_row = (p.width + kPackGroup - 1) / kPackGroup;
+    const bool there = r < cnt && g < per_row;
+    const long long at = there ? (row + r) * per_row + g : 0;
+    return {p.gate_scales[at], p.value_scales[at]};
 }
 // gate and value as their codes give them
 template <int S>
-__device__ __forceinline__ void take_packed(const Rows<unsigned char, S> &gates, const Rows<unsigned char, S> &values, unsigned scales, int cnt, int nch,
+__device__ __forceinline__ void take_packed(const Rows<unsigned char, S> &gates, const Rows<unsigned char, S> &values, Scales scales, int cnt, int nch,
                                             float end, float2 (&z)[S], float2 (&u)[S])
 {
     const int lane = threadIdx.x & 31;
@@ -424,7 +461,7 @@ __device__ __forceinline__ void take_packed(const Rows<unsigned char, S> &gates,
         whole(wz[s / 2] = word(gates, s), z[s], z[s + 1]);
         whole(wu[s / 2] = word(values, s), u[s], u[s + 1]);
     }
-    const unsigned steps = scales << 7;  // the upper halves of both 2^e (the lower ones are 0)
+    const unsigned steps = (scales.gate | (unsigned)scales.value << 16) << 7;  // the upper halves of both 2^e (the lower ones are 0)
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         const unsigned both = __shfl_sync(0xffffffffu, steps, 2 * s + (lane >> 4));
@@ -457,91 +494,259 @@ __device__ __forceinline__ float2 straight(float4 m, float2 h) { return fma2(fac
 template <int WAYS>
 struct Exchange {
     float4 warp[2][WAYS][kScanWarps][32];
-    float4 rank[2][WAYS][kMaxCluster][32];
+};
+__device__ __forceinline__ float2 *plane(const Scan &p, int way, long long row, int slab)
+{
+    return reinterpret_cast<float2 *>(p.maps + (way * p.map_rows + row) * p.padded + slab * kSlab) + (threadIdx.x & 31);
+}
+
+// Where a warp's rows of gate and value (and g) come from; S rows at a time
+template <typename T, bool PACKED, bool GRAD, int S>
+struct Source {
+    using V = std::conditional_t<PACKED, unsigned char, T>;
+    static constexpr size_t kBytes = sizeof(Rows<V, S>) * 2 + (GRAD ? sizeof(Rows<T, S>) : 0);  // shared memory of a warp
+    const Scan &p;
+    const int slab, ch, nch, left;
+    const long long first, gate_step, value_step;
+    const V *gate, *value;
+    const T *grad;
+    Rows<V, S> *zs, *us;
+    Rows<T, S> *gs;
+    Scales scales;
+
+    __device__ __forceinline__ Source(const Scan &p, const Place &q, int seq, int slab, unsigned char *shared)
+        : p(p), slab(slab), ch(slab * kSlab + (threadIdx.x & 31) * 2), nch(min(2, max(0, p.width - ch))), left(p.width - slab * kSlab), first(q.first),
+          // codes lie in rows of width, one after the other
+          gate_step(PACKED ? p.width : p.gate_step), value_step(PACKED ? p.width : p.value_step)
+    {
+        gate = (const V *)p.gate + (PACKED || p.offsets ? first * gate_step : seq * p.gate_seq) + slab * kSlab;
+        value = (const V *)p.value + (PACKED || p.offsets ? first * value_step : seq * p.value_seq) + slab * kSlab;
+        grad = GRAD ? (const T *)p.gh + first * p.width + slab * kSlab : nullptr;
+        zs = reinterpret_cast<Rows<V, S> *>(shared);
+        us = zs + 1;
+        gs = reinterpret_cast<Rows<T, S> *>(us + 1);
+    }
+    // cnt rows from step t of the sequence on (none: nothing)
+    __device__ __forceinline__ void ask_for(long long t, int cnt)
+    {
+        if (!p.wide || cnt <= 0) return;
+        ask(*zs, asks_from<V, S>(gate + t * gate_step, gate_step), gate_step, cnt, left);
+        ask(*us, asks_from<V, S>(value + t * value_step, value_step), value_step, cnt, left);
+        if constexpr (GRAD) ask(*gs, asks_from<T, S>(grad + t * p.width, p.width), (long long)p.width, cnt, left);
+        copies_on_their_way();
+        if constexpr (PACKED) scales = ask_scales(p, first + t, slab, cnt);
+    }
+    // What was asked for; a step behind the end holds the state and has no gradient of its own. Then `ask_for` may ask for other rows
+    __device__ __forceinline__ void take_from(long long t, int cnt, float2 (&z)[S], float2 (&u)[S], float2 (&g)[GRAD ? S : 1])
+    {
+        const float inf = __uint_as_float(0x7f800000u);
+        if (p.wide) {
+            copies_there();
+            if constexpr (PACKED) {
+                take_packed<S>(*zs, *us, scales, cnt, nch, inf, z, u);
+            } else {
+                take(*zs, cnt, nch, inf, z);
+                take(*us, cnt, nch, 0.0f, u);
+            }
+            if constexpr (GRAD) take(*gs, cnt, nch, 0.0f, g);
+            __syncwarp();
+        } else {
+            const int lane = threadIdx.x & 31;
+            if constexpr (PACKED) {
+                load_packed<S>((const unsigned char *)p.gate, p.gate_scales, first + t, p.width, ch, p.vec, cnt, nch, inf, z);
+                load_packed<S>((const unsigned char *)p.value, p.value_scales, first + t, p.width, ch, p.vec, cnt, nch, 0.0f, u);
+            } else {
+                load_rows<T, S>(gate + lane * 2 + t * gate_step, gate_step, p.vec, cnt, nch, inf, z);
+                load_rows<T, S>(value + lane * 2 + t * value_step, value_step, p.vec, cnt, nch, 0.0f, u);
+            }
+            if constexpr (GRAD) load_rows<T, S>(grad + lane * 2 + t * p.width, p.width, p.vec, cnt, nch, 0.0f, g);
+        }
+    }
 };
 
-// ------------------------------------------------------------------ forward
-// PACKED: gate and value are codes, and only the states at the boundaries are wanted. KEEP: packs gate and value.
-template <typename T, bool PACKED, bool KEEP>
-__global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
+// ------------------------------------------------------------------ chunks: what each tile amounts to, a warp per tile
+template <typename T, bool PACKED, bool BACKWARD>
+__global__ void __launch_bounds__(kScanThreads, 7) scan_maps_k(const Scan p)
 {
-    using V = std::conditional_t<PACKED, unsigned char, T>;
-    constexpr int S = kFwdSteps;
+    constexpr int S = kSumSteps, kLog2 = BACKWARD ? kBwdLog2 : kFwdLog2;
+    using From = Source<T, PACKED, BACKWARD, S>;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ __align__(16) Exchange<1> ex;
-    const int rank = blockIdx.x % p.cluster, id = blockIdx.x / p.cluster;
-    const int slab = id % p.slabs, seq = id / p.slabs;
+    const int warp = threadIdx.x >> 5;
+    const long long id = (long long)blockIdx.x * kScanWarps + warp, row = id / p.slabs;
+    const int slab = (int)(id - row * p.slabs);
+    if (row >= p.map_rows) return;
+    int seq;
+    Place q;
+    long long k;
+    if (!tile_of_row<kLog2>(p, row, seq, q, k)) return;
+    From from(p, q, seq, slab, dynamic + warp * From::kBytes);
+    long long t = k << kLog2;
+    int rows = (int)min(1LL << kLog2, q.len - t);
+    from.ask_for(t, min(S, rows));
+    float2 A = two(1.0f), H = two(0.0f), C = two(0.0f);
+    for (; rows > 0; t += S, rows -= S) {
+        float2 z[S], u[S], g[BACKWARD ? S : 1];
+        from.take_from(t, min(S, rows), z, u, g);
+        from.ask_for(t + S, min(S, rows - S));
+        if (farthest(z) < kFar) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                float2 a, n;
+                gates(z[s], a, n);
+                H = fma2(a, H, mul2(n, u[s]));
+                A = product(A, a);
+                if constexpr (BACKWARD) C = make_float2(resets(A.x) ? C.x : fmaf(A.x, g[s].x, C.x), resets(A.y) ? C.y : fmaf(A.y, g[s].y, C.y));
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < S; ++s) {
+                float2 a, n;
+                gates_any(z[s], a, n);
+                H = after(a, H, mul2(n, looked_at(n, u[s])));
+                A = more(A, a);
+                if constexpr (BACKWARD) C = make_float2(resets(A.x) ? C.x : fmaf(A.x, g[s].x, C.x), resets(A.y) ? C.y : fmaf(A.y, g[s].y, C.y));
+            }
+        }
+    }
+    *plane(p, 0, row, slab) = A;
+    *plane(p, 1, row, slab) = H;
+    if (BACKWARD) *plane(p, 2, row, slab) = C;
+}
+
+// ------------------------------------------------------------------ chunks: where each tile starts. A CTA has 64 channels of a sequence, a warp a
+// run of its tiles
+template <typename T, bool BACKWARD>
+__global__ void __launch_bounds__(32 * kStartWarps) scan_starts_k(const Scan p)
+{
+    constexpr int kLog2 = BACKWARD ? kBwdLog2 : kFwdLog2, kBatch = 8;
+    __shared__ float4 runs[BACKWARD ? 2 : 1][kStartWarps][32];
+    const int slab = blockIdx.x % p.slabs, seq = blockIdx.x / p.slabs;
+    previous_done();
     if (seq >= p.n) {
-        if (!PACKED) clear_rows<T>(p, (T *)p.h, slab, rank);
+        if (BACKWARD) {
+            clear_rows<T>(p, (T *)p.dgate, slab);
+            clear_rows<T>(p, (T *)p.dvalue, slab);
+        } else {
+            clear_rows<T>(p, (T *)p.h, slab);
+        }
         return;
     }
     const Place q = sequence(p, seq);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int ch = slab * kSlab + lane * 2, nch = min(2, max(0, p.width - ch));
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ch = slab * kSlab + lane * 2, nch = min(2, max(0, p.width - ch));
+    const long long state_at = (long long)seq * p.width + ch, tiles = (q.len + (1 << kLog2) - 1) >> kLog2, row = tile_row<kLog2>(p, seq, q, 0);
+    const long long per = (tiles + kStartWarps - 1) / kStartWarps, lo = min(tiles, warp * per), hi = min(tiles, lo + per);
+    float2 A = two(1.0f), H = two(0.0f), C = two(0.0f);
+    for (long long k = lo; k < hi; k += kBatch) {
+        float2 a[kBatch], h[kBatch], c[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const long long at = row + min(k + i, hi - 1);
+            a[i] = *plane(p, 0, at, slab);
+            h[i] = *plane(p, 1, at, slab);
+            if (BACKWARD) c[i] = *plane(p, 2, at, slab);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (k + i < hi) {
+                if (BACKWARD) C = make_float2(resets(A.x) ? C.x : fmaf(A.x, c[i].x, C.x), resets(A.y) ? C.y : fmaf(A.y, c[i].y, C.y));
+                H = through(a[i], H, h[i]);
+                A = product(A, a[i]);
+            }
+    }
+    runs[0][warp][lane] = map_of(A, H);
+    if (BACKWARD) runs[BACKWARD][warp][lane] = map_of(A, C);
+    __syncthreads();
+    float2 h = two(0.0f), c = two(0.0f);
+    if (p.state) h = load2(p.state + state_at, p.vec, nch);
+    if (!BACKWARD && tiles == 0 && warp == 0 && p.last) store2(p.last + state_at, p.vec, nch, h);
+    for (int w = 0; w < warp; ++w) h = through(runs[0][w][lane], h);
+    if (BACKWARD) {
+        if (p.glast) c = load2(p.glast + state_at, p.vec, nch);
+        for (int w = kStartWarps - 1; w > warp; --w) c = through(runs[BACKWARD][w][lane], c);
+    }
+    for (long long k = lo; k < hi; k += kBatch) {
+        float2 a[kBatch], b[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const long long at = row + min(k + i, hi - 1);
+            a[i] = *plane(p, 0, at, slab);
+            b[i] = *plane(p, 1, at, slab);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (k + i < hi) {
+                *plane(p, 1, row + k + i, slab) = h;
+                h = through(a[i], h, b[i]);
+            }
+    }
+    if (BACKWARD) {
+        for (long long k = hi - 1; k >= lo; k -= kBatch) {
+            float2 a[kBatch], b[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const long long at = row + max(k - i, lo);
+                a[i] = *plane(p, 0, at, slab);
+                b[i] = *plane(p, 2, at, slab);
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+                if (k - i >= lo) {
+                    *plane(p, 2, row + k - i, slab) = c;
+                    c = through(a[i], c, b[i]);
+                }
+        }
+        if (p.dstate && warp == 0) store2(p.dstate + state_at, p.vec, nch, c);
+    }
+}
+
+// ------------------------------------------------------------------ forward. KEEP: packs gate and value. CHUNK: a tile, else a sequence
+template <typename T, bool KEEP, bool CHUNK>
+__global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
+{
+    constexpr int S = kFwdSteps;
+    using From = Source<T, false, false, S>;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ __align__(16) Exchange<1> ex;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slab = blockIdx.x % p.slabs;
+    int seq = blockIdx.x / p.slabs;
+    Place q;
+    long long row = 0, tile = 0;
+    if constexpr (CHUNK) {
+        row = blockIdx.x / p.slabs;
+        if (!tile_of_row<kFwdLog2>(p, row, seq, q, tile)) {
+            previous_done();
+            return;
+        }
+    } else {
+        if (seq >= p.n) {
+            clear_rows<T>(p, (T *)p.h, slab);
+            return;
+        }
+        q = sequence(p, seq);
+    }
+    From from(p, q, seq, slab, dynamic + warp * From::kBytes);
+    const int ch = from.ch, nch = from.nch;
     const bool vec = p.vec;
     const long long state_at = (long long)seq * p.width + ch;
+    long long t0 = (tile << kFwdLog2) + warp * S;
+    auto rows_at = [&](long long t) { return (int)min((long long)S, max(0LL, q.len - t)); };
+    from.ask_for(t0, rows_at(t0));
     float2 carry = two(0.0f);
-    if (p.state) carry = load2(p.state + state_at, vec, nch);
-    if (q.len == 0) {
-        if (!PACKED && p.last && rank == 0 && warp == 0) store2(p.last + state_at, vec, nch, carry);
-        return;
+    if constexpr (CHUNK) {
+        previous_done();
+        carry = *plane(p, 1, row, slab);
+    } else {
+        if (p.state) carry = load2(p.state + state_at, vec, nch);
+        if (q.len == 0 && p.last && warp == 0) store2(p.last + state_at, vec, nch, carry);
     }
-    if (PACKED && q.len <= 1LL << p.interval_log2) return;  // the whole cluster
-    const long long held = (long long)kFwdTile * p.cluster;
-    long long t0 = (long long)rank * kFwdTile + warp * S;
-    // codes lie in rows of width, one after the other
-    const long long gate_step = PACKED ? p.width : p.gate_step, value_step = PACKED ? p.width : p.value_step;
-    const V *gate = (const V *)p.gate + (PACKED || p.offsets ? q.first * gate_step : seq * p.gate_seq) + t0 * gate_step + slab * kSlab;
-    const V *value = (const V *)p.value + (PACKED || p.offsets ? q.first * value_step : seq * p.value_seq) + t0 * value_step + slab * kSlab;
-    const int per_row = (p.width + kPackGroup - 1) / kPackGroup, left = p.width - slab * kSlab;
-    Rows<V, S> &zs = reinterpret_cast<Rows<V, S> *>(dynamic)[warp], &us = reinterpret_cast<Rows<V, S> *>(dynamic)[kScanWarps + warp];
-    unsigned scales = 0;
-    const bool wide = p.wide;
-    auto ask_all = [&](long long t) {
-        const int cnt = (int)min((long long)S, max(0LL, q.len - t));
-        ask(zs, gate, gate_step, cnt, left);
-        ask(us, value, value_step, cnt, left);
-        copies_on_their_way();
-        if (PACKED) {
-            scales = ask_scales(p, q.first + t, per_row, slab, cnt);
-        }
-    };
-    if (wide) {
-        gate = asks_from<V, S>(gate, gate_step);
-        value = asks_from<V, S>(value, value_step);
-        ask_all(t0);
-    }
-    // a CTA's shared memory may be written to by others once it runs: waited for ahead of the first such store
-    if (p.cluster > 1) cg::this_cluster().sync();
-    const float inf = __uint_as_float(0x7f800000u);
-    for (int par = 0; t0 - (long long)rank * kFwdTile - warp * S < q.len; t0 += held, par ^= 1) {
-        const int cnt = (int)min((long long)S, max(0LL, q.len - t0));
-        // a step behind the end holds the state
-        float2 a[S], b[S];
-        if (wide) {
-            copies_there();
-            if constexpr (PACKED) {
-                take_packed<S>(zs, us, scales, cnt, nch, inf, a, b);
-            } else {
-                take(zs, cnt, nch, inf, a);
-                take(us, cnt, nch, 0.0f, b);
-            }
-            __syncwarp();
-            gate += held * gate_step;
-            value += held * value_step;
-            ask_all(t0 + held);
-        } else if constexpr (PACKED) {
-            load_packed<S>((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, inf, a);
-            load_packed<S>((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, 0.0f, b);
-        } else {
-            load_rows<T, S>(gate + lane * 2, gate_step, vec, cnt, nch, inf, a);
-            load_rows<T, S>(value + lane * 2, value_step, vec, cnt, nch, 0.0f, b);
-            gate += held * gate_step;
-            value += held * value_step;
-        }
+    for (int par = 0; t0 - warp * S < q.len; t0 += kFwdTile, par ^= 1) {
+        const int cnt = rows_at(t0);
+        float2 a[S], b[S], none[1];
+        from.take_from(t0, cnt, a, b, none);
+        if (!CHUNK) from.ask_for(t0 + kFwdTile, rows_at(t0 + kFwdTile));
         if constexpr (KEEP) {
             const PackTo to = {p.pack_gate, p.pack_value, p.pack_gate_scales, p.pack_value_scales};
-            pack_rows(a, b, to, q.first + t0, p.width, ch, vec && left >= kSlab && cnt == S, cnt, nch);
+            pack_rows(a, b, to, q.first + t0, p.width, ch, vec && from.left >= kSlab && cnt == S, cnt, nch);
         }
         const bool special = farthest(a) >= kFar;
         float2 A = two(1.0f), H = two(0.0f);
@@ -569,24 +774,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
         ex.warp[par][0][warp][lane] = map_of(A, H);
         const bool any = __syncthreads_or(special);
         float2 h = carry;
-        if (p.cluster > 1) {
-            cg::cluster_group cluster = cg::this_cluster();
-            // every warp composes the CTA's steps and tells every fourth CTA
-            float2 ta = two(1.0f), th = two(0.0f);
-#pragma unroll
-            for (int w = 0; w < kScanWarps; ++w) {
-                const float4 m = ex.warp[par][0][w][lane];
-                th = through(m, th);
-                ta = product(ta, factor(m));
-            }
-            for (int r = warp; r < p.cluster; r += kScanWarps) *cluster.map_shared_rank(&ex.rank[par][0][rank][lane], r) = map_of(ta, th);
-            cluster.sync();
-            for (int r = 0; r < p.cluster; ++r) {
-                if (r == rank) h = carry;
-                carry = through(ex.rank[par][0][r][lane], carry);
-            }
-            for (int w = 0; w < warp; ++w) h = through(ex.warp[par][0][w][lane], h);
-        } else if (!any) {
+        if (!any) {
 #pragma unroll
             for (int w = 0; w < kScanWarps; ++w) {
                 if (w == warp) h = carry;
@@ -599,114 +787,84 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
                 carry = through(ex.warp[par][0][w][lane], carry);
             }
         }
-        // intervals are multiples of 32 steps: boundaries lie at the start of a thread's steps
-        if (p.bounds && cnt > 0 && t0 > 0 && (t0 & ((1 << p.interval_log2) - 1)) == 0)
-            store2(p.bounds + bound_row(p, seq, q, t0 >> p.interval_log2) * p.width + ch, vec, nch, h);
-        if (!PACKED) {
-            T *out = (T *)p.h + (q.first + t0) * p.width + ch;
-            if (!special) {
+        // a backward tile is a multiple of a thread's steps: boundaries lie at the start of a thread's steps
+        if (!CHUNK && p.bounds && cnt > 0 && t0 > 0 && (t0 & (kBwdTile - 1)) == 0)
+            store2(p.bounds + tile_row<kBwdLog2>(p, seq, q, t0 >> kBwdLog2) * p.width + ch, vec, nch, h);
+        T *out = (T *)p.h + (q.first + t0) * p.width + ch;
+        if (!special) {
 #pragma unroll
-                for (int s = 0; s < S; ++s) a[s] = h = fma2(a[s], h, b[s]);
-            } else {
+            for (int s = 0; s < S; ++s) a[s] = h = fma2(a[s], h, b[s]);
+        } else {
 #pragma unroll
-                for (int s = 0; s < S; ++s) a[s] = h = after(a[s], h, b[s]);
-            }
-            if (vec && nch == 2 && cnt == S) {
-#pragma unroll
-                for (int s = 0; s < S; ++s, out += p.width) store2v(out, a[s]);
-            } else {
-#pragma unroll
-                for (int s = 0; s < S; ++s)
-                    if (s < cnt) store2(out + (long long)s * p.width, vec, nch, a[s]);
-            }
-            if (p.last && cnt > 0 && t0 + cnt == q.len) store2(p.last + state_at, vec, nch, h);
+            for (int s = 0; s < S; ++s) a[s] = h = after(a[s], h, b[s]);
         }
+        if (vec && nch == 2 && cnt == S) {
+#pragma unroll
+            for (int s = 0; s < S; ++s, out += p.width) store2v(out, a[s]);
+        } else {
+#pragma unroll
+            for (int s = 0; s < S; ++s)
+                if (s < cnt) store2(out + (long long)s * p.width, vec, nch, a[s]);
+        }
+        if (p.last && cnt > 0 && t0 + cnt == q.len) store2(p.last + state_at, vec, nch, h);
+        if (CHUNK) break;
     }
 }
 
 // ------------------------------------------------------------------ backward
-template <typename T, bool PACKED>
+template <typename T, bool PACKED, bool CHUNK>
 __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
 {
-    using V = std::conditional_t<PACKED, unsigned char, T>;
     constexpr int S = kBwdSteps;
+    using From = Source<T, PACKED, true, S>;
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) Exchange<2> ex;
-    const int rank = blockIdx.x % p.cluster, id = blockIdx.x / p.cluster;
-    const int slab = id % p.slabs, seq = id / p.slabs;
-    if (seq >= p.n) {
-        clear_rows<T>(p, (T *)p.dgate, slab, rank);
-        clear_rows<T>(p, (T *)p.dvalue, slab, rank);
-        return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slab = blockIdx.x % p.slabs;
+    int seq = blockIdx.x / p.slabs;
+    Place q;
+    long long row = 0, tile = 0;
+    if constexpr (CHUNK) {
+        row = blockIdx.x / p.slabs;
+        if (!tile_of_row<kBwdLog2>(p, row, seq, q, tile)) {
+            previous_done();
+            return;
+        }
+    } else {
+        if (seq >= p.n) {
+            clear_rows<T>(p, (T *)p.dgate, slab);
+            clear_rows<T>(p, (T *)p.dvalue, slab);
+            return;
+        }
+        q = sequence(p, seq);
+        tile = ((q.len + kBwdTile - 1) >> kBwdLog2) - 1;
     }
-    const Place q = sequence(p, seq);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int ch = slab * kSlab + lane * 2, nch = min(2, max(0, p.width - ch));
+    From from(p, q, seq, slab, dynamic + warp * From::kBytes);
+    const int ch = from.ch, nch = from.nch;
     const bool vec = p.vec;
     const long long state_at = (long long)seq * p.width + ch;
+    auto rows_at = [&](long long t) { return (int)min((long long)S, max(0LL, q.len - t)); };
+    if (tile >= 0) from.ask_for((tile << kBwdLog2) + warp * S, rows_at((tile << kBwdLog2) + warp * S));
     float2 carry = two(0.0f);  // gradient of the state behind the steps in hand
-    if (p.glast) carry = load2(p.glast + state_at, vec, nch);
-    // codes lie in rows of width, one after the other
-    const long long gate_step = PACKED ? p.width : p.gate_step, value_step = PACKED ? p.width : p.value_step;
-    const V *const gate = (const V *)p.gate + (PACKED || p.offsets ? q.first * gate_step : seq * p.gate_seq) + slab * kSlab;
-    const V *const value = (const V *)p.value + (PACKED || p.offsets ? q.first * value_step : seq * p.value_seq) + slab * kSlab;
-    const T *const grad = (const T *)p.gh + q.first * p.width + slab * kSlab;
-    const int held_log2 = p.interval_log2, held = 1 << held_log2;  // kBwdTile * p.cluster
-    const int per_row = (p.width + kPackGroup - 1) / kPackGroup, left = p.width - slab * kSlab;
-    Rows<T, S> &gs = reinterpret_cast<Rows<T, S> *>(dynamic)[warp];
-    Rows<V, S> *const inputs = reinterpret_cast<Rows<V, S> *>(dynamic + kScanWarps * sizeof(Rows<T, S>));
-    Rows<V, S> &zs = inputs[warp], &us = inputs[kScanWarps + warp];
-    unsigned scales = 0;
-    const bool wide = p.wide;
-    const V *const gate_from = asks_from<V, S>(gate, gate_step), *const value_from = asks_from<V, S>(value, value_step);
-    const T *const grad_from = asks_from<T, S>(grad, p.width);
-    auto ask_all = [&](long long t) {
-        const int cnt = (int)min((long long)S, max(0LL, q.len - t));
-        if (cnt <= 0) return;
-        ask(zs, gate_from + t * gate_step, gate_step, cnt, left);
-        ask(us, value_from + t * value_step, value_step, cnt, left);
-        ask(gs, grad_from + t * p.width, (long long)p.width, cnt, left);
-        copies_on_their_way();
-        if (PACKED) {
-            scales = ask_scales(p, q.first + t, per_row, slab, cnt);
-        }
-    };
-    int par = 0;
-    const long long last = ((q.len + held - 1) >> held_log2) - 1, mine = (long long)rank * kBwdTile + warp * S;
-    if (wide && last >= 0) ask_all((last << held_log2) + mine);
-    // a CTA's shared memory may be written to by others once it runs: waited for ahead of the first such store
-    if (p.cluster > 1) cg::this_cluster().sync();
-    const float inf = __uint_as_float(0x7f800000u);
-    for (long long k = last; k >= 0; --k, par ^= 1) {
-        const long long t0 = (k << held_log2) + mine;
-        const int cnt = (int)min((long long)S, max(0LL, q.len - t0));
-        // a step behind the end holds the state and has no gradient of its own
+    if constexpr (CHUNK) {
+        previous_done();
+        carry = *plane(p, 2, row, slab);
+    } else if (p.glast) {
+        carry = load2(p.glast + state_at, vec, nch);
+    }
+    for (int par = 0; tile >= 0; --tile, par ^= 1) {
+        const long long t0 = (tile << kBwdLog2) + warp * S;
+        const int cnt = rows_at(t0);
         float2 a[S], n[S], u[S], g[S], h = two(0.0f);
-        if (wide) {
-            copies_there();
-            if constexpr (PACKED) {
-                take_packed<S>(zs, us, scales, cnt, nch, inf, a, u);
-            } else {
-                take(zs, cnt, nch, inf, a);
-                take(us, cnt, nch, 0.0f, u);
-            }
-            take(gs, cnt, nch, 0.0f, g);
-            __syncwarp();
-            if (k > 0) ask_all(t0 - held);
+        from.take_from(t0, cnt, a, u, g);
+        if (!CHUNK && tile > 0) from.ask_for(t0 - kBwdTile, S);
+        if constexpr (CHUNK) {
+            h = *plane(p, 1, row, slab);
         } else {
-            if constexpr (PACKED) {
-                load_packed<S>((const unsigned char *)p.gate, p.gate_scales, q.first + t0, p.width, ch, vec, cnt, nch, inf, a);
-                load_packed<S>((const unsigned char *)p.value, p.value_scales, q.first + t0, p.width, ch, vec, cnt, nch, 0.0f, u);
-            } else {
-                load_rows<T, S>(gate + lane * 2 + t0 * gate_step, gate_step, vec, cnt, nch, inf, a);
-                load_rows<T, S>(value + lane * 2 + t0 * value_step, value_step, vec, cnt, nch, 0.0f, u);
-            }
-            load_rows<T, S>(grad + lane * 2 + t0 * p.width, p.width, vec, cnt, nch, 0.0f, g);
+            if (tile > 0)
+                h = load2(p.bounds + tile_row<kBwdLog2>(p, seq, q, tile) * p.width + ch, vec, nch);
+            else if (p.state)
+                h = load2(p.state + state_at, vec, nch);
         }
-        if (k > 0)
-            h = load2(p.bounds + bound_row(p, seq, q, k) * p.width + ch, vec, nch);
-        else if (p.state)
-            h = load2(p.state + state_at, vec, nch);
         float2 A = two(1.0f), H = two(0.0f), C = two(0.0f);
         const bool special = farthest(a) >= kFar;
         if (!special) {
@@ -717,9 +875,8 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
                 a[s] = w;
                 H = fma2(w, H, mul2(n[s], u[s]));
                 A = mul2(A, w);
+                C = fma2(A, g[s], C);
             }
-#pragma unroll
-            for (int s = S - 1; s >= 0; --s) C = mul2(a[s], add2(g[s], C));
         } else {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
@@ -729,37 +886,14 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
                 u[s] = looked_at(n[s], u[s]);
                 H = after(w, H, mul2(n[s], u[s]));
                 A = more(A, w);
+                C = make_float2(resets(A.x) ? C.x : fmaf(A.x, g[s].x, C.x), resets(A.y) ? C.y : fmaf(A.y, g[s].y, C.y));
             }
-#pragma unroll
-            for (int s = S - 1; s >= 0; --s) C = looked_at(a[s], mul2(a[s], add2(g[s], C)));
         }
         ex.warp[par][0][warp][lane] = map_of(A, H);
         ex.warp[par][1][warp][lane] = map_of(A, C);
         const bool any = __syncthreads_or(special);
         float2 c = carry;
-        if (p.cluster > 1) {
-            cg::cluster_group cluster = cg::this_cluster();
-            float2 ta = two(1.0f), th = two(0.0f), tc = two(0.0f);
-#pragma unroll
-            for (int w = 0; w < kScanWarps; ++w) {
-                const float4 m = ex.warp[par][0][w][lane];
-                th = through(m, th);
-                ta = product(ta, factor(m));
-                tc = through(ex.warp[par][1][kScanWarps - 1 - w][lane], tc);
-            }
-            for (int r = warp; r < p.cluster; r += kScanWarps) {
-                *cluster.map_shared_rank(&ex.rank[par][0][rank][lane], r) = map_of(ta, th);
-                *cluster.map_shared_rank(&ex.rank[par][1][rank][lane], r) = map_of(ta, tc);
-            }
-            cluster.sync();
-            for (int r = 0; r < rank; ++r) h = through(ex.rank[par][0][r][lane], h);
-            for (int r = p.cluster - 1; r >= 0; --r) {
-                if (r == rank) c = carry;
-                carry = through(ex.rank[par][1][r][lane], carry);
-            }
-            for (int w = kScanWarps - 1; w > warp; --w) c = through(ex.warp[par][1][w][lane], c);
-            for (int w = 0; w < warp; ++w) h = through(ex.warp[par][0][w][lane], h);
-        } else if (!any) {
+        if (!any) {
 #pragma unroll
             for (int w = kScanWarps - 1; w >= 0; --w) {
                 if (w == warp) c = carry;
@@ -820,8 +954,9 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
                     store2(du + (long long)s * p.width, vec, nch, g[s]);
                 }
         }
+        if (CHUNK) return;
     }
-    if (p.dstate && rank == 0 && warp == 0) store2(p.dstate + state_at, vec, nch, carry);
+    if (p.dstate && warp == 0) store2(p.dstate + state_at, vec, nch, carry);
 }
 
 // ------------------------------------------------------------------ one step
@@ -845,75 +980,104 @@ __global__ void __launch_bounds__(256) scan_step_k(const T *__restrict__ gate, c
 
 // ------------------------------------------------------------------ host side
 static bool aligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+static long long slabs_of(int width) { return (width + kSlab - 1) / kSlab; }
 
-// CTAs that share a sequence's steps
-static int scan_cluster(int n, long long steps, int width, int size, bool backward)
-{
-    (void)n; (void)steps; (void)width; (void)size; (void)backward;
-    return 1;
-}
+struct ScanDims {
+    int n;
+    long long steps, total;
+    int width, dtype;
+    bool ragged;
+    int size() const { return dtype == GN_F32 ? 4 : 2; }
+    long long tiles(int log2) const { return (steps + (1LL << log2) - 1) >> log2; }
+    long long tile_rows(int log2) const { return ragged ? (total >> log2) + n + 1 : n * tiles(log2); }
+};
 
-static int scan_check(int n, long long steps, long long total, int width, int dtype, bool ragged)
+static int scan_check(const ScanDims &d)
 {
-    if (n < 0 || steps < 0 || total < 0 || width <= 0) return GN_ERR_BAD_SHAPE;
-    if (!ragged && total != n * steps) return GN_ERR_BAD_SHAPE;
-    if (dtype < GN_F32 || dtype > GN_F16) return GN_ERR_UNSUPPORTED;
-    if (total > (1LL << 48) / width) return GN_ERR_TOO_LARGE;
-    const long long slabs = (width + kSlab - 1) / kSlab;
-    if ((n + 1LL) * slabs * kMaxCluster > 0x7fffffffLL) return GN_ERR_TOO_LARGE;
+    if (d.n < 0 || d.steps < 0 || d.total < 0 || d.width <= 0) return GN_ERR_BAD_SHAPE;
+    if (d.steps > 0 && d.n > (1LL << 48) / d.steps) return GN_ERR_TOO_LARGE;
+    if (!d.ragged && d.total != d.n * d.steps) return GN_ERR_BAD_SHAPE;
+    if (d.dtype < GN_F32 || d.dtype > GN_F16) return GN_ERR_UNSUPPORTED;
+    if (d.total > (1LL << 48) / d.width) return GN_ERR_TOO_LARGE;
+    if ((d.n + 1LL) * slabs_of(d.width) > 0x7fffffffLL || d.tile_rows(kBwdLog2) > 0x7fffffffLL / slabs_of(d.width)) return GN_ERR_TOO_LARGE;
     return GN_OK;
 }
 
-// log2 of the steps between two states that a backward pass starts from: what its CTA or cluster holds
-static int scan_interval_log2(int n, long long steps, long long total, int width, int dtype, bool ragged)
+// Whether the forward pass (backward: the backward pass) walks or goes by chunks
+static bool scan_walks(const ScanDims &d, bool backward, bool packed)
 {
-    const long long mean = ragged ? total / (n > 0 ? n : 1) : steps;
-    int log2 = 0;
-    while ((1 << log2) < kBwdTile * scan_cluster(n, mean, width, dtype == GN_F32 ? 4 : 2, true)) ++log2;
-    return log2;
+    const int log2 = backward ? kBwdLog2 : kFwdLog2;
+    if (d.n == 0 || (d.ragged ? d.total : d.steps) <= 1LL << log2) return true;  // nothing, or a single tile
+    if (backward && packed) return false;
+    return d.n * slabs_of(d.width) >= 3 * sm_count();
 }
 
-static int launch_scan(void (*kern)(const Scan), const Scan &p, size_t tile_bytes, const char *what, cudaStream_t st)
+static size_t bounds_bytes(const ScanDims &d)
 {
-    const size_t smem = p.wide ? tile_bytes * kSlab : 0;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((p.n + (p.offsets ? 1LL : 0LL)) * p.slabs * p.cluster));
-    cfg.blockDim = dim3(kScanThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = p.cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-    cudaError_t e = cudaSuccess;
-    if (smem > 0) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kern, p);
-    if (e != cudaSuccess) {
-        record_cuda_error(e, what);
-        (void)cudaGetLastError();
-        return GN_ERR_CUDA;
-    }
+    if (d.n == 0 || d.total == 0 || (d.ragged ? d.total : d.steps) <= kBwdTile || !scan_walks(d, true, false)) return 0;
+    return sizeof(float) * (size_t)d.tile_rows(kBwdLog2) * d.width;
+}
+static size_t maps_bytes(const ScanDims &d, bool backward, bool packed)
+{
+    if ((d.n == 0 && !d.ragged) || d.total == 0 || scan_walks(d, backward, packed)) return 0;
+    return sizeof(float) * (backward ? 3 : 2) * (size_t)d.tile_rows(backward ? kBwdLog2 : kFwdLog2) * slabs_of(d.width) * kSlab;
+}
+
+static int prepare_kernel(const void *kern, size_t smem, const char *what)
+{
+    if (smem == 0) return GN_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) return GN_OK;
+    record_cuda_error(e, what);
+    (void)cudaGetLastError();
+    return GN_ERR_CUDA;
+}
+
+// the three kernels of the way by chunks
+template <typename T, bool PACKED, bool BACKWARD>
+static int launch_chunks(Scan &p, const ScanDims &d, void (*work)(const Scan), size_t work_smem, const char *what, cudaStream_t st)
+{
+    constexpr int kLog2 = BACKWARD ? kBwdLog2 : kFwdLog2;
+    p.map_rows = d.tile_rows(kLog2);
+    const size_t smem = p.wide ? kScanWarps * Source<T, PACKED, BACKWARD, kSumSteps>::kBytes : 0;
+    int rc = prepare_kernel((const void *)scan_maps_k<T, PACKED, BACKWARD>, smem, what);
+    if (rc == GN_OK) rc = prepare_kernel((const void *)work, work_smem, what);
+    if (rc != GN_OK) return rc;
+    const long long warps = p.map_rows * p.slabs;
+    scan_maps_k<T, PACKED, BACKWARD><<<(unsigned)((warps + kScanWarps - 1) / kScanWarps), kScanThreads, smem, st>>>(p);
+    launch_after(scan_starts_k<T, BACKWARD>, dim3((unsigned)((p.n + (d.ragged ? 1LL : 0LL)) * p.slabs)), dim3(32 * kStartWarps), 0, st, p);
+    launch_after(work, dim3((unsigned)warps), dim3(kScanThreads), work_smem, st, p);
     return check_launch(what);
 }
 
 template <typename T>
-static int scan_forward(Scan &p, cudaStream_t st)
+static int launch_forward(Scan &p, const ScanDims &d, cudaStream_t st)
 {
-    p.slabs = (p.width + kSlab - 1) / kSlab;
-    return launch_scan(p.pack_gate ? scan_forward_k<T, false, true> : scan_forward_k<T, false, false>, p, kFwdTile * 2 * sizeof(T), "gated_scan", st);
+    const bool keep = p.pack_gate != nullptr;
+    const size_t smem = p.wide ? kScanWarps * Source<T, false, false, kFwdSteps>::kBytes : 0;
+    if (!scan_walks(d, false, false))
+        return launch_chunks<T, false, false>(p, d, keep ? scan_forward_k<T, true, true> : scan_forward_k<T, false, true>, smem, "gated_scan", st);
+    void (*const kern)(const Scan) = keep ? scan_forward_k<T, true, false> : scan_forward_k<T, false, false>;
+    const int rc = prepare_kernel((const void *)kern, smem, "gated_scan");
+    if (rc != GN_OK) return rc;
+    kern<<<(unsigned)((p.n + (d.ragged ? 1LL : 0LL)) * p.slabs), kScanThreads, smem, st>>>(p);
+    return check_launch("gated_scan");
 }
 
-template <typename T>
-static int scan_backward(Scan &p, bool packed, bool long_sequences, cudaStream_t st)
+template <typename T, bool PACKED>
+static int launch_backward(Scan &p, const ScanDims &d, cudaStream_t st)
 {
-    p.slabs = (p.width + kSlab - 1) / kSlab;
-    if (packed && long_sequences) {  // the states that the codes lead to
-        const int rc = launch_scan(scan_forward_k<T, true, false>, p, kFwdTile * 2, "gated_scan states", st);
-        if (rc != GN_OK) return rc;
-    }
-    return launch_scan(packed ? scan_backward_k<T, true> : scan_backward_k<T, false>, p, kBwdTile * ((packed ? 2 : 2 * sizeof(T)) + sizeof(T)), "gated_scan backward", st);
+    const size_t smem = p.wide ? kScanWarps * Source<T, PACKED, true, kBwdSteps>::kBytes : 0;
+    if (!scan_walks(d, true, PACKED)) return launch_chunks<T, PACKED, true>(p, d, scan_backward_k<T, PACKED, true>, smem, "gated_scan backward", st);
+    const int rc = prepare_kernel((const void *)scan_backward_k<T, PACKED, false>, smem, "gated_scan backward");
+    if (rc != GN_OK) return rc;
+    scan_backward_k<T, PACKED, false><<<(unsigned)((p.n + (d.ragged ? 1LL : 0LL)) * p.slabs), kScanThreads, smem, st>>>(p);
+    return check_launch("gated_scan backward");
+}
+template <typename T>
+static int launch_backward(Scan &p, const ScanDims &d, bool packed, cudaStream_t st)
+{
+    return packed ? launch_backward<T, true>(p, d, st) : launch_backward<T, false>(p, d, st);
 }
 
 }  // namespace gn
@@ -924,74 +1088,88 @@ extern "C" {
 
 GN_API size_t gn_gated_scan_bounds_bytes(int n, long long steps, long long total, int width, int dtype, int ragged)
 {
-    if (scan_check(n, steps, total, width, dtype, ragged != 0) != GN_OK || n == 0 || total == 0) return 0;
-    const int interval = 1 << scan_interval_log2(n, steps, total, width, dtype, ragged != 0);
-    if ((ragged ? total : steps) <= interval) return 0;
-    const long long rows = ragged ? total / interval + n + 1 : n * ((steps + interval - 1) / interval);
-    return sizeof(float) * (size_t)rows * width;
+    const ScanDims d{n, ragged ? 0 : steps, total, width, dtype, ragged != 0};
+    return scan_check(d) == GN_OK ? bounds_bytes(d) : 0;
+}
+
+GN_API size_t gn_gated_scan_workspace_bytes(int n, long long steps, long long total, int width, int dtype, int ragged, int backward, int packed)
+{
+    const ScanDims d{n, ragged ? 0 : steps, total, width, dtype, ragged != 0};
+    return scan_check(d) == GN_OK ? maps_bytes(d, backward != 0, packed != 0) : 0;
 }
 
 GN_API int gn_gated_scan_forward(const void *gate, const void *value, const float *state, const long long *offsets, void *h, float *last,
                                  void *gate_codes, void *gate_scales, void *value_codes, void *value_scales, float *bounds, int n,
                                  long long steps, long long total, int width, long long gate_seq, long long gate_step, long long value_seq,
-                                 long long value_step, int dtype, void *stream)
+                                 long long value_step, int dtype, void *workspace, size_t workspace_bytes, void *stream)
 {
-    const int rc = scan_check(n, steps, total, width, dtype, offsets != nullptr);
+    const ScanDims d{n, offsets ? 0 : steps, total, width, dtype, offsets != nullptr};
+    const int rc = scan_check(d);
     if (rc != GN_OK) return rc;
     if (gate_codes && (!gate_scales || !value_codes || !value_scales)) return GN_ERR_NULL_POINTER;
     if (total > 0 && (!gate || !value || !h)) return GN_ERR_NULL_POINTER;
     if (n == 0 && !(offsets && total > 0)) return GN_OK;
+    const size_t need = maps_bytes(d, false, false);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return GN_ERR_WORKSPACE;
     Scan p{};
     p.gate = gate; p.value = value; p.state = state; p.offsets = offsets; p.h = h; p.last = last;
     p.pack_gate = (unsigned char *)gate_codes; p.pack_gate_scales = (unsigned char *)gate_scales;
     p.pack_value = (unsigned char *)value_codes; p.pack_value_scales = (unsigned char *)value_scales;
-    p.bounds = gate_codes ? nullptr : bounds;  // those of the codes are found when they are wanted
-    p.interval_log2 = scan_interval_log2(n, steps, total, width, dtype, offsets != nullptr);
+    p.bounds = gate_codes || bounds_bytes(d) == 0 ? nullptr : bounds;
+    p.maps = static_cast<float *>(workspace);
     p.gate_seq = gate_seq; p.gate_step = gate_step; p.value_seq = value_seq; p.value_step = value_step;
-    p.n = n; p.steps = steps; p.total = total; p.width = width;
-    const int size = dtype == GN_F32 ? 4 : 2;
-    p.cluster = scan_cluster(n, offsets ? total / (n > 0 ? n : 1) : steps, width, size, false);
+    p.n = n; p.steps = d.steps; p.total = total; p.width = width;
+    p.slabs = (int)slabs_of(width);
+    p.padded = p.slabs * kSlab;
+    const int size = d.size();
     p.vec = width % 2 == 0 && gate_seq % 2 == 0 && gate_step % 2 == 0 && value_seq % 2 == 0 && value_step % 2 == 0 && aligned(gate, 2 * size) &&
             aligned(value, 2 * size) && aligned(h, 2 * size) && aligned(state, 8) && aligned(last, 8) && aligned(bounds, 8) &&
             aligned(gate_codes, 2) && aligned(value_codes, 2);
     p.wide = (long long)width * size % 16 == 0 && gate_seq * size % 16 == 0 && gate_step * size % 16 == 0 && value_seq * size % 16 == 0 &&
              value_step * size % 16 == 0 && aligned(gate, 16) && aligned(value, 16);
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == GN_F32) return scan_forward<float>(p, st);
-    if (dtype == GN_BF16) return scan_forward<__nv_bfloat16>(p, st);
-    return scan_forward<__half>(p, st);
+    if (dtype == GN_F32) return launch_forward<float>(p, d, st);
+    if (dtype == GN_BF16) return launch_forward<__nv_bfloat16>(p, d, st);
+    return launch_forward<__half>(p, d, st);
 }
 
 GN_API int gn_gated_scan_backward(const void *gate, const void *value, const void *gate_scales, const void *value_scales, const float *state,
-                                  const long long *offsets, float *bounds, const void *grad_h, const float *grad_last, void *grad_gate,
+                                  const long long *offsets, const float *bounds, const void *grad_h, const float *grad_last, void *grad_gate,
                                   void *grad_value, float *grad_state, int n, long long steps, long long total, int width, long long gate_seq,
-                                  long long gate_step, long long value_seq, long long value_step, int dtype, void *stream)
+                                  long long gate_step, long long value_seq, long long value_step, int dtype, void *workspace,
+                                  size_t workspace_bytes, void *stream)
 {
-    const int rc = scan_check(n, steps, total, width, dtype, offsets != nullptr);
+    const ScanDims d{n, offsets ? 0 : steps, total, width, dtype, offsets != nullptr};
+    const int rc = scan_check(d);
     if (rc != GN_OK) return rc;
     if (!gate_scales != !value_scales) return GN_ERR_NULL_POINTER;
+    const bool packed = gate_scales != nullptr;
     if (total > 0 && (!gate || !value || !grad_h || !grad_gate || !grad_value)) return GN_ERR_NULL_POINTER;
     if (n == 0 && !(offsets && total > 0)) return GN_OK;
-    const bool long_sequences = gn_gated_scan_bounds_bytes(n, steps, total, width, dtype, offsets != nullptr) > 0;
-    if (long_sequences && !bounds) return GN_ERR_WORKSPACE;
+    if (!packed && bounds_bytes(d) > 0 && !bounds) return GN_ERR_WORKSPACE;
+    const size_t need = maps_bytes(d, true, packed);
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return GN_ERR_WORKSPACE;
     Scan p{};
-    p.gate = gate; p.value = value; p.state = state; p.offsets = offsets; p.bounds = bounds;
+    p.gate = gate; p.value = value; p.state = state; p.offsets = offsets; p.bounds = const_cast<float *>(bounds);
+    p.maps = static_cast<float *>(workspace);
     p.gate_scales = (const unsigned char *)gate_scales; p.value_scales = (const unsigned char *)value_scales;
     p.gh = grad_h; p.glast = grad_last; p.dgate = grad_gate; p.dvalue = grad_value; p.dstate = grad_state;
-    p.interval_log2 = scan_interval_log2(n, steps, total, width, dtype, offsets != nullptr);
-    p.gate_seq = gate_seq; p.gate_step = gate_step; p.value_seq = value_seq; p.value_step = value_step;
-    p.n = n; p.steps = steps; p.total = total; p.width = width;
-    p.cluster = (1 << p.interval_log2) / kBwdTile;
-    const int size = dtype == GN_F32 ? 4 : 2, in = gate_scales ? 1 : size;
-    p.vec = width % 2 == 0 && gate_seq % 2 == 0 && gate_step % 2 == 0 && value_seq % 2 == 0 && value_step % 2 == 0 && aligned(gate, 2 * in) &&
+    if (!packed) {
+        p.gate_seq = gate_seq; p.gate_step = gate_step; p.value_seq = value_seq; p.value_step = value_step;
+    }
+    p.n = n; p.steps = d.steps; p.total = total; p.width = width;
+    p.slabs = (int)slabs_of(width);
+    p.padded = p.slabs * kSlab;
+    const int size = d.size(), in = packed ? 1 : size;
+    p.vec = width % 2 == 0 && p.gate_seq % 2 == 0 && p.gate_step % 2 == 0 && p.value_seq % 2 == 0 && p.value_step % 2 == 0 && aligned(gate, 2 * in) &&
             aligned(value, 2 * in) && aligned(grad_h, 2 * size) && aligned(grad_gate, 2 * size) && aligned(grad_value, 2 * size) &&
             aligned(state, 8) && aligned(grad_last, 8) && aligned(grad_state, 8) && aligned(bounds, 8);
-    p.wide = (long long)width * in % 16 == 0 && (long long)width * size % 16 == 0 && gate_seq * in % 16 == 0 && gate_step * in % 16 == 0 &&
-             value_seq * in % 16 == 0 && value_step * in % 16 == 0 && aligned(gate, 16) && aligned(value, 16) && aligned(grad_h, 16);
+    p.wide = (long long)width * in % 16 == 0 && (long long)width * size % 16 == 0 && p.gate_seq * in % 16 == 0 && p.gate_step * in % 16 == 0 &&
+             p.value_seq * in % 16 == 0 && p.value_step * in % 16 == 0 && aligned(gate, 16) && aligned(value, 16) && aligned(grad_h, 16);
     cudaStream_t st = (cudaStream_t)stream;
-    if (dtype == GN_F32) return scan_backward<float>(p, gate_scales != nullptr, long_sequences, st);
-    if (dtype == GN_BF16) return scan_backward<__nv_bfloat16>(p, gate_scales != nullptr, long_sequences, st);
-    return scan_backward<__half>(p, gate_scales != nullptr, long_sequences, st);
+    if (dtype == GN_F32) return launch_backward<float>(p, d, packed, st);
+    if (dtype == GN_BF16) return launch_backward<__nv_bfloat16>(p, d, packed, st);
+    return launch_backward<__half>(p, d, packed, st);
 }
 
 GN_API int gn_gated_scan_step(const void *gate, const void *value, const float *state, void *h, float *out_state, long long rows, int width,

@@ -25,6 +25,18 @@ def _strides(t: torch.Tensor):
     return (t.stride(0), t.stride(1)) if t.dim() == 3 else (0, t.stride(0))
 
 
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _nbytes(t) -> int:
+    return 0 if t is None else t.numel()
+
+
+def _scratch(nbytes: int, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
 def _check_scan(gate, value, state, offsets):
     """Returns (sequences, steps of each (0: ragged), rows in all)."""
     for name, t in (("gate", gate), ("value", value)):
@@ -70,26 +82,26 @@ class GatedScanOp(_Op):
         dtype, dev = dtype_id(gate, "gate"), gate.device
         lead = 2 if offsets is None else 1
         ctx.set_materialize_grads(False)
-        ctx.shape, ctx.dims, ctx.has_state = gate.shape, (n, steps, total), state is not None
+        ctx.shape, ctx.has_state = gate.shape, state is not None
         z, u = _rows(gate, lead), _rows(value, lead)
         width = z.shape[-1]
         s = None if state is None else state.contiguous()
         offsets = None if offsets is None else _device_offsets(offsets, total, dev)
         h = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
         last = torch.empty((n, *gate.shape[lead:]), dtype=torch.float32, device=dev)
+        size = (n, steps, total, width, dtype, int(lead == 1))
         kept, bounds = [None] * 4, None
         with torch.cuda.device(dev):
-            need = 0
             if any(ctx.needs_input_grad[:3]):
-                need = int(lib.gn_gated_scan_bounds_bytes(n, steps, total, width, dtype, int(lead == 1)))
                 if packed:
                     kept = [t for x in (z, u) for t in empty_packed(x.shape, lead, x.dtype, dev)[:2]]
-                elif need:
-                    bounds = torch.empty(need, dtype=torch.uint8, device=dev)
-            ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-            check(lib.gn_gated_scan_forward(z.data_ptr(), u.data_ptr(), ptr(s), ptr(offsets), h.data_ptr(), last.data_ptr(), *map(ptr, kept),
-                                            ptr(bounds), n, steps, total, width, *_strides(z), *_strides(u), dtype, stream_of(gate)))
-        ctx.cfg = (need, width, dtype, gate.dtype)
+                else:
+                    bounds = _scratch(lib.gn_gated_scan_bounds_bytes(*size), dev)
+            work = _scratch(lib.gn_gated_scan_workspace_bytes(*size, 0, 0), dev)
+            check(lib.gn_gated_scan_forward(z.data_ptr(), u.data_ptr(), _ptr(s), _ptr(offsets), h.data_ptr(), last.data_ptr(), *map(_ptr, kept),
+                                            _ptr(bounds), n, steps, total, width, *_strides(z), *_strides(u), dtype, _ptr(work), _nbytes(work),
+                                            stream_of(gate)))
+        ctx.cfg = (size, gate.dtype)
         if kept[0] is not None:
             ctx.save_for_backward(kept[0], kept[2], kept[1], kept[3], s, offsets, None)
         else:
@@ -100,20 +112,18 @@ class GatedScanOp(_Op):
     @once_differentiable
     def backward(ctx, grad_h, grad_last):
         z, u, z_scales, u_scales, s, offsets, bounds = ctx.saved_tensors
-        (n, steps, total), (need, width, dtype, kind) = ctx.dims, ctx.cfg
-        dev = z.device
+        size, kind = ctx.cfg
+        dev, packed = z.device, z_scales is not None
         grad_h = torch.zeros(ctx.shape, dtype=kind, device=dev) if grad_h is None else grad_h.contiguous()
         grad_last = None if grad_last is None else grad_last.contiguous()
         dz, du = (torch.empty(ctx.shape, dtype=kind, device=dev) for _ in range(2))
         ds = torch.empty_like(s) if ctx.has_state and ctx.needs_input_grad[2] else None
-        strides = (0, 0, 0, 0) if z_scales is not None else (*_strides(z), *_strides(u))
+        strides = (0, 0, 0, 0) if packed else (*_strides(z), *_strides(u))
         with torch.cuda.device(dev):
-            if need and bounds is None:
-                bounds = torch.empty(need, dtype=torch.uint8, device=dev)
-            ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-            check(lib.gn_gated_scan_backward(z.data_ptr(), u.data_ptr(), ptr(z_scales), ptr(u_scales), ptr(s), ptr(offsets), ptr(bounds),
-                                             grad_h.data_ptr(), ptr(grad_last), dz.data_ptr(), du.data_ptr(), ptr(ds), n, steps, total, width,
-                                             *strides, dtype, stream_of(z)))
+            work = _scratch(lib.gn_gated_scan_workspace_bytes(*size, 1, int(packed)), dev)
+            check(lib.gn_gated_scan_backward(z.data_ptr(), u.data_ptr(), _ptr(z_scales), _ptr(u_scales), _ptr(s), _ptr(offsets), _ptr(bounds),
+                                             grad_h.data_ptr(), _ptr(grad_last), dz.data_ptr(), du.data_ptr(), _ptr(ds), *size[:4], *strides,
+                                             size[4], _ptr(work), _nbytes(work), stream_of(z)))
         return dz, du, ds, None, None
 
 

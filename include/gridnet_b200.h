@@ -559,19 +559,22 @@ GN_API int gn_norm_backward_packed_f32(const void *codes, const void *scales, co
  *
  * For the backward pass either keep gate, value, state and `bounds` (gn_gated_scan_bounds_bytes; 0: none needed), or pass
  * gate_codes, gate_scales, value_codes, value_scales ([total][width] and [total][ceil(width / 32)] bytes, format as above) to the
- * forward call and keep those: the gradients are then those of the same recurrence at the unpacked gate and value, gate and value of the
- * backward call are the codes, their strides are not looked at, and bounds is scratch of the same size. Without a backward pass all five may be NULL. grad_last,
- * grad_state and state may be NULL. All gradients are overwritten. */
+ * forward call and keep those: the gradients are then those of the same recurrence at the unpacked gate and value; gate and value of the
+ * backward call are the codes, their strides are not looked at. Without a backward pass all five may be NULL. grad_last, grad_state and state
+ * may be NULL. All gradients are overwritten. workspace: 16-byte aligned, gn_gated_scan_workspace_bytes (0: none needed). */
 GN_API size_t gn_gated_scan_bounds_bytes(int n, long long steps, long long total, int width, int dtype, int ragged);
+GN_API size_t gn_gated_scan_workspace_bytes(int n, long long steps, long long total, int width, int dtype, int ragged, int backward,
+                                            int packed);
 GN_API int gn_gated_scan_forward(const void *gate, const void *value, const float *state, const long long *offsets, void *h, float *last,
                                  void *gate_codes, void *gate_scales, void *value_codes, void *value_scales, float *bounds, int n,
                                  long long steps, long long total, int width, long long gate_seq, long long gate_step,
-                                 long long value_seq, long long value_step, int dtype, void *stream);
+                                 long long value_seq, long long value_step, int dtype, void *workspace, size_t workspace_bytes,
+                                 void *stream);
 GN_API int gn_gated_scan_backward(const void *gate, const void *value, const void *gate_scales, const void *value_scales,
-                                  const float *state, const long long *offsets, float *bounds, const void *grad_h,
+                                  const float *state, const long long *offsets, const float *bounds, const void *grad_h,
                                   const float *grad_last, void *grad_gate, void *grad_value, float *grad_state, int n, long long steps,
                                   long long total, int width, long long gate_seq, long long gate_step, long long value_seq,
-                                  long long value_step, int dtype, void *stream);
+                                  long long value_step, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 /* One step of `rows` sequences: h and out_state [rows][width]; out_state may be state. gate_row, value_row: distance of rows in elements. */
 GN_API int gn_gated_scan_step(const void *gate, const void *value, const float *state, void *h, float *out_state, long long rows, int width,
                               long long gate_row, long long value_row, int dtype, void *stream);

@@ -40,17 +40,30 @@ def test_argument_errors_of_the_library():
     assert lib.gn_pack8(None, None, None, 0, 4, 0, None) == 0 and lib.gn_unpack8(None, None, None, 4, 0, 2, None) == 0
     fwd, bwd, step = lib.gn_gated_scan_forward, lib.gn_gated_scan_backward, lib.gn_gated_scan_step
     head, tail = [one, one, None, None, one, None], [32, 8, 32, 8]
-    assert fwd(*head, *[None] * 5, 1, 4, 4, 0, *tail, 0, None) == -3  # width
-    assert fwd(*head, *[None] * 5, 1, 4, 5, 8, *tail, 0, None) == -3  # total
-    assert fwd(*head, *[None] * 5, 1, 4, 4, 8, *tail, 9, None) == -8  # type
-    assert fwd(*head, *[None] * 5, 1, 1 << 40, 1 << 40, 1 << 20, *tail, 0, None) == -9
-    assert fwd(None, *head[1:], *[None] * 5, 1, 4, 4, 8, *tail, 0, None) == -1
-    assert fwd(*head, one, *[None] * 4, 1, 4, 4, 8, *tail, 0, None) == -1  # codes of the gate alone
-    assert fwd(None, None, None, None, None, None, *[None] * 5, 0, 4, 0, 8, *tail, 0, None) == 0
-    assert bwd(one, one, one, None, None, None, None, one, None, one, one, None, 1, 4, 4, 8, *tail, 0, None) == -1
-    assert bwd(one, one, None, None, None, None, None, None, None, one, one, None, 1, 4, 4, 8, *tail, 0, None) == -1
-    assert lib.gn_gated_scan_bounds_bytes(1, 100000, 100000, 8, 0, 0) > 0  # and without that scratch:
-    assert bwd(one, one, None, None, None, None, None, one, None, one, one, None, 1, 100000, 100000, 8, *tail, 0, None) == -6
+    assert fwd(*head, *[None] * 5, 1, 4, 4, 0, *tail, 0, None, 0, None) == -3  # width
+    assert fwd(*head, *[None] * 5, 1, 4, 5, 8, *tail, 0, None, 0, None) == -3  # total
+    assert fwd(*head, *[None] * 5, 1, 4, 4, 8, *tail, 9, None, 0, None) == -8  # type
+    assert fwd(*head, *[None] * 5, 1, 1 << 40, 1 << 40, 1 << 20, *tail, 0, None, 0, None) == -9
+    assert fwd(*head, *[None] * 5, 1 << 30, 1 << 40, 1, 8, *tail, 0, None, 0, None) == -9
+    assert fwd(None, *head[1:], *[None] * 5, 1, 4, 4, 8, *tail, 0, None, 0, None) == -1
+    assert fwd(*head, one, *[None] * 4, 1, 4, 4, 8, *tail, 0, None, 0, None) == -1  # codes of the gate alone
+    assert fwd(None, None, None, None, None, None, *[None] * 5, 0, 4, 0, 8, *tail, 0, None, 0, None) == 0
+    assert bwd(one, one, one, None, None, None, None, one, None, one, one, None, 1, 4, 4, 8, *tail, 0, None, 0, None) == -1
+    assert bwd(one, one, None, None, None, None, None, None, None, one, one, None, 1, 4, 4, 8, *tail, 0, None, 0, None) == -1
+    # scratch that is needed and is not there, too small, or not on 16 bytes; what the forward pass leaves for the backward pass
+    few, many = (1, 100000, 100000, 8), (1000, 100, 100000, 64)
+    need = lib.gn_gated_scan_workspace_bytes(*few, 0, 0, 0, 0)
+    assert need > 0 and lib.gn_gated_scan_bounds_bytes(*few, 0, 0) == 0
+    for work in ((None, need), (one, need - 1), (one + 4, need)):
+        assert fwd(*head, *[None] * 5, *few, *tail, 0, *work, None) == -6
+    for packed in (0, 1):
+        need = lib.gn_gated_scan_workspace_bytes(*few, 0, 0, 1, packed)
+        scales = (one, one) if packed else (None, None)
+        for work in ((None, need), (one, need - 1), (one + 4, need)):
+            assert bwd(one, one, *scales, None, None, None, one, None, one, one, None, *few, *tail, 0, *work, None) == -6
+    assert lib.gn_gated_scan_workspace_bytes(*many, 0, 0, 0, 0) == 0 and lib.gn_gated_scan_workspace_bytes(*many, 0, 0, 1, 1) > 0
+    assert lib.gn_gated_scan_bounds_bytes(*many, 0, 0) > 0
+    assert bwd(one, one, None, None, None, None, None, one, None, one, one, None, *many, 6400, 64, 6400, 64, 0, None, 0, None) == -6
     assert lib.gn_gated_scan_bounds_bytes(1, 1, 1, 8, 0, 0) == 0 and lib.gn_gated_scan_bounds_bytes(-1, 1, 1, 8, 0, 0) == 0
     assert step(one, one, one, one, one, -1, 8, 8, 8, 0, None) == -3 and step(one, one, one, one, one, 1, 0, 8, 8, 0, None) == -3
     assert step(one, one, one, one, one, 1, 8, 8, 8, -1, None) == -8 and step(one, one, None, one, one, 1, 8, 8, 8, 0, None) == -1
@@ -62,21 +75,37 @@ def test_argument_errors_of_the_library():
     assert nb(*[one] * 5, None, one, one, 1, 8, one, 1 << 20, None) == -1 and nb(*[one] * 8, 1, 8, None, 0, None) == -6
 
 
-def test_boundaries_lie_apart():
-    """Ragged: the rows that hold states at boundaries (first / interval + sequence + k, k from 1) are rows of the scratch and no two the
-    same, whatever the lengths. The interval is found from the size that the library asks for."""
+def test_tiles_of_ragged_sequences_lie_apart():
+    """Rows that hold states and maps of tiles (first / tile + sequence + k): rows of the scratch, no two the same, and found again by the
+    search that the kernels do, whatever the lengths. The numbers of rows are found from the sizes that the library asks for."""
     from gridnet_b200._lib import lib
 
     r = np.random.default_rng(0)
-    for width, dtype in ((8, 0), (100, 1), (4096, 0)):
-        for n, total in ((1, 5000), (7, 5000), (40, 3000), (300, 4000)):
-            nbytes = lib.gn_gated_scan_bounds_bytes(n, 0, total, width, dtype, 1)
-            rows = nbytes // (4 * width)
-            interval = next(i for i in (64, 128, 256, 512, 1024, 2048) if total // i + n + 1 == rows) if rows else None
-            for _ in range(20 if rows else 0):
+    for n, total, width in ((1, 5000, 8), (7, 5000, 100), (40, 3000, 64), (600, 4000, 64)):
+        size = (n, 0, total, width, 0, 1)
+        padded = (width + 63) // 64 * 64
+        found = [(64, lib.gn_gated_scan_workspace_bytes(*size, 0, 0), 8 * padded), (32, lib.gn_gated_scan_workspace_bytes(*size, 1, 1), 12 * padded),
+                 (32, lib.gn_gated_scan_bounds_bytes(*size), 4 * width)]
+        assert sum(nbytes > 0 for _, nbytes, _ in found) == 2
+        for tile, nbytes, row_bytes in found:
+            if not nbytes:
+                continue
+            rows, rest = divmod(nbytes, row_bytes)
+            assert rest == 0
+            for _ in range(20):
                 ends = np.sort(np.concatenate([[0, total], r.integers(0, total + 1, n - 1)]))
-                used = [first // interval + i + k for i, (first, end) in enumerate(zip(ends, ends[1:])) for k in range(1, (end - first + interval - 1) // interval)]
-                assert len(set(used)) == len(used) and all(0 <= u < rows for u in used)
+                base = [int(first) // tile + i for i, first in enumerate(ends[:-1])]
+                used = {base[i] + k: (i, k) for i, (first, end) in enumerate(zip(ends, ends[1:])) for k in range((end - first + tile - 1) // tile)}
+                assert len(used) == sum((end - first + tile - 1) // tile for first, end in zip(ends, ends[1:]))
+                assert all(0 <= u < rows for u in used)
+                for row in range(rows):
+                    lo, hi = 0, n
+                    while hi - lo > 1:
+                        mid = (lo + hi) // 2
+                        lo, hi = (mid, hi) if base[mid] <= row else (lo, mid)
+                    k = row - base[lo]
+                    valid = k >= 0 and k * tile < ends[lo + 1] - ends[lo]
+                    assert used.get(row) == ((lo, k) if valid else None)
 
 
 def test_python_refusals():
