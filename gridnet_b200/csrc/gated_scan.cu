@@ -39,7 +39,7 @@ constexpr int kFwdLog2 = 6, kBwdLog2 = 5;     // of a tile's steps
 constexpr int kFwdTile = 1 << kFwdLog2, kBwdTile = 1 << kBwdLog2;
 static_assert(kFwdTile == kScanWarps * kFwdSteps && kBwdTile == kScanWarps * kBwdSteps, "a tile is what a CTA holds");
 constexpr int kSumSteps = 8;                  // steps that a thread composes at a time when a warp has a tile to itself
-constexpr int kStartWarps = 16;
+constexpr int kStartRuns = 64;                // at most
 
 struct Scan {
     const void *gate, *value;  // or codes
@@ -53,6 +53,7 @@ struct Scan {
     float *bounds;  // walk: state ahead of each backward tile of a sequence but the first
     float *maps;    // chunks: A, H and (backward) C of each tile, planes of map_rows x padded; H and C give way to where the tile starts
     long long map_rows;
+    int tiles_per_cta;  // chunks
     const void *gh;
     const float *glast;
     void *dgate, *dvalue;
@@ -146,9 +147,9 @@ __device__ __forceinline__ void store2(T *p, bool vec, int n, float2 v)
 
 // s(z) and s(-z) for |z| < kFar; everything else, and what is behind the end, goes through gates_any.
 // e = exp(-z) as 2^t: t is rounded, which is as if z were another number 1.3 half steps of float32 away, about as far as z has been rounded
-// to begin with. a = 1 / (1 + e) by the approximation and a Newton step r (2 - (1 + e) r), all with signs turned so that no operand has
-// to be negated: the approximation's error has a sign that is not even, which a memory of thousands of steps would add up
-// (8 x 2048 x 4096 without the step, gradient of the state: 1.4e-6 off in the 2-norm; the plain form is 2.7e-7 off).
+// to begin with. Where s(z) is the larger of the two it is 1 less the other, so that its error is its own rounding: memories of thousands of
+// steps add it up (8 x 2048 x 4096, gradient of the state, off in the 2-norm: 1.8e-7; as 1 / (1 + e) with a Newton step 2.3e-6, because of
+// the rounding of 1 + e; without that step 1.4e-6).
 constexpr float kFar = 80.0f;
 __device__ __forceinline__ void gates(float2 z, float2 &a, float2 &n)
 {
@@ -156,11 +157,12 @@ __device__ __forceinline__ void gates(float2 z, float2 &a, float2 &n)
     float2 e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
-    const float2 w = fma2(e, two(-1.0f), two(-1.0f));  // -(1 + e)
+    const float2 one = two(1.0f), w = add2(e, one);
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(w.x));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(w.y));
-    a = mul2(r, fma2(w, r, two(-2.0f)));
-    n = mul2(e, a);
+    n = mul2(e, r);
+    const float2 p = fma2(n, two(-1.0f), one);
+    a = make_float2(z.x < 0.0f ? r.x : p.x, z.y < 0.0f ? r.y : p.y);
 }
 // For every z: the smaller from exp(-|z|), which is 0 from |z| = 104 on, the larger as 1 less it
 __device__ __forceinline__ float2 gate_any(float z)  // (s(z), s(-z))
@@ -507,24 +509,29 @@ struct Source {
     static constexpr size_t kBytes = sizeof(Rows<V, S>) * 2 + (GRAD ? sizeof(Rows<T, S>) : 0);  // shared memory of a warp
     const Scan &p;
     const int slab, ch, nch, left;
-    const long long first, gate_step, value_step;
+    const long long gate_step, value_step;
+    long long first;
     const V *gate, *value;
     const T *grad;
     Rows<V, S> *zs, *us;
     Rows<T, S> *gs;
     Scales scales;
 
-    __device__ __forceinline__ Source(const Scan &p, const Place &q, int seq, int slab, unsigned char *shared)
-        : p(p), slab(slab), ch(slab * kSlab + (threadIdx.x & 31) * 2), nch(min(2, max(0, p.width - ch))), left(p.width - slab * kSlab), first(q.first),
+    __device__ __forceinline__ Source(const Scan &p, int slab, unsigned char *shared)
+        : p(p), slab(slab), ch(slab * kSlab + (threadIdx.x & 31) * 2), nch(min(2, max(0, p.width - ch))), left(p.width - slab * kSlab),
           // codes lie in rows of width, one after the other
           gate_step(PACKED ? p.width : p.gate_step), value_step(PACKED ? p.width : p.value_step)
     {
-        gate = (const V *)p.gate + (PACKED || p.offsets ? first * gate_step : seq * p.gate_seq) + slab * kSlab;
-        value = (const V *)p.value + (PACKED || p.offsets ? first * value_step : seq * p.value_seq) + slab * kSlab;
-        grad = GRAD ? (const T *)p.gh + first * p.width + slab * kSlab : nullptr;
         zs = reinterpret_cast<Rows<V, S> *>(shared);
         us = zs + 1;
         gs = reinterpret_cast<Rows<T, S> *>(us + 1);
+    }
+    __device__ __forceinline__ void turn_to(int seq, const Place &q)
+    {
+        first = q.first;
+        gate = (const V *)p.gate + (PACKED || p.offsets ? first * gate_step : seq * p.gate_seq) + slab * kSlab;
+        value = (const V *)p.value + (PACKED || p.offsets ? first * value_step : seq * p.value_seq) + slab * kSlab;
+        grad = GRAD ? (const T *)p.gh + first * p.width + slab * kSlab : nullptr;
     }
     // cnt rows from step t of the sequence on (none: nothing)
     __device__ __forceinline__ void ask_for(long long t, int cnt)
@@ -564,6 +571,44 @@ struct Source {
     }
 };
 
+// A tile of a sequence, and what comes after it: walk - the next one of the sequence (backward: the one before); chunks - the next
+// row of p.maps that belongs to a tile, up to the CTA's last one
+template <int LOG2, bool CHUNK, bool BACKWARD>
+struct Cursor {
+    Place q;
+    long long tile, row, end;
+    int seq;
+
+    __device__ __forceinline__ bool find(const Scan &p)
+    {
+        while (row < end && !tile_of_row<LOG2>(p, row, seq, q, tile)) ++row;
+        return row < end;
+    }
+    __device__ __forceinline__ bool start(const Scan &p, int place)
+    {
+        if (CHUNK) {
+            row = (long long)place * p.tiles_per_cta;
+            end = min(row + p.tiles_per_cta, p.map_rows);
+            return find(p);
+        }
+        seq = place;
+        q = sequence(p, seq);
+        tile = BACKWARD ? ((q.len + (1 << LOG2) - 1) >> LOG2) - 1 : 0;
+        return q.len > 0;
+    }
+    __device__ __forceinline__ bool next(const Scan &p)
+    {
+        if (CHUNK) {
+            ++row;
+            ++tile;
+            if (row < end && tile << LOG2 < q.len) return true;  // of the same sequence
+            return find(p);
+        }
+        if (BACKWARD) return --tile >= 0;
+        return ++tile << LOG2 < q.len;
+    }
+};
+
 // ------------------------------------------------------------------ chunks: what each tile amounts to, a warp per tile
 template <typename T, bool PACKED, bool BACKWARD>
 __global__ void __launch_bounds__(kScanThreads, 7) scan_maps_k(const Scan p)
@@ -579,7 +624,8 @@ __global__ void __launch_bounds__(kScanThreads, 7) scan_maps_k(const Scan p)
     Place q;
     long long k;
     if (!tile_of_row<kLog2>(p, row, seq, q, k)) return;
-    From from(p, q, seq, slab, dynamic + warp * From::kBytes);
+    From from(p, slab, dynamic + warp * From::kBytes);
+    from.turn_to(seq, q);
     long long t = k << kLog2;
     int rows = (int)min(1LL << kLog2, q.len - t);
     from.ask_for(t, min(S, rows));
@@ -613,37 +659,41 @@ __global__ void __launch_bounds__(kScanThreads, 7) scan_maps_k(const Scan p)
     if (BACKWARD) *plane(p, 2, row, slab) = C;
 }
 
-// ------------------------------------------------------------------ chunks: where each tile starts. A CTA has 64 channels of a sequence, a warp a
-// run of its tiles
+// ------------------------------------------------------------------ chunks: where each tile starts. A CTA has 16 channels of a sequence; 8 lanes, two
+// channels each, have a run of its tiles; there are up to 64 runs. Channels of the last slab that are not there are computed along
 template <typename T, bool BACKWARD>
-__global__ void __launch_bounds__(32 * kStartWarps) scan_starts_k(const Scan p)
+__global__ void __launch_bounds__(8 * kStartRuns) scan_starts_k(const Scan p)
 {
     constexpr int kLog2 = BACKWARD ? kBwdLog2 : kFwdLog2, kBatch = 8;
-    __shared__ float4 runs[BACKWARD ? 2 : 1][kStartWarps][32];
-    const int slab = blockIdx.x % p.slabs, seq = blockIdx.x / p.slabs;
+    __shared__ float4 runs[BACKWARD ? 2 : 1][kStartRuns][8];
+    const int all_runs = blockDim.x >> 3;
+    const int parts = p.padded / 16, part = blockIdx.x % parts, seq = blockIdx.x / parts;
     previous_done();
     if (seq >= p.n) {
-        if (BACKWARD) {
-            clear_rows<T>(p, (T *)p.dgate, slab);
-            clear_rows<T>(p, (T *)p.dvalue, slab);
-        } else {
-            clear_rows<T>(p, (T *)p.h, slab);
+        if (part % 4 == 0) {
+            if (BACKWARD) {
+                clear_rows<T>(p, (T *)p.dgate, part / 4);
+                clear_rows<T>(p, (T *)p.dvalue, part / 4);
+            } else {
+                clear_rows<T>(p, (T *)p.h, part / 4);
+            }
         }
         return;
     }
     const Place q = sequence(p, seq);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, ch = slab * kSlab + lane * 2, nch = min(2, max(0, p.width - ch));
+    const int lane = threadIdx.x & 7, run = threadIdx.x >> 3, ch = part * 16 + lane * 2, nch = min(2, max(0, p.width - ch));
     const long long state_at = (long long)seq * p.width + ch, tiles = (q.len + (1 << kLog2) - 1) >> kLog2, row = tile_row<kLog2>(p, seq, q, 0);
-    const long long per = (tiles + kStartWarps - 1) / kStartWarps, lo = min(tiles, warp * per), hi = min(tiles, lo + per);
+    const long long per = (tiles + all_runs - 1) / all_runs, lo = min(tiles, run * per), hi = min(tiles, lo + per);
+    auto at = [&](int way, long long k) { return reinterpret_cast<float2 *>(p.maps + (way * p.map_rows + row + k) * p.padded + ch); };
     float2 A = two(1.0f), H = two(0.0f), C = two(0.0f);
     for (long long k = lo; k < hi; k += kBatch) {
         float2 a[kBatch], h[kBatch], c[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const long long at = row + min(k + i, hi - 1);
-            a[i] = *plane(p, 0, at, slab);
-            h[i] = *plane(p, 1, at, slab);
-            if (BACKWARD) c[i] = *plane(p, 2, at, slab);
+            const long long j = min(k + i, hi - 1);
+            a[i] = *at(0, j);
+            h[i] = *at(1, j);
+            if (BACKWARD) c[i] = *at(2, j);
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i)
@@ -653,29 +703,30 @@ __global__ void __launch_bounds__(32 * kStartWarps) scan_starts_k(const Scan p)
                 A = product(A, a[i]);
             }
     }
-    runs[0][warp][lane] = map_of(A, H);
-    if (BACKWARD) runs[BACKWARD][warp][lane] = map_of(A, C);
+    runs[0][run][lane] = map_of(A, H);
+    if (BACKWARD) runs[BACKWARD][run][lane] = map_of(A, C);
     __syncthreads();
     float2 h = two(0.0f), c = two(0.0f);
     if (p.state) h = load2(p.state + state_at, p.vec, nch);
-    if (!BACKWARD && tiles == 0 && warp == 0 && p.last) store2(p.last + state_at, p.vec, nch, h);
-    for (int w = 0; w < warp; ++w) h = through(runs[0][w][lane], h);
+    if (!BACKWARD && tiles == 0 && run == 0 && p.last) store2(p.last + state_at, p.vec, nch, h);
+    const int used = per > 0 ? (int)((tiles + per - 1) / per) : 0;  // runs that have tiles
+    for (int r = 0; r < min(run, used); ++r) h = through(runs[0][r][lane], h);
     if (BACKWARD) {
         if (p.glast) c = load2(p.glast + state_at, p.vec, nch);
-        for (int w = kStartWarps - 1; w > warp; --w) c = through(runs[BACKWARD][w][lane], c);
+        for (int r = used - 1; r > run; --r) c = through(runs[BACKWARD][r][lane], c);
     }
     for (long long k = lo; k < hi; k += kBatch) {
         float2 a[kBatch], b[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const long long at = row + min(k + i, hi - 1);
-            a[i] = *plane(p, 0, at, slab);
-            b[i] = *plane(p, 1, at, slab);
+            const long long j = min(k + i, hi - 1);
+            a[i] = *at(0, j);
+            b[i] = *at(1, j);
         }
 #pragma unroll
         for (int i = 0; i < kBatch; ++i)
             if (k + i < hi) {
-                *plane(p, 1, row + k + i, slab) = h;
+                *at(1, k + i) = h;
                 h = through(a[i], h, b[i]);
             }
     }
@@ -684,18 +735,18 @@ __global__ void __launch_bounds__(32 * kStartWarps) scan_starts_k(const Scan p)
             float2 a[kBatch], b[kBatch];
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-                const long long at = row + max(k - i, lo);
-                a[i] = *plane(p, 0, at, slab);
-                b[i] = *plane(p, 2, at, slab);
+                const long long j = max(k - i, lo);
+                a[i] = *at(0, j);
+                b[i] = *at(2, j);
             }
 #pragma unroll
             for (int i = 0; i < kBatch; ++i)
                 if (k - i >= lo) {
-                    *plane(p, 2, row + k - i, slab) = c;
+                    *at(2, k - i) = c;
                     c = through(a[i], c, b[i]);
                 }
         }
-        if (p.dstate && warp == 0) store2(p.dstate + state_at, p.vec, nch, c);
+        if (p.dstate && run == 0) store2(p.dstate + state_at, p.vec, nch, c);
     }
 }
 
@@ -708,45 +759,41 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) Exchange<1> ex;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slab = blockIdx.x % p.slabs;
-    int seq = blockIdx.x / p.slabs;
-    Place q;
-    long long row = 0, tile = 0;
-    if constexpr (CHUNK) {
-        row = blockIdx.x / p.slabs;
-        if (!tile_of_row<kFwdLog2>(p, row, seq, q, tile)) {
-            previous_done();
-            return;
-        }
-    } else {
-        if (seq >= p.n) {
-            clear_rows<T>(p, (T *)p.h, slab);
-            return;
-        }
-        q = sequence(p, seq);
+    Cursor<kFwdLog2, CHUNK, false> now;
+    if (!CHUNK && (int)(blockIdx.x / p.slabs) >= p.n) {
+        clear_rows<T>(p, (T *)p.h, slab);
+        return;
     }
-    From from(p, q, seq, slab, dynamic + warp * From::kBytes);
+    bool more_to_come = now.start(p, blockIdx.x / p.slabs);
+    From from(p, slab, dynamic + warp * From::kBytes);
     const int ch = from.ch, nch = from.nch;
     const bool vec = p.vec;
-    const long long state_at = (long long)seq * p.width + ch;
-    long long t0 = (tile << kFwdLog2) + warp * S;
-    auto rows_at = [&](long long t) { return (int)min((long long)S, max(0LL, q.len - t)); };
-    from.ask_for(t0, rows_at(t0));
+    auto rows_at = [&](long long t) { return (int)min((long long)S, max(0LL, now.q.len - t)); };
+    auto ask_now = [&] {
+        from.turn_to(now.seq, now.q);
+        from.ask_for((now.tile << kFwdLog2) + warp * S, rows_at((now.tile << kFwdLog2) + warp * S));
+    };
+    if (more_to_come) ask_now();
     float2 carry = two(0.0f);
     if constexpr (CHUNK) {
         previous_done();
-        carry = *plane(p, 1, row, slab);
     } else {
+        const long long state_at = (long long)now.seq * p.width + ch;
         if (p.state) carry = load2(p.state + state_at, vec, nch);
-        if (q.len == 0 && p.last && warp == 0) store2(p.last + state_at, vec, nch, carry);
+        if (!more_to_come && p.last && warp == 0) store2(p.last + state_at, vec, nch, carry);
     }
-    for (int par = 0; t0 - warp * S < q.len; t0 += kFwdTile, par ^= 1) {
+    for (int par = 0; more_to_come; par ^= 1) {
+        const long long t0 = (now.tile << kFwdLog2) + warp * S, len = now.q.len, first = now.q.first, state_at = (long long)now.seq * p.width + ch;
         const int cnt = rows_at(t0);
+        if constexpr (CHUNK) carry = *plane(p, 1, now.row, slab);
         float2 a[S], b[S], none[1];
         from.take_from(t0, cnt, a, b, none);
-        if (!CHUNK) from.ask_for(t0 + kFwdTile, rows_at(t0 + kFwdTile));
+        const long long bound_at = !CHUNK && p.bounds ? tile_row<kBwdLog2>(p, now.seq, now.q, t0 >> kBwdLog2) * p.width + ch : 0;
+        more_to_come = now.next(p);
+        if (more_to_come) ask_now();
         if constexpr (KEEP) {
             const PackTo to = {p.pack_gate, p.pack_value, p.pack_gate_scales, p.pack_value_scales};
-            pack_rows(a, b, to, q.first + t0, p.width, ch, vec && from.left >= kSlab && cnt == S, cnt, nch);
+            pack_rows(a, b, to, first + t0, p.width, ch, vec && from.left >= kSlab && cnt == S, cnt, nch);
         }
         const bool special = farthest(a) >= kFar;
         float2 A = two(1.0f), H = two(0.0f);
@@ -789,8 +836,8 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
         }
         // a backward tile is a multiple of a thread's steps: boundaries lie at the start of a thread's steps
         if (!CHUNK && p.bounds && cnt > 0 && t0 > 0 && (t0 & (kBwdTile - 1)) == 0)
-            store2(p.bounds + tile_row<kBwdLog2>(p, seq, q, t0 >> kBwdLog2) * p.width + ch, vec, nch, h);
-        T *out = (T *)p.h + (q.first + t0) * p.width + ch;
+            store2(p.bounds + bound_at, vec, nch, h);
+        T *out = (T *)p.h + (first + t0) * p.width + ch;
         if (!special) {
 #pragma unroll
             for (int s = 0; s < S; ++s) a[s] = h = fma2(a[s], h, b[s]);
@@ -806,8 +853,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
             for (int s = 0; s < S; ++s)
                 if (s < cnt) store2(out + (long long)s * p.width, vec, nch, a[s]);
         }
-        if (p.last && cnt > 0 && t0 + cnt == q.len) store2(p.last + state_at, vec, nch, h);
-        if (CHUNK) break;
+        if (p.last && cnt > 0 && t0 + cnt == len) store2(p.last + state_at, vec, nch, h);
     }
 }
 
@@ -820,51 +866,44 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) Exchange<2> ex;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, slab = blockIdx.x % p.slabs;
-    int seq = blockIdx.x / p.slabs;
-    Place q;
-    long long row = 0, tile = 0;
-    if constexpr (CHUNK) {
-        row = blockIdx.x / p.slabs;
-        if (!tile_of_row<kBwdLog2>(p, row, seq, q, tile)) {
-            previous_done();
-            return;
-        }
-    } else {
-        if (seq >= p.n) {
-            clear_rows<T>(p, (T *)p.dgate, slab);
-            clear_rows<T>(p, (T *)p.dvalue, slab);
-            return;
-        }
-        q = sequence(p, seq);
-        tile = ((q.len + kBwdTile - 1) >> kBwdLog2) - 1;
+    Cursor<kBwdLog2, CHUNK, true> now;
+    if (!CHUNK && (int)(blockIdx.x / p.slabs) >= p.n) {
+        clear_rows<T>(p, (T *)p.dgate, slab);
+        clear_rows<T>(p, (T *)p.dvalue, slab);
+        return;
     }
-    From from(p, q, seq, slab, dynamic + warp * From::kBytes);
+    bool more_to_come = now.start(p, blockIdx.x / p.slabs);
+    From from(p, slab, dynamic + warp * From::kBytes);
     const int ch = from.ch, nch = from.nch;
     const bool vec = p.vec;
-    const long long state_at = (long long)seq * p.width + ch;
-    auto rows_at = [&](long long t) { return (int)min((long long)S, max(0LL, q.len - t)); };
-    if (tile >= 0) from.ask_for((tile << kBwdLog2) + warp * S, rows_at((tile << kBwdLog2) + warp * S));
+    auto rows_at = [&](long long t) { return (int)min((long long)S, max(0LL, now.q.len - t)); };
+    auto ask_now = [&] {
+        from.turn_to(now.seq, now.q);
+        from.ask_for((now.tile << kBwdLog2) + warp * S, rows_at((now.tile << kBwdLog2) + warp * S));
+    };
+    if (more_to_come) ask_now();
     float2 carry = two(0.0f);  // gradient of the state behind the steps in hand
     if constexpr (CHUNK) {
         previous_done();
-        carry = *plane(p, 2, row, slab);
     } else if (p.glast) {
-        carry = load2(p.glast + state_at, vec, nch);
+        carry = load2(p.glast + (long long)now.seq * p.width + ch, vec, nch);
     }
-    for (int par = 0; tile >= 0; --tile, par ^= 1) {
-        const long long t0 = (tile << kBwdLog2) + warp * S;
+    for (int par = 0; more_to_come; par ^= 1) {
+        const long long t0 = (now.tile << kBwdLog2) + warp * S, at = (now.q.first + t0) * p.width + ch;
         const int cnt = rows_at(t0);
         float2 a[S], n[S], u[S], g[S], h = two(0.0f);
-        from.take_from(t0, cnt, a, u, g);
-        if (!CHUNK && tile > 0) from.ask_for(t0 - kBwdTile, S);
         if constexpr (CHUNK) {
-            h = *plane(p, 1, row, slab);
+            h = *plane(p, 1, now.row, slab);
+            carry = *plane(p, 2, now.row, slab);
         } else {
-            if (tile > 0)
-                h = load2(p.bounds + tile_row<kBwdLog2>(p, seq, q, tile) * p.width + ch, vec, nch);
+            if (now.tile > 0)
+                h = load2(p.bounds + tile_row<kBwdLog2>(p, now.seq, now.q, now.tile) * p.width + ch, vec, nch);
             else if (p.state)
-                h = load2(p.state + state_at, vec, nch);
+                h = load2(p.state + (long long)now.seq * p.width + ch, vec, nch);
         }
+        from.take_from(t0, cnt, a, u, g);
+        more_to_come = now.next(p);
+        if (more_to_come) ask_now();
         float2 A = two(1.0f), H = two(0.0f), C = two(0.0f);
         const bool special = farthest(a) >= kFar;
         if (!special) {
@@ -938,7 +977,6 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
                 c = looked_at(a[s], mul2(a[s], dh));
             }
         }
-        const long long at = (q.first + t0) * p.width + ch;
         T *dz = (T *)p.dgate + at, *du = (T *)p.dvalue + at;
         if (vec && nch == 2 && cnt == S) {
 #pragma unroll
@@ -954,9 +992,8 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
                     store2(du + (long long)s * p.width, vec, nch, g[s]);
                 }
         }
-        if (CHUNK) return;
     }
-    if (p.dstate && warp == 0) store2(p.dstate + state_at, vec, nch, carry);
+    if (!CHUNK && p.dstate && warp == 0) store2(p.dstate + (long long)now.seq * p.width + ch, vec, nch, carry);
 }
 
 // ------------------------------------------------------------------ one step
@@ -999,17 +1036,21 @@ static int scan_check(const ScanDims &d)
     if (!d.ragged && d.total != d.n * d.steps) return GN_ERR_BAD_SHAPE;
     if (d.dtype < GN_F32 || d.dtype > GN_F16) return GN_ERR_UNSUPPORTED;
     if (d.total > (1LL << 48) / d.width) return GN_ERR_TOO_LARGE;
-    if ((d.n + 1LL) * slabs_of(d.width) > 0x7fffffffLL || d.tile_rows(kBwdLog2) > 0x7fffffffLL / slabs_of(d.width)) return GN_ERR_TOO_LARGE;
+    if ((d.n + 1LL) * slabs_of(d.width) > 0x7fffffffLL / 4 || d.tile_rows(kBwdLog2) > 0x7fffffffLL / slabs_of(d.width)) return GN_ERR_TOO_LARGE;
     return GN_OK;
 }
 
-// Whether the forward pass (backward: the backward pass) walks or goes by chunks
+// Whether the forward pass (backward: the backward pass) walks or goes by chunks. A walk's tile takes 1.2 to 1.4 us however few CTAs there
+// are, chunks cost two more kernels (10 us) and a second reading. us, walk / chunks, forward and backward: 64 CTAs, 8 x 1024 x 512 float32
+// 21.5 / 17.5 and 45 / 31, 4 x 4097 x 1024 90 / 61 and 203 / 108; 256 CTAs, 16 x 1024 x 1000 float32 44 / 62 and 78 / 118, 16 x 512 x 1024
+// bfloat16 13 / 24 and 25 / 41; 16 CTAs, 1 x 300 x 1024 float32 14 / 18 and 17 / 15. So: a CTA per SM, or few tiles one after the other.
 static bool scan_walks(const ScanDims &d, bool backward, bool packed)
 {
     const int log2 = backward ? kBwdLog2 : kFwdLog2;
-    if (d.n == 0 || (d.ragged ? d.total : d.steps) <= 1LL << log2) return true;  // nothing, or a single tile
+    const long long longest = d.ragged ? d.total : d.steps;
+    if (d.n == 0 || longest <= 1LL << log2) return true;  // nothing, or a single tile
     if (backward && packed) return false;
-    return d.n * slabs_of(d.width) >= 3 * sm_count();
+    return longest <= 8LL << log2 || d.n * slabs_of(d.width) >= sm_count();
 }
 
 static size_t bounds_bytes(const ScanDims &d)
@@ -1044,9 +1085,18 @@ static int launch_chunks(Scan &p, const ScanDims &d, void (*work)(const Scan), s
     if (rc == GN_OK) rc = prepare_kernel((const void *)work, work_smem, what);
     if (rc != GN_OK) return rc;
     const long long warps = p.map_rows * p.slabs;
+    // More than one tile to a CTA, the next asked for while one is worked on, where six rounds of CTAs are left (four fit an SM): 2 x 20000 x
+    // 2048 bfloat16 backward 335 -> 291 us; with fewer rounds the last one costs more (4 x 4097 x 1024 float32 forward 61 -> 67 us)
+    p.tiles_per_cta = 1;
+    while (p.tiles_per_cta < 8 && warps / (2 * p.tiles_per_cta) >= 24LL * sm_count()) p.tiles_per_cta *= 2;
+    const long long ctas = (p.map_rows + p.tiles_per_cta - 1) / p.tiles_per_cta * p.slabs;
     scan_maps_k<T, PACKED, BACKWARD><<<(unsigned)((warps + kScanWarps - 1) / kScanWarps), kScanThreads, smem, st>>>(p);
-    launch_after(scan_starts_k<T, BACKWARD>, dim3((unsigned)((p.n + (d.ragged ? 1LL : 0LL)) * p.slabs)), dim3(32 * kStartWarps), 0, st, p);
-    launch_after(work, dim3((unsigned)warps), dim3(kScanThreads), work_smem, st, p);
+    // eight tiles to a run (they are read together), 64 runs at most and four at least, a warp; ragged: for twice the mean sequence
+    const long long tiles = d.ragged ? 2 * (d.total >> kLog2) / (p.n > 0 ? p.n : 1) : d.tiles(kLog2);
+    int runs = 4;
+    while (runs < kStartRuns && 8 * runs < tiles) runs *= 2;
+    launch_after(scan_starts_k<T, BACKWARD>, dim3((unsigned)((p.n + (d.ragged ? 1LL : 0LL)) * p.slabs * (kSlab / 16))), dim3(8 * runs), 0, st, p);
+    launch_after(work, dim3((unsigned)ctas), dim3(kScanThreads), work_smem, st, p);
     return check_launch(what);
 }
 
