@@ -507,6 +507,7 @@ template <typename T, bool PACKED, bool GRAD, int S>
 struct Source {
     using V = std::conditional_t<PACKED, unsigned char, T>;
     static constexpr size_t kBytes = sizeof(Rows<V, S>) * 2 + (GRAD ? sizeof(Rows<T, S>) : 0);  // shared memory of a warp
+    static_assert(kScanWarps * kBytes + 8192 <= 48 * 1024, "what a kernel may have without being asked for, with an Exchange");
     const Scan &p;
     const int slab, ch, nch, left;
     const long long gate_step, value_step;
@@ -1064,26 +1065,13 @@ static size_t maps_bytes(const ScanDims &d, bool backward, bool packed)
     return sizeof(float) * (backward ? 3 : 2) * (size_t)d.tile_rows(backward ? kBwdLog2 : kFwdLog2) * slabs_of(d.width) * kSlab;
 }
 
-static int prepare_kernel(const void *kern, size_t smem, const char *what)
-{
-    if (smem == 0) return GN_OK;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) return GN_OK;
-    record_cuda_error(e, what);
-    (void)cudaGetLastError();
-    return GN_ERR_CUDA;
-}
-
 // the three kernels of the way by chunks
-template <typename T, bool PACKED, bool BACKWARD>
-static int launch_chunks(Scan &p, const ScanDims &d, void (*work)(const Scan), size_t work_smem, const char *what, cudaStream_t st)
+template <typename T, bool PACKED, bool BACKWARD, void (*WORK)(const Scan)>
+static int launch_chunks(Scan &p, const ScanDims &d, size_t work_smem, const char *what, cudaStream_t st)
 {
     constexpr int kLog2 = BACKWARD ? kBwdLog2 : kFwdLog2;
     p.map_rows = d.tile_rows(kLog2);
     const size_t smem = p.wide ? kScanWarps * Source<T, PACKED, BACKWARD, kSumSteps>::kBytes : 0;
-    int rc = prepare_kernel((const void *)scan_maps_k<T, PACKED, BACKWARD>, smem, what);
-    if (rc == GN_OK) rc = prepare_kernel((const void *)work, work_smem, what);
-    if (rc != GN_OK) return rc;
     const long long warps = p.map_rows * p.slabs;
     // More than one tile to a CTA, the next asked for while one is worked on, where six rounds of CTAs are left (four fit an SM): 2 x 20000 x
     // 2048 bfloat16 backward 335 -> 291 us; with fewer rounds the last one costs more (4 x 4097 x 1024 float32 forward 61 -> 67 us)
@@ -1096,33 +1084,36 @@ static int launch_chunks(Scan &p, const ScanDims &d, void (*work)(const Scan), s
     int runs = 4;
     while (runs < kStartRuns && 8 * runs < tiles) runs *= 2;
     launch_after(scan_starts_k<T, BACKWARD>, dim3((unsigned)((p.n + (d.ragged ? 1LL : 0LL)) * p.slabs * (kSlab / 16))), dim3(8 * runs), 0, st, p);
-    launch_after(work, dim3((unsigned)ctas), dim3(kScanThreads), work_smem, st, p);
+    launch_after(WORK, dim3((unsigned)ctas), dim3(kScanThreads), work_smem, st, p);
     return check_launch(what);
 }
 
+template <void (*KERN)(const Scan)>
+static int launch_walk(const Scan &p, const ScanDims &d, size_t smem, const char *what, cudaStream_t st)
+{
+    KERN<<<(unsigned)((p.n + (d.ragged ? 1LL : 0LL)) * p.slabs), kScanThreads, smem, st>>>(p);
+    return check_launch(what);
+}
+
+template <typename T, bool KEEP>
+static int launch_forward(Scan &p, const ScanDims &d, cudaStream_t st)
+{
+    const size_t smem = p.wide ? kScanWarps * Source<T, false, false, kFwdSteps>::kBytes : 0;
+    if (scan_walks(d, false, false)) return launch_walk<scan_forward_k<T, KEEP, false>>(p, d, smem, "gated_scan", st);
+    return launch_chunks<T, false, false, scan_forward_k<T, KEEP, true>>(p, d, smem, "gated_scan", st);
+}
 template <typename T>
 static int launch_forward(Scan &p, const ScanDims &d, cudaStream_t st)
 {
-    const bool keep = p.pack_gate != nullptr;
-    const size_t smem = p.wide ? kScanWarps * Source<T, false, false, kFwdSteps>::kBytes : 0;
-    if (!scan_walks(d, false, false))
-        return launch_chunks<T, false, false>(p, d, keep ? scan_forward_k<T, true, true> : scan_forward_k<T, false, true>, smem, "gated_scan", st);
-    void (*const kern)(const Scan) = keep ? scan_forward_k<T, true, false> : scan_forward_k<T, false, false>;
-    const int rc = prepare_kernel((const void *)kern, smem, "gated_scan");
-    if (rc != GN_OK) return rc;
-    kern<<<(unsigned)((p.n + (d.ragged ? 1LL : 0LL)) * p.slabs), kScanThreads, smem, st>>>(p);
-    return check_launch("gated_scan");
+    return p.pack_gate ? launch_forward<T, true>(p, d, st) : launch_forward<T, false>(p, d, st);
 }
 
 template <typename T, bool PACKED>
 static int launch_backward(Scan &p, const ScanDims &d, cudaStream_t st)
 {
     const size_t smem = p.wide ? kScanWarps * Source<T, PACKED, true, kBwdSteps>::kBytes : 0;
-    if (!scan_walks(d, true, PACKED)) return launch_chunks<T, PACKED, true>(p, d, scan_backward_k<T, PACKED, true>, smem, "gated_scan backward", st);
-    const int rc = prepare_kernel((const void *)scan_backward_k<T, PACKED, false>, smem, "gated_scan backward");
-    if (rc != GN_OK) return rc;
-    scan_backward_k<T, PACKED, false><<<(unsigned)((p.n + (d.ragged ? 1LL : 0LL)) * p.slabs), kScanThreads, smem, st>>>(p);
-    return check_launch("gated_scan backward");
+    if (scan_walks(d, true, PACKED)) return launch_walk<scan_backward_k<T, PACKED, false>>(p, d, smem, "gated_scan backward", st);
+    return launch_chunks<T, PACKED, true, scan_backward_k<T, PACKED, true>>(p, d, smem, "gated_scan backward", st);
 }
 template <typename T>
 static int launch_backward(Scan &p, const ScanDims &d, bool packed, cudaStream_t st)

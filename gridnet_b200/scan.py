@@ -5,24 +5,27 @@ and value do not depend on the state - frames, read-out planes, tokens - the ste
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from ._lib import GridnetB200Error, check, lib
 from .backend_cuda import _Op
-from .packed import dtype_id, empty_packed, keeps_packed, stream_of
+from .packed import DTYPES, dtype_id, empty_packed, keeps_packed, stream_of
 
 
 def _rows(t: torch.Tensor, lead: int) -> torch.Tensor:
     """``t`` as [..., width] with ``lead`` dimensions in front and the values of a step side by side: a view where there is one."""
-    t = t.reshape(*t.shape[:lead], t.shape[lead:].numel())
+    if t.dim() != lead + 1:
+        t = t.reshape(*t.shape[:lead], t.shape[lead:].numel())
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _strides(t: torch.Tensor):
     """Distances of sequences (0: ragged) and of steps."""
-    return (t.stride(0), t.stride(1)) if t.dim() == 3 else (0, t.stride(0))
+    return t.stride()[:2] if t.dim() == 3 else (0, t.stride(0))
 
 
 def _ptr(t):
@@ -35,6 +38,14 @@ def _nbytes(t) -> int:
 
 def _scratch(nbytes: int, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+@functools.lru_cache(maxsize=512)
+def _sizes(device: int, *size):
+    """Bytes of what a forward pass leaves, and of scratch: forward, backward, backward from packed copies."""
+    with torch.cuda.device(device):
+        work = lib.gn_gated_scan_workspace_bytes
+        return int(lib.gn_gated_scan_bounds_bytes(*size)), int(work(*size, 0, 0)), int(work(*size, 1, 0)), int(work(*size, 1, 1))
 
 
 def _check_scan(gate, value, state, offsets):
@@ -73,57 +84,61 @@ def _device_offsets(offsets, total: int, device):
     return offsets.to(device=device, dtype=torch.int64).contiguous()
 
 
+def _forward(gate, value, state, offsets, kept_packed: bool, need_grad: bool):
+    """(h, last), and what the backward pass needs: the tensors to save and the sizes."""
+    n, steps, total = _check_scan(gate, value, state, offsets)
+    dtype, dev = DTYPES[gate.dtype], gate.device
+    lead = 2 if offsets is None else 1
+    z, u = _rows(gate, lead), _rows(value, lead)
+    width = z.shape[-1]
+    s = None if state is None else state.contiguous()
+    offsets = None if offsets is None else _device_offsets(offsets, total, dev)
+    size = (n, steps, total, width, dtype, lead & 1)
+    left, scratch = _sizes(dev.index, *size)[:2]
+    h = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
+    last = torch.empty((n, *gate.shape[lead:]), dtype=torch.float32, device=dev)
+    codes, bounds = (None, None, None, None), None
+    if need_grad and kept_packed:
+        codes = [t for x in (z, u) for t in empty_packed(x.shape, lead, x.dtype, dev)[:2]]
+    elif need_grad:
+        bounds = _scratch(left, dev)
+    work = _scratch(scratch, dev)
+    with torch.cuda.device(dev):
+        check(lib.gn_gated_scan_forward(z.data_ptr(), u.data_ptr(), _ptr(s), _ptr(offsets), h.data_ptr(), last.data_ptr(), *map(_ptr, codes),
+                                        _ptr(bounds), n, steps, total, width, *_strides(z), *_strides(u), dtype, _ptr(work), scratch,
+                                        stream_of(gate)))
+    if codes[0] is not None:
+        return h, last, (codes[0], codes[2], codes[1], codes[3], s, offsets, None), size
+    return h, last, (z, u, None, None, s, offsets, bounds), size
+
+
 class GatedScanOp(_Op):
     """``GatedScanOp.apply(gate, value, state, offsets, packed)``: :func:`gated_scan` as an autograd op."""
 
     @staticmethod
     def forward(ctx, gate, value, state, offsets, packed: bool):
-        n, steps, total = _check_scan(gate, value, state, offsets)
-        dtype, dev = dtype_id(gate, "gate"), gate.device
-        lead = 2 if offsets is None else 1
+        h, last, kept, ctx.size = _forward(gate, value, state, offsets, packed, any(ctx.needs_input_grad[:3]))
         ctx.set_materialize_grads(False)
-        ctx.shape, ctx.has_state = gate.shape, state is not None
-        z, u = _rows(gate, lead), _rows(value, lead)
-        width = z.shape[-1]
-        s = None if state is None else state.contiguous()
-        offsets = None if offsets is None else _device_offsets(offsets, total, dev)
-        h = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
-        last = torch.empty((n, *gate.shape[lead:]), dtype=torch.float32, device=dev)
-        size = (n, steps, total, width, dtype, int(lead == 1))
-        kept, bounds = [None] * 4, None
-        with torch.cuda.device(dev):
-            if any(ctx.needs_input_grad[:3]):
-                if packed:
-                    kept = [t for x in (z, u) for t in empty_packed(x.shape, lead, x.dtype, dev)[:2]]
-                else:
-                    bounds = _scratch(lib.gn_gated_scan_bounds_bytes(*size), dev)
-            work = _scratch(lib.gn_gated_scan_workspace_bytes(*size, 0, 0), dev)
-            check(lib.gn_gated_scan_forward(z.data_ptr(), u.data_ptr(), _ptr(s), _ptr(offsets), h.data_ptr(), last.data_ptr(), *map(_ptr, kept),
-                                            _ptr(bounds), n, steps, total, width, *_strides(z), *_strides(u), dtype, _ptr(work), _nbytes(work),
-                                            stream_of(gate)))
-        ctx.cfg = (size, gate.dtype)
-        if kept[0] is not None:
-            ctx.save_for_backward(kept[0], kept[2], kept[1], kept[3], s, offsets, None)
-        else:
-            ctx.save_for_backward(z, u, None, None, s, offsets, bounds)
+        ctx.shape, ctx.dtype = gate.shape, gate.dtype
+        ctx.save_for_backward(*kept)
         return h, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_h, grad_last):
         z, u, z_scales, u_scales, s, offsets, bounds = ctx.saved_tensors
-        size, kind = ctx.cfg
-        dev, packed = z.device, z_scales is not None
-        grad_h = torch.zeros(ctx.shape, dtype=kind, device=dev) if grad_h is None else grad_h.contiguous()
+        size, dev, packed = ctx.size, z.device, z_scales is not None
+        grad_h = torch.zeros(ctx.shape, dtype=ctx.dtype, device=dev) if grad_h is None else grad_h.contiguous()
         grad_last = None if grad_last is None else grad_last.contiguous()
-        dz, du = (torch.empty(ctx.shape, dtype=kind, device=dev) for _ in range(2))
-        ds = torch.empty_like(s) if ctx.has_state and ctx.needs_input_grad[2] else None
+        dz, du = torch.empty(ctx.shape, dtype=ctx.dtype, device=dev), torch.empty(ctx.shape, dtype=ctx.dtype, device=dev)
+        ds = torch.empty_like(s) if s is not None and ctx.needs_input_grad[2] else None
         strides = (0, 0, 0, 0) if packed else (*_strides(z), *_strides(u))
+        scratch = _sizes(dev.index, *size)[2 + packed]
+        work = _scratch(scratch, dev)
         with torch.cuda.device(dev):
-            work = _scratch(lib.gn_gated_scan_workspace_bytes(*size, 1, int(packed)), dev)
             check(lib.gn_gated_scan_backward(z.data_ptr(), u.data_ptr(), _ptr(z_scales), _ptr(u_scales), _ptr(s), _ptr(offsets), _ptr(bounds),
                                              grad_h.data_ptr(), _ptr(grad_last), dz.data_ptr(), du.data_ptr(), _ptr(ds), *size[:4], *strides,
-                                             size[4], _ptr(work), _nbytes(work), stream_of(z)))
+                                             size[4], _ptr(work), scratch, stream_of(z)))
         return dz, du, ds, None, None
 
 
@@ -145,34 +160,38 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor | No
     halves of a wider projection are read where they are."""
     if offsets is not None and not isinstance(offsets, torch.Tensor):
         offsets = torch.as_tensor(offsets, dtype=torch.int64)
+    if not (torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or (state is not None and state.requires_grad))):
+        return _forward(gate.detach(), value.detach(), state, offsets, False, False)[:2]
     return GatedScanOp.apply(gate, value, state, offsets, keeps_packed() if packed is None else bool(packed))
 
 
-@torch.no_grad()
 def gated_scan_step(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor, out_state: torch.Tensor | None = None):
     """One step of :func:`gated_scan` without gradients: ``gate`` and ``value`` [batch, ...], ``state`` [batch, ...] float32. Returns
     ``(h, new_state)``; ``out_state`` (which may be ``state``) receives the new state."""
+    gate, value, state = gate.detach(), value.detach(), state.detach()
     for name, t in (("gate", gate), ("value", value), ("state", state)):
         if not t.is_cuda:
             raise GridnetB200Error(f"{name} must be a CUDA tensor")
     dtype = dtype_id(gate, "gate")
-    assert gate.dim() >= 2 and gate.shape == value.shape == state.shape, f"{value.shape=} {state.shape=} invalid for {gate.shape=}"
+    shape, dev = gate.shape, gate.device
+    assert len(shape) >= 2 and shape == value.shape == state.shape, f"{value.shape=} {state.shape=} invalid for {gate.shape=}"
     assert gate.dtype == value.dtype, f"mismatching dtypes: {gate.dtype=} {value.dtype=}"
     assert state.dtype == torch.float32, f"{state.dtype=}: states are float32"
-    assert gate.device == value.device == state.device, f"mismatching devices: {gate.device=} {value.device=} {state.device=}"
-    assert gate.shape[1:].numel() > 0, f"{gate.shape=}: steps of no values"
+    assert dev == value.device == state.device, f"mismatching devices: {gate.device=} {value.device=} {state.device=}"
     z, u, s = _rows(gate, 1), _rows(value, 1), state.contiguous()
+    rows, width = z.shape
+    assert width > 0, f"{gate.shape=}: steps of no values"
     if out_state is None:
         out_state = torch.empty_like(s)
     else:
-        assert out_state.shape == state.shape and out_state.dtype == torch.float32 and out_state.device == state.device, (
+        assert out_state.shape == shape and out_state.dtype == torch.float32 and out_state.device == dev, (
             f"{out_state.shape=} {out_state.dtype=} {out_state.device=} invalid for a state of {state.shape}")
         if not out_state.is_contiguous():
             raise GridnetB200Error("out_state must be contiguous")
-    h = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
-    with torch.cuda.device(gate.device):
-        check(lib.gn_gated_scan_step(z.data_ptr(), u.data_ptr(), s.data_ptr(), h.data_ptr(), out_state.data_ptr(), z.shape[0], z.shape[1],
-                                     z.stride(0), u.stride(0), dtype, stream_of(gate)))
+    h = torch.empty(shape, dtype=gate.dtype, device=dev)
+    with torch.cuda.device(dev):
+        check(lib.gn_gated_scan_step(z.data_ptr(), u.data_ptr(), s.data_ptr(), h.data_ptr(), out_state.data_ptr(), rows, width, z.stride(0),
+                                     u.stride(0), dtype, stream_of(gate)))
     return h, out_state
 
 
