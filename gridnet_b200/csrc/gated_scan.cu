@@ -164,18 +164,25 @@ __device__ __forceinline__ void gates(float2 z, float2 &a, float2 &n)
     const float2 p = fma2(n, two(-1.0f), one);
     a = make_float2(z.x < 0.0f ? r.x : p.x, z.y < 0.0f ? r.y : p.y);
 }
-// For every z: the smaller from exp(-|z|), which is 0 from |z| = 104 on, the larger as 1 less it
-__device__ __forceinline__ float2 gate_any(float z)  // (s(z), s(-z))
-{
-    const float e = expf(-fabsf(z));
-    const float q = e / (1.0f + e), p = 1.0f - q;
-    return z < 0.0f ? make_float2(q, p) : make_float2(p, q);
-}
+// For every z. From kFar on 1 + e is 1 and the smaller of the two is e itself, 0 from |z| = 104 on
 __device__ __forceinline__ void gates_any(float2 z, float2 &a, float2 &n)
 {
-    const float2 x = gate_any(z.x), y = gate_any(z.y);
-    a = make_float2(x.x, y.x);
-    n = make_float2(x.y, y.y);
+    const float dx = fabsf(z.x), dy = fabsf(z.y);
+    const bool fx = !(dx < kFar), fy = !(dy < kFar);
+    gates(make_float2(fx ? 0.0f : z.x, fy ? 0.0f : z.y), a, n);
+    float ex, ey;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(ex) : "f"(-1.4426950408889634f * dx));
+    asm("ex2.approx.f32 %0, %1;" : "=f"(ey) : "f"(-1.4426950408889634f * dy));
+    if (fx) {
+        const float one = dx == dx ? 1.0f : dx;  // NaN: both
+        a.x = z.x < 0.0f ? ex : one;
+        n.x = z.x < 0.0f ? one : ex;
+    }
+    if (fy) {
+        const float one = dy == dy ? 1.0f : dy;
+        a.y = z.y < 0.0f ? ey : one;
+        n.y = z.y < 0.0f ? one : ey;
+    }
 }
 
 // ---- maps of runs. The sign bit of A: the run has a reset, what was before it does not show
@@ -1045,13 +1052,15 @@ static int scan_check(const ScanDims &d)
 // are, chunks cost two more kernels (10 us) and a second reading. us, walk / chunks, forward and backward: 64 CTAs, 8 x 1024 x 512 float32
 // 21.5 / 17.5 and 45 / 31, 4 x 4097 x 1024 90 / 61 and 203 / 108; 256 CTAs, 16 x 1024 x 1000 float32 44 / 62 and 78 / 118, 16 x 512 x 1024
 // bfloat16 13 / 24 and 25 / 41; 16 CTAs, 1 x 300 x 1024 float32 14 / 18 and 17 / 15. So: a CTA per SM, or few tiles one after the other.
+// How long the longest of ragged sequences is is not known here: eight rounds of CTAs, so that one of eight times the mean takes no longer
+// than all (37 of mean 300, the longest 2380, x 1000 bfloat16: a walk takes 118 and 183 us, chunks 50 and 75).
 static bool scan_walks(const ScanDims &d, bool backward, bool packed)
 {
     const int log2 = backward ? kBwdLog2 : kFwdLog2;
     const long long longest = d.ragged ? d.total : d.steps;
     if (d.n == 0 || longest <= 1LL << log2) return true;  // nothing, or a single tile
     if (backward && packed) return false;
-    return longest <= 8LL << log2 || d.n * slabs_of(d.width) >= sm_count();
+    return longest <= 8LL << log2 || d.n * slabs_of(d.width) >= (d.ragged ? 32LL : 1LL) * sm_count();
 }
 
 static size_t bounds_bytes(const ScanDims &d)

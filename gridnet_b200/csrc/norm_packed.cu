@@ -4,39 +4,43 @@
 //     with p = (x~ - m) r from the packed copy x~ and q = gamma g:
 //     gx = r (q - mean(q) - p mean(q p)),  ggamma = sum over the batch of g p,  gbeta = sum over the batch of g
 //
-// HBM-bound: forward 4 + 4 bytes for a value (and 4 more where a sample's second reading does not hit L2) and 1.03 for its packed
+// HBM-bound: forward 8 bytes for a value (and 4 more where its second reading does not hit L2) and 1.03 for its packed
 // copy, backward 5.03 twice and 4. Sums are in double, in a fixed order.
 #include "kernels.h"
 #include "packed8.cuh"
 
 namespace gn {
 
-// y and the packed copy, eight lanes a group
-__global__ void __launch_bounds__(256) norm_apply_pack_k(const float *__restrict__ x, const float *__restrict__ gamma,
-                                                         const float *__restrict__ beta, const float2 *__restrict__ stats, float *__restrict__ y,
-                                                         unsigned char *__restrict__ codes, unsigned char *__restrict__ scales, long long groups,
-                                                         long long per_row, long long P, int vec)
+// y and the packed copy. A thread has four positions of four samples, with gamma and beta read once for them; eight lanes have a group. Later
+// samples first: of them, what the sums were taken from is still in L2.
+constexpr int kTogether = 4;
+__global__ void __launch_bounds__(256) norm_apply_pack_k(const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta,
+                                                         const float2 *stats, float *__restrict__ y, unsigned char *__restrict__ codes,
+                                                         unsigned char *__restrict__ scales, int B, int slices, long long per_row, long long P, int vec)
 {
-    const int lane8 = threadIdx.x & 7;
-    const long long stride = (long long)gridDim.x * 32;
-    for (long long g0 = (long long)blockIdx.x * 32 + (threadIdx.x >> 5) * 4; g0 < groups; g0 += stride) {
-        const long long g = g0 + ((threadIdx.x & 31) >> 3);
-        const long long row = g / per_row, col = (g - row * per_row) * kPackGroup + lane8 * 4;
-        const int n = g < groups ? (int)min(4LL, max(0LL, P - col)) : 0;
-        const long long at = row * P + col;
-        float v[4], ga[4], be[4];
-        load4(x + at, vec, n, v);
-        load4(gamma + col, vec, n, ga);
-        load4(beta + col, vec, n, be);
-        unsigned scale;
-        const unsigned w = pack_group(v, scale);
-        store_codes(codes + at, vec, n, w);
-        if (lane8 == 0 && g < groups) scales[g] = (unsigned char)scale;
-        if (n > 0) {
-            const float2 mr = stats[row];
+    const int chunk = blockIdx.x / slices, last = B - 1 - chunk * kTogether;
+    const long long col = ((long long)(blockIdx.x - chunk * slices) * 256 + threadIdx.x) * 4;
+    const int n = (int)min(4LL, max(0LL, P - col));
+    float v[kTogether][4], ga[4], be[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = fmaf((v[i] - mr.x) * mr.y, ga[i], be[i]);
-            store4(y + at, vec, n, v);
+    for (int i = 0; i < kTogether; ++i) load4(x + (long long)max(last - i, 0) * P + col, vec, n, v[i]);
+    load4(gamma + col, vec, n, ga);
+    load4(beta + col, vec, n, be);
+    previous_done();
+#pragma unroll
+    for (int i = 0; i < kTogether; ++i) {
+        const int b = last - i;
+        if (b < 0) return;
+        unsigned scale;
+        const unsigned w = pack_group(v[i], scale);
+        if (n > 0) {
+            const long long at = b * P + col;
+            store_codes(codes + at, vec, n, w);
+            if ((threadIdx.x & 7) == 0) scales[b * per_row + col / kPackGroup] = (unsigned char)scale;
+            const float2 mr = stats[b];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[i][k] = fmaf((v[i][k] - mr.x) * mr.y, ga[k], be[k]);
+            store4(y + at, vec, n, v[i]);
         }
     }
 }
@@ -52,23 +56,45 @@ __global__ void __launch_bounds__(256) norm_packed_sums_k(const unsigned char *_
     const float2 mr = stats[b];
     const long long lo = part * slice, hi = min(P, lo + slice);
     double sq = 0.0, sp = 0.0;
-    for (long long col = lo + 4 * threadIdx.x; col < hi; col += 4 * 256) {
-        const int n = (int)min(4LL, hi - col);
-        const long long at = b * P + col;
-        float v[4], g[4], ga[4];
-        load4(gy + at, vec, n, g);
-        load4(gamma + col, vec, n, ga);
-        unpack4(load_codes(codes + at, vec, n), pack_step(scales[b * per_row + col / kPackGroup]), v);
-        float q = 0.0f, p = 0.0f;
+    const float *const gs = gy + b * P;
+    const unsigned char *const cs = codes + b * P, *const ss = scales + b * per_row;
+    auto add = [&](const float (&g)[4], const float (&ga)[4], unsigned w, unsigned scale, int n) {
+        float v[4], q = 0.0f, p = 0.0f;
+        unpack4(w, pack_step(scale), v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < n) {
-                const float t = g[i] * ga[i];
+        for (int k = 0; k < 4; ++k)
+            if (k < n) {
+                const float t = g[k] * ga[k];
                 q += t;
-                p = fmaf(t, (v[i] - mr.x) * mr.y, p);
+                p = fmaf(t, (v[k] - mr.x) * mr.y, p);
             }
         sq += (double)q;
         sp += (double)p;
+    };
+    long long col = lo + 4 * threadIdx.x;
+    constexpr int kStride = 4 * 256;
+    if (vec) {
+        constexpr int kAtOnce = 4;
+        for (; col + (kAtOnce - 1) * kStride < hi; col += kAtOnce * kStride) {  // loads first
+            float g[kAtOnce][4], ga[kAtOnce][4];
+            unsigned w[kAtOnce], sc[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                load4v(gs + col + i * kStride, g[i]);
+                load4v(gamma + col + i * kStride, ga[i]);
+                w[i] = *reinterpret_cast<const unsigned *>(cs + col + i * kStride);
+                sc[i] = ss[(col + i * kStride) / kPackGroup];
+            }
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) add(g[i], ga[i], w[i], sc[i], 4);
+        }
+    }
+    for (; col < hi; col += kStride) {
+        const int n = (int)min(4LL, hi - col);
+        float g[4], ga[4];
+        load4(gs + col, vec, n, g);
+        load4(gamma + col, vec, n, ga);
+        add(g, ga, load_codes(cs + col, vec, n), ss[col / kPackGroup], n);
     }
     sq = block_sum(sq, red);
     sp = block_sum(sp, red);
@@ -76,9 +102,10 @@ __global__ void __launch_bounds__(256) norm_packed_sums_k(const unsigned char *_
 }
 
 // one CTA per sample: means of q and q p
-__global__ void __launch_bounds__(64) norm_packed_means_k(const double2 *__restrict__ partials, int parts, float2 *__restrict__ ac, long long P)
+__global__ void __launch_bounds__(64) norm_packed_means_k(const double2 *partials, int parts, float2 *__restrict__ ac, long long P)
 {
     __shared__ double red[33];
+    previous_done();
     double q = 0.0, p = 0.0;
     for (int i = threadIdx.x; i < parts; i += blockDim.x) {
         q += partials[(size_t)blockIdx.x * parts + i].x;
@@ -89,35 +116,69 @@ __global__ void __launch_bounds__(64) norm_packed_means_k(const double2 *__restr
     if (threadIdx.x == 0) ac[blockIdx.x] = make_float2((float)(q / (double)P), (float)(p / (double)P));
 }
 
-// a thread has four positions and walks the batch
+// A thread has four positions and every PARTS-th sample, 256 / PARTS threads side by side; the parts' sums are added up in a fixed order. Four
+// samples' loads ahead of the rest. One part where that leaves CTAs enough (rows of 4 KB: 128^3 x 32 127 us, with eight parts 146), else
+// eight (40 x 56 x 72 x 37 37 -> 19 us, 32^3 x 8 10.6 -> 4.5).
+template <int PARTS>
 __global__ void __launch_bounds__(256) norm_packed_apply_k(const unsigned char *__restrict__ codes, const unsigned char *__restrict__ scales,
-                                                           const float2 *__restrict__ stats, const float2 *__restrict__ ac,
-                                                           const float *__restrict__ gamma, const float *__restrict__ gy, float *__restrict__ gx,
-                                                           float *__restrict__ ggamma, float *__restrict__ gbeta, int B, long long P,
-                                                           long long per_row, int vec)
+                                                           const float2 *stats, const float2 *ac, const float *__restrict__ gamma,
+                                                           const float *__restrict__ gy, float *__restrict__ gx, float *__restrict__ ggamma,
+                                                           float *__restrict__ gbeta, int B, long long P, long long per_row, int vec)
 {
-    const long long col = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (col >= P) return;
-    const int n = (int)min(4LL, P - col);
+    constexpr int kSide = 256 / PARTS;
+    __shared__ float4 sums[2][PARTS][PARTS > 1 ? kSide : 1];
+    const int place = threadIdx.x % kSide, part = threadIdx.x / kSide;
+    const long long col = ((long long)blockIdx.x * kSide + place) * 4;
+    const int n = (int)min(4LL, max(0LL, P - col));
     float ga[4], sg[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sb[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     load4(gamma + col, vec, n, ga);
-    for (int b = 0; b < B; ++b) {
-        const long long at = b * P + col;
-        const float2 mr = stats[b], m = ac[b];
-        float v[4], g[4];
-        load4(gy + at, vec, n, g);
-        unpack4(load_codes(codes + at, vec, n), pack_step(scales[b * per_row + col / kPackGroup]), v);
+    previous_done();
+    if (n > 0) {
+        for (int b0 = part; b0 < B; b0 += PARTS * kTogether) {
+            float g[kTogether][4];
+            unsigned w[kTogether], sc[kTogether];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float p = (v[i] - mr.x) * mr.y;
-            sg[i] = fmaf(g[i], p, sg[i]);
-            sb[i] += g[i];
-            v[i] = mr.y * (fmaf(-p, m.y, g[i] * ga[i]) - m.x);
+            for (int i = 0; i < kTogether; ++i) {
+                const int b = min(b0 + PARTS * i, B - 1);
+                const long long at = b * P + col;
+                load4(gy + at, vec, n, g[i]);
+                w[i] = load_codes(codes + at, vec, n);
+                sc[i] = scales[b * per_row + col / kPackGroup];
+            }
+#pragma unroll
+            for (int i = 0; i < kTogether; ++i) {
+                const int b = b0 + PARTS * i;
+                if (b >= B) break;
+                const float2 mr = stats[b], m = ac[b];
+                float v[4];
+                unpack4(w[i], pack_step(sc[i]), v);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float p = (v[k] - mr.x) * mr.y;
+                    sg[k] = fmaf(g[i][k], p, sg[k]);
+                    sb[k] += g[i][k];
+                    v[k] = mr.y * (fmaf(-p, m.y, g[i][k] * ga[k]) - m.x);
+                }
+                store4(gx + b * P + col, vec, n, v);
+            }
         }
-        store4(gx + at, vec, n, v);
     }
-    store4(ggamma + col, vec, n, sg);
-    store4(gbeta + col, vec, n, sb);
+    if constexpr (PARTS > 1) {
+        sums[0][part][place] = make_float4(sg[0], sg[1], sg[2], sg[3]);
+        sums[1][part][place] = make_float4(sb[0], sb[1], sb[2], sb[3]);
+        __syncthreads();
+        if (part < 2) {
+            float t[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < PARTS; ++i) {
+                const float4 s = sums[part][i][place];
+                t[0] += s.x; t[1] += s.y; t[2] += s.z; t[3] += s.w;
+            }
+            store4((part ? gbeta : ggamma) + col, vec, n, t);
+        }
+    } else {
+        store4(ggamma + col, vec, n, sg);
+        store4(gbeta + col, vec, n, sb);
+    }
 }
 
 static bool aligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -138,7 +199,7 @@ static PackedNormWs carve_packed_norm(void *base, int B)
 }
 static int packed_norm_check(int B, long long P, const void *workspace, size_t bytes)
 {
-    if (B < 0 || P <= 0 || P > (1LL << 40) || (long long)B * ((P + 1023) / 1024) > 0x7fffffffLL) return GN_ERR_BAD_SHAPE;
+    if (B < 0 || P <= 0 || P > (1LL << 37) || (long long)B * ((P + 1023) / 1024) > 0x7fffffffLL) return GN_ERR_BAD_SHAPE;
     if (B > 0 && (!workspace || !aligned(workspace, 16) || bytes < carve_packed_norm(nullptr, B).bytes)) return GN_ERR_WORKSPACE;
     return GN_OK;
 }
@@ -170,10 +231,10 @@ GN_API int gn_norm_forward_packed_f32(const float *x, const float *gamma, const 
     rc = launch_norm_partial_stats(x, ws.partials, B, P, parts, st);
     if (rc == GN_OK) rc = launch_norm_finalize(ws.partials, parts, stats, B, P, eps, st);
     if (rc != GN_OK) return rc;
-    const long long per_row = (P + kPackGroup - 1) / kPackGroup, groups = B * per_row, want = (groups + 31) / 32, most = 16LL * sm_count();
+    const long long per_row = (P + kPackGroup - 1) / kPackGroup, slices = (P + 1023) / 1024;
     const int vec = P % 4 == 0 && aligned(x, 16) && aligned(gamma, 16) && aligned(beta, 16) && aligned(y, 16) && aligned(codes, 4);
-    norm_apply_pack_k<<<(unsigned)(want < most ? want : most), 256, 0, st>>>(x, gamma, beta, stats, y, (unsigned char *)codes,
-                                                                             (unsigned char *)scales, groups, per_row, P, vec);
+    launch_after(norm_apply_pack_k, dim3((unsigned)(slices * ((B + kTogether - 1) / kTogether))), dim3(256), 0, st, x, gamma, beta, stats, y,
+                 (unsigned char *)codes, (unsigned char *)scales, B, (int)slices, per_row, P, vec);
     return check_launch("norm_apply_pack");
 }
 
@@ -198,9 +259,14 @@ GN_API int gn_norm_backward_packed_f32(const void *codes, const void *scales, co
         const int parts = norm_pick_parts(P);
         const long long slice = ((P + parts - 1) / parts + kPackGroup - 1) / kPackGroup * kPackGroup;
         norm_packed_sums_k<<<(unsigned)B * parts, 256, 0, st>>>(c, s, stats, gamma, gy, ws.partials, P, slice, per_row, parts, vec);
-        norm_packed_means_k<<<B, 64, 0, st>>>(ws.partials, parts, ws.ac, P);
+        launch_after(norm_packed_means_k, dim3(B), dim3(64), 0, st, ws.partials, parts, ws.ac, P);
     }
-    norm_packed_apply_k<<<(unsigned)((P + 1023) / 1024), 256, 0, st>>>(c, s, stats, ws.ac, gamma, gy, gx, ggamma, gbeta, B, P, per_row, vec);
+    if (P >= 2048LL * sm_count())
+        launch_after(norm_packed_apply_k<1>, dim3((unsigned)((P + 1023) / 1024)), dim3(256), 0, st, c, s, stats, ws.ac, gamma, gy, gx, ggamma, gbeta,
+                     B, P, per_row, vec);
+    else
+        launch_after(norm_packed_apply_k<8>, dim3((unsigned)((P + 127) / 128)), dim3(256), 0, st, c, s, stats, ws.ac, gamma, gy, gx, ggamma, gbeta, B,
+                     P, per_row, vec);
     return check_launch("norm_backward_packed");
 }
 

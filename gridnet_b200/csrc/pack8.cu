@@ -52,6 +52,121 @@ __global__ void __launch_bounds__(256) unpack8_k(const unsigned char *__restrict
     }
 }
 
+// Whole groups one after the other, everything on 16 bytes: a thread has 16 bytes of values four times, all loads ahead of the rest. us for
+// 64 x 64^3 floats (84 MB, 13 at 6.5 TB/s), both directions, against the kernels above: 25.6 -> 14.9 and 20.3 -> 14.7
+template <typename T>
+struct Flat {
+    static constexpr int kPer = 16 / sizeof(T), kLanes = kPackGroup / kPer, kTimes = 4;  // values of a thread, threads of a group
+};
+__device__ __forceinline__ void load16(const float *p, float (&v)[4]) { load4v(p, v); }
+template <typename T>
+__device__ __forceinline__ void load16(const T *p, float (&v)[8])
+{
+    const uint4 q = *reinterpret_cast<const uint4 *>(p);
+    const uint2 h[2] = {{q.x, q.y}, {q.z, q.w}};
+    float a[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        load4v(reinterpret_cast<const T *>(&h[i]), a);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[4 * i + k] = a[k];
+    }
+}
+__device__ __forceinline__ void store16(float *p, const float (&v)[4]) { store4v(p, v); }
+template <typename T>
+__device__ __forceinline__ void store16(T *p, const float (&v)[8])
+{
+    uint4 q;
+    store4v(reinterpret_cast<T *>(&q.x), {v[0], v[1], v[2], v[3]});
+    store4v(reinterpret_cast<T *>(&q.z), {v[4], v[5], v[6], v[7]});
+    *reinterpret_cast<uint4 *>(p) = q;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) pack8_flat_k(const T *__restrict__ x, unsigned char *__restrict__ codes, unsigned char *__restrict__ scales,
+                                                    long long values)
+{
+    using F = Flat<T>;
+    const long long at0 = ((long long)blockIdx.x * F::kTimes * 256 + threadIdx.x) * F::kPer;
+    float v[F::kTimes][F::kPer];
+#pragma unroll
+    for (int i = 0; i < F::kTimes; ++i) load16(x + min(at0 + (long long)i * 256 * F::kPer, values - F::kPer), v[i]);
+#pragma unroll
+    for (int i = 0; i < F::kTimes; ++i) {
+        const long long at = at0 + (long long)i * 256 * F::kPer;
+        const bool there = at < values;  // of a group all threads or none
+        unsigned m = 0;
+#pragma unroll
+        for (int k = 0; k < F::kPer; ++k) m = max(m, magnitude_bits(v[i][k]));
+#pragma unroll
+        for (int o = F::kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const bool rare = __any_sync(0xffffffffu, m > kPackLargest);
+        if (rare) {  // once more over what is finite
+            m = 0;
+#pragma unroll
+            for (int k = 0; k < F::kPer; ++k) {
+                const unsigned b = magnitude_bits(v[i][k]);
+                if (bits_finite(b)) m = max(m, b);
+            }
+#pragma unroll
+            for (int o = F::kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        }
+        const unsigned scale = pack_scale(m);
+        const float inverse = pack_inverse(scale);
+        unsigned w[F::kPer / 4];
+#pragma unroll
+        for (int k = 0; k < F::kPer; k += 4) {
+            if (rare)
+                w[k / 4] = pack_word(pack_code_any(v[i][k], scale), pack_code_any(v[i][k + 1], scale), pack_code_any(v[i][k + 2], scale),
+                                     pack_code_any(v[i][k + 3], scale));
+            else
+                w[k / 4] = pack_word(pack_code(v[i][k], inverse), pack_code(v[i][k + 1], inverse), pack_code(v[i][k + 2], inverse),
+                                     pack_code(v[i][k + 3], inverse));
+        }
+        if (there) {
+            if constexpr (F::kPer == 4)
+                *reinterpret_cast<unsigned *>(codes + at) = w[0];
+            else
+                *reinterpret_cast<uint2 *>(codes + at) = make_uint2(w[0], w[1]);
+            if (threadIdx.x % F::kLanes == 0) scales[at / kPackGroup] = (unsigned char)scale;
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) unpack8_flat_k(const unsigned char *__restrict__ codes, const unsigned char *__restrict__ scales,
+                                                      T *__restrict__ x, long long values)
+{
+    using F = Flat<T>;
+    const long long at0 = ((long long)blockIdx.x * F::kTimes * 256 + threadIdx.x) * F::kPer;
+    unsigned w[F::kTimes][F::kPer / 4], scale[F::kTimes];
+#pragma unroll
+    for (int i = 0; i < F::kTimes; ++i) {
+        const long long at = min(at0 + (long long)i * 256 * F::kPer, values - F::kPer);
+        if constexpr (F::kPer == 4) {
+            w[i][0] = *reinterpret_cast<const unsigned *>(codes + at);
+        } else {
+            const uint2 q = *reinterpret_cast<const uint2 *>(codes + at);
+            w[i][0] = q.x;
+            w[i][1] = q.y;
+        }
+        scale[i] = scales[at / kPackGroup];
+    }
+#pragma unroll
+    for (int i = 0; i < F::kTimes; ++i) {
+        const long long at = at0 + (long long)i * 256 * F::kPer;
+        float v[F::kPer];
+#pragma unroll
+        for (int k = 0; k < F::kPer; k += 4) {
+            float f[4];
+            unpack4(w[i][k / 4], pack_step(scale[i]), f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[k + j] = held_by<T>(f[j]);
+        }
+        if (at < values) store16(x + at, v);
+    }
+}
+
 static unsigned pack_blocks(long long groups)
 {
     const long long want = (groups + 31) / 32, most = 16LL * sm_count();
@@ -62,6 +177,16 @@ template <typename T>
 static int launch_pack8(const void *x, void *codes, void *scales, long long rows, long long cols, bool unpack, cudaStream_t st)
 {
     const long long per_row = (cols + kPackGroup - 1) / kPackGroup, groups = rows * per_row;
+    if (cols % kPackGroup == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(codes) % 8 == 0) {
+        const long long values = rows * cols, of_cta = 256LL * Flat<T>::kTimes * Flat<T>::kPer, blocks = (values + of_cta - 1) / of_cta;
+        if (blocks <= 0x7fffffffLL) {
+            if (unpack)
+                unpack8_flat_k<T><<<(unsigned)blocks, 256, 0, st>>>((const unsigned char *)codes, (const unsigned char *)scales, (T *)x, values);
+            else
+                pack8_flat_k<T><<<(unsigned)blocks, 256, 0, st>>>((const T *)x, (unsigned char *)codes, (unsigned char *)scales, values);
+            return check_launch(unpack ? "unpack8" : "pack8");
+        }
+    }
     const int vec = cols % 4 == 0 && reinterpret_cast<uintptr_t>(x) % (4 * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(codes) % 4 == 0;
     if (unpack)
         unpack8_k<T><<<pack_blocks(groups), 256, 0, st>>>((const unsigned char *)codes, (const unsigned char *)scales, (T *)x, groups, per_row,
