@@ -101,6 +101,12 @@ SIGNATURES = {
     "gn_norm_packed_workspace_bytes": (c_size_t, [c_int, c_longlong]),
     "gn_norm_forward_packed_f32": (c_int, [_P] * 7 + [c_int, c_longlong, c_float, _P, c_size_t, _P]),
     "gn_norm_backward_packed_f32": (c_int, [_P] * 8 + [c_int, c_longlong, _P, c_size_t, _P]),
+    "gn_loop_packed_bytes": (c_size_t, [c_int] * 4),
+    "gn_loop_packed_workspace_bytes": (c_size_t, [c_int] * 10),
+    "gn_loop_forward_packed_f32": (c_int, [_P] * 3 + [c_int] + [_P] * 6 + _geom + [c_int, c_int, c_int, c_float, c_int, c_int, _P, c_size_t, _P]),
+    "gn_loop_backward_packed_f32": (c_int, [_P] * 3 + [c_int] + [_P] * 11 + _geom + [c_int] * 5 + [_P, c_size_t, _P]),
+    "gn_gated_loop_forward_packed_f32": (c_int, [_P] * 8 + _geom + [c_int, c_int, c_float, c_int, _P, c_size_t, _P]),
+    "gn_gated_loop_backward_packed_f32": (c_int, [_P] * 12 + _geom + [c_int] * 3 + [_P, c_size_t, _P]),
     "gn_gated_scan_bounds_bytes": (c_size_t, [c_int, c_longlong, c_longlong, c_int, c_int, c_int]),
     "gn_gated_scan_workspace_bytes": (c_size_t, [c_int, c_longlong, c_longlong] + [c_int] * 5),
     "gn_gated_scan_forward": (c_int, [_P] * 11 + [c_int, c_longlong, c_longlong, c_int] + [c_longlong] * 4 + [c_int, _P, c_size_t, _P]),

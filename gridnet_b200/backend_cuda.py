@@ -22,7 +22,7 @@ from torch.autograd.function import once_differentiable
 
 from . import gridnet_cuda, patch_loop
 from ._lib import activation_id, check, lib
-from .packed import empty_packed, stream_of
+from .packed import PackedActivations, empty_packed, keeps_packed, pack_activations, stream_of, unpack_activations
 
 
 def _assert_step_args(weight, bias, residual_scale, init_activations, block_size, gated):
@@ -138,6 +138,10 @@ class _Op(torch.autograd.Function):
         return super().apply(*args)
 
 
+def _unpacked(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    return unpack_activations(PackedActivations(codes, scales, torch.float32))
+
+
 class GridnetCudaOp(_Op):
     """One outer-loop step of the plain gridnet (gridnet/backend_cuda.py:5-108)."""
 
@@ -147,7 +151,11 @@ class GridnetCudaOp(_Op):
         batch_size = _assert_step_args(weight, bias, residual_scale, init_activations, block_size, False)
         if not batch_size:
             return init_activations.clone()
-        ctx.save_for_backward(weight, bias, residual_scale, init_activations)
+        ctx.packed = keeps_packed() and weight.dtype == torch.float32 and init_activations.is_cuda and any(ctx.needs_input_grad[:4])
+        if ctx.packed:
+            ctx.save_for_backward(weight, bias, residual_scale, *pack_activations(init_activations)[:2])
+        else:
+            ctx.save_for_backward(weight, bias, residual_scale, init_activations)
         ctx.cfg = (inner_iters, block_size, eps, normalize, activation)
         ctx.kept = None
         outputs = torch.empty_like(init_activations)
@@ -155,7 +163,7 @@ class GridnetCudaOp(_Op):
         quad = _quad_step(weight, init_activations, inner_iters, block_size, normalize)
         ctx.quad = quad is not None
         need = 0
-        if weight.dtype == torch.float32 and any(ctx.needs_input_grad[:4]):
+        if weight.dtype == torch.float32 and any(ctx.needs_input_grad[:4]) and not ctx.packed:
             if quad is not None:
                 need = quad[0]
             elif not normalize:
@@ -176,10 +184,11 @@ class GridnetCudaOp(_Op):
 
     @staticmethod
     def backward(ctx, grad_output):
-        weight, bias, residual_scale, init_activations = ctx.saved_tensors
+        weight, bias, residual_scale, *rest = ctx.saved_tensors
+        init_activations = _unpacked(*rest) if ctx.packed else rest[0]
         inner_iters, block_size, eps, normalize, activation = ctx.cfg
         # every gradient buffer is written in full by the library: no zero fill
-        grads = [torch.empty_like(t) for t in ctx.saved_tensors]
+        grads = [torch.empty_like(t) for t in (weight, bias, residual_scale, init_activations)]
         args = (weight, bias, residual_scale, init_activations, grad_output.contiguous(), *grads, inner_iters, block_size)
         kept, ctx.kept = ctx.kept, None
         if ctx.quad:
@@ -199,7 +208,8 @@ class GatedGridnetCudaOp(torch.autograd.Function):
         batch_size = _assert_step_args(weight, bias, None, init_activations, block_size, True)
         if not batch_size:
             return init_activations.clone()
-        ctx.save_for_backward(weight, bias, init_activations)
+        ctx.packed = keeps_packed() and weight.dtype == torch.float32 and init_activations.is_cuda and any(ctx.needs_input_grad[:3])
+        ctx.save_for_backward(weight, bias, *(pack_activations(init_activations)[:2] if ctx.packed else (init_activations,)))
         ctx.cfg = (inner_iters, block_size, activation)
         outputs = torch.empty_like(init_activations)
         gridnet_cuda.forward_gated(weight, bias, init_activations, outputs, inner_iters, block_size, activation)
@@ -207,7 +217,8 @@ class GatedGridnetCudaOp(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_output):
-        weight, bias, init_activations = ctx.saved_tensors
+        weight, bias, *rest = ctx.saved_tensors
+        init_activations = _unpacked(*rest) if ctx.packed else rest[0]
         inner_iters, block_size, activation = ctx.cfg
         weight_grad = torch.empty_like(weight)
         bias_grad = torch.empty_like(bias)
@@ -363,6 +374,34 @@ class _Pool:
         return iter(self._cut(lambda off, nbytes: self.memory[off:off + nbytes]))
 
 
+class _PackedLoop:
+    """What a loop keeps in 8 bits: its statistics, then the input and the output of each step, in one allocation."""
+
+    def __init__(self, memory: torch.Tensor, layout):
+        self.memory, self.layout = memory, layout
+
+    def addresses(self):
+        outer, stat, one = self.layout
+        base = self.memory.data_ptr()
+        return base, (ctypes.c_void_p * (outer + 1))(*[base + stat + k * one for k in range(outer + 1)])
+
+
+class _PackedPatches:
+    """The same for the register-patch kernels: tensors in the grid's own layout, each packed by itself (the input first)."""
+
+    def __init__(self, stats: torch.Tensor, packed):
+        self.stats, self.packed = stats, packed
+        self.at_hand = {}
+
+    def __getitem__(self, k: int) -> torch.Tensor:
+        """The output of step k (-1: the input), unpacked; the two asked for last are kept."""
+        if k not in self.at_hand:
+            while len(self.at_hand) > 1:
+                self.at_hand.pop(next(iter(self.at_hand)))
+            self.at_hand[k] = unpack_activations(self.packed[k + 1])
+        return self.at_hand[k]
+
+
 def _kept_steps(nbytes_out: int, nbytes_stash: int, outer: int, device) -> int:
     """How many of the ``outer`` steps of a differentiated loop keep their inner iterations (the LAST ones: their
     backward comes first): all or none when :func:`keep_forward_stash` forces it; otherwise as many as fit into 70 % of the
@@ -406,6 +445,14 @@ def _patch_forward(plist, norm_weight, norm_bias, x, inner: int, outer: int, blo
                    residual: bool, need_grad: bool):
     """:func:`_loop_forward` where :func:`on_patches`: x, outs and stashes are in the grid's own layout, x in float32."""
     one, dev = x.numel() * 4, x.device
+    if need_grad and keeps_packed():
+        with torch.cuda.device(dev):
+            stats = torch.empty(outer, x.shape[0], 2, dtype=torch.float32, device=dev)
+            turns = [torch.empty_like(x) for _ in range(min(2, outer))]
+            packed = [pack_activations(x)]
+            y = patch_loop.forward(plist, norm_weight, norm_bias, x, inner, outer, block, activation, ln_eps, residual,
+                                   [turns[k & 1] for k in range(outer)], stats, [None] * outer, lambda out: packed.append(pack_activations(out)))
+        return y, _PackedPatches(stats, packed)
     with torch.cuda.device(dev):
         stash = patch_loop.stash_bytes(x, inner, block)
         keep = _kept_steps(one, stash, outer, dev) if need_grad and stash else 0
@@ -436,6 +483,21 @@ def _loop_forward(plist, norm_weight, norm_bias, x, inner: int, outer: int, bloc
     stat = outer * 4 * ((B + 3) // 4) * 8
     stat = (stat + 255) // 256 * 256
     y = torch.empty_like(x)
+    if need_grad and keeps_packed():
+        one = int(lib.gn_loop_packed_bytes(B, M, N, K))
+        with torch.cuda.device(dev):
+            ws = torch.empty(int(lib.gn_loop_packed_workspace_bytes(B, M, N, K, inner, outer, block, int(residual), int(gated), 0)),
+                             dtype=torch.uint8, device=dev)
+            saved = _PackedLoop(torch.empty(stat + (outer + 1) * one, dtype=torch.uint8, device=dev), (outer, stat, one))
+            stats, packed = saved.addresses()
+            tail = (norm_weight.data_ptr(), norm_bias.data_ptr(), x.data_ptr(), y.data_ptr(), packed, stats, B, M, N, K, inner, outer)
+            end = (ws.data_ptr(), ws.numel(), stream_of(x))
+            if gated:
+                check(lib.gn_gated_loop_forward_packed_f32(plist[0][0].data_ptr(), plist[0][1].data_ptr(), *tail, ln_eps, activation_id(activation), *end))
+            else:
+                check(lib.gn_loop_forward_packed_f32(*(_pointers([p[i] for p in plist]) for i in range(3)), len(plist), *tail, block, ln_eps,
+                                                     activation_id(activation), int(residual), *end))
+        return y, saved
     with torch.cuda.device(dev):
         if gated:
             wbytes = int(lib.gn_gated_loop_workspace_bytes(B, M, N, K, inner, outer, 0, 0))
@@ -487,10 +549,16 @@ def _loop_backward(plist, norm_weight, norm_bias, saved, grad_y, inner: int, out
                    residual: bool, gated: bool = False):
     """The gradients of :func:`_loop_forward` through ``gn_loop_backward_f32``: one (weight, bias, residual_scale) triple per
     entry of ``plist``, then those of the norm's weight and bias and of x."""
-    x_il4, stats, outs, stashes = saved
     g = grad_y.contiguous()
     B, M, N, K = g.shape
     dev = g.device
+    if isinstance(saved, _PackedPatches):
+        with torch.cuda.device(dev):
+            return patch_loop.backward(plist, norm_weight, norm_bias, saved[-1], saved, saved.stats, [None] * outer, g, inner, outer, block, activation,
+                                       residual)
+    if isinstance(saved, _PackedLoop):
+        return _packed_loop_backward(plist, norm_weight, norm_bias, saved, g, inner, outer, block, activation, residual, gated)
+    x_il4, stats, outs, stashes = saved
     if x_il4.dtype == torch.float32:  # _patch_forward
         with torch.cuda.device(dev):
             return patch_loop.backward(plist, norm_weight, norm_bias, x_il4, outs, stats, stashes, g, inner, outer, block, activation, residual)
@@ -518,8 +586,36 @@ def _loop_backward(plist, norm_weight, norm_bias, saved, grad_y, inner: int, out
     return grads, gg, gb, gx
 
 
+def _packed_loop_backward(plist, norm_weight, norm_bias, saved, g, inner: int, outer: int, block: int, activation: str, residual: bool, gated: bool):
+    B, M, N, K = g.shape
+    dev = g.device
+    grads = [tuple(torch.empty_like(t) for t in params) for params in plist]
+    gg, gb, gx = torch.empty_like(norm_weight), torch.empty_like(norm_bias), torch.empty_like(g)
+    with torch.cuda.device(dev):
+        ws = torch.empty(int(lib.gn_loop_packed_workspace_bytes(B, M, N, K, inner, outer, block, int(residual), int(gated), 1)), dtype=torch.uint8,
+                         device=dev)
+        stats, packed = saved.addresses()
+        norms, end = (gg.data_ptr(), gb.data_ptr(), gx.data_ptr(), B, M, N, K, inner, outer), (ws.data_ptr(), ws.numel(), stream_of(g))
+        if gated:
+            check(lib.gn_gated_loop_backward_packed_f32(*(t.data_ptr() for t in plist[0]), norm_weight.data_ptr(), norm_bias.data_ptr(), packed, stats,
+                                                        g.data_ptr(), *(t.data_ptr() for t in grads[0]), *norms, activation_id(activation), *end))
+        else:
+            columns = [_pointers([p[i] for p in plist]) for i in range(3)] + [_pointers([p[i] for p in grads]) for i in range(3)]
+            check(lib.gn_loop_backward_packed_f32(*columns[:3], len(plist), norm_weight.data_ptr(), norm_bias.data_ptr(), packed, stats, g.data_ptr(),
+                                                  *columns[3:], *norms, block, activation_id(activation), int(residual), *end))
+    return grads, gg, gb, gx
+
+
 def _save_loop(ctx, params, saved):
-    ctx.layout = None
+    ctx.layout = ctx.packed = None
+    if isinstance(saved, _PackedLoop):
+        ctx.packed = saved.layout
+        ctx.save_for_backward(*params, saved.memory)
+        return
+    if isinstance(saved, _PackedPatches):
+        ctx.packed = "patches"
+        ctx.save_for_backward(*params, saved.stats, *(t for p in saved.packed for t in p[:2]))
+        return
     if isinstance(saved, _Pool):
         ctx.layout = saved.layout
         ctx.save_for_backward(*params, saved.memory)
@@ -532,6 +628,10 @@ def _save_loop(ctx, params, saved):
 def _restore_loop(ctx, nparams: int, outer: int):
     t = ctx.saved_tensors
     params, rest = t[:nparams], t[nparams:]
+    if ctx.packed == "patches":
+        return params, _PackedPatches(rest[0], [PackedActivations(c, sc, torch.float32) for c, sc in zip(rest[1::2], rest[2::2])])
+    if ctx.packed:
+        return params, _PackedLoop(rest[0], ctx.packed)
     if ctx.layout:
         return params, _Pool(rest[0], ctx.layout).pieces()
     outs, kept = rest[2:2 + outer], iter(rest[2 + outer:])

@@ -330,4 +330,32 @@ int launch_norm_backward_apply(const float *x, const float *gamma, const float *
                                const double2 *sums, long long P_total, float2 *ac, float *gx, float *ggamma, float *gbeta,
                                int B, long long P, cudaStream_t st);
 
+// ---- quad_loop.cu: the loops with 8-bit copies between the passes, and packed_loop.cu, which brings what packs them
+struct LoopPacked {
+    void *const *of;  // [outer + 1]: the input, the output of each step
+    int (*pack)(const float *x, void *packed, int Q, long long P, cudaStream_t st);
+    int (*unpack)(const void *packed, float *x, int Q, long long P, cudaStream_t st);
+};
+size_t loop_packed_workspace(int B, int M, int N, int K, int inner, int outer, int block, int residual, bool gated, bool backward);
+int loop_forward_packed(const LoopPacked &packed, const float *const *weights, const float *const *biases, const float *const *scales,
+                        int nparams, const float *gamma, const float *beta, const float *x, float *y, float *stats, int B, int M, int N,
+                        int K, int inner, int outer, int block, float ln_eps, int act, int residual, void *workspace,
+                        size_t workspace_bytes, cudaStream_t st);
+int loop_backward_packed(const LoopPacked &packed, const float *const *weights, const float *const *biases, const float *const *scales,
+                         int nparams, const float *gamma, const float *beta, const float *stats, const float *gy, float *const *gw,
+                         float *const *gb, float *const *gs, float *ggamma, float *gbeta, float *gx, int B, int M, int N, int K, int inner,
+                         int outer, int block, int act, int residual, void *workspace, size_t workspace_bytes, cudaStream_t st);
+int gated_loop_forward_packed(const LoopPacked &packed, const float *weight, const float *bias, const float *gamma, const float *beta,
+                              const float *x, float *y, float *stats, int B, int M, int N, int K, int inner, int outer, float ln_eps,
+                              int act, void *workspace, size_t workspace_bytes, cudaStream_t st);
+int gated_loop_backward_packed(const LoopPacked &packed, const float *weight, const float *bias, const float *gamma, const float *beta,
+                               const float *stats, const float *gy, float *gw, float *gb, float *ggamma, float *gbeta, float *gx, int B,
+                               int M, int N, int K, int inner, int outer, int act, void *workspace, size_t workspace_bytes,
+                               cudaStream_t st);
+
+// ---- pack8.cu: IL4 tensors in 8 bits (P a multiple of 32, 256-byte aligned)
+size_t il4_packed_bytes(int Q, long long P);
+int launch_pack_il4(const float *x, void *packed, int Q, long long P, cudaStream_t st);
+int launch_unpack_il4(const void *packed, float *x, int Q, long long P, cudaStream_t st);
+
 }  // namespace gn

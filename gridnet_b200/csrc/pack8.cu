@@ -209,6 +209,84 @@ static int pack8_call(const void *x, void *codes, void *scales, long long rows, 
     return launch_pack8<__half>(x, codes, scales, rows, cols, unpack, st);
 }
 
+// ---- IL4 tensors ([Q][P][4 samples], P a multiple of 32): a group is 32 neighbouring positions of one sample, so that no sample's scale
+// depends on another's. A lane has a position, a word the codes of its four samples; behind the codes a word of four scales per 32 positions.
+__global__ void __launch_bounds__(256) pack_il4_k(const float4 *x, unsigned *codes, unsigned *scales, long long groups)
+{
+    constexpr int kTimes = 4;
+    const int lane = threadIdx.x & 31;
+    const long long g0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kTimes;
+    float4 v[kTimes];
+#pragma unroll
+    for (int i = 0; i < kTimes; ++i) v[i] = x[min(g0 + i, groups - 1) * 32 + lane];
+#pragma unroll
+    for (int i = 0; i < kTimes; ++i) {
+        if (g0 + i >= groups) return;
+        const float f[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        unsigned m[4], code[4], scale[4];
+        bool rare = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            m[k] = __reduce_max_sync(0xffffffffu, magnitude_bits(f[k]));
+            rare |= m[k] > kPackLargest;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (rare) {
+                const unsigned b = magnitude_bits(f[k]);
+                m[k] = __reduce_max_sync(0xffffffffu, bits_finite(b) ? b : 0u);
+            }
+            scale[k] = pack_scale(m[k]);
+            code[k] = rare ? pack_code_any(f[k], scale[k]) : pack_code(f[k], pack_inverse(scale[k]));
+        }
+        codes[(g0 + i) * 32 + lane] = pack_word(code[0], code[1], code[2], code[3]);
+        if (lane == 0) scales[g0 + i] = pack_word(scale[0], scale[1], scale[2], scale[3]);
+    }
+}
+
+__global__ void __launch_bounds__(256) unpack_il4_k(const unsigned *__restrict__ codes, const unsigned *__restrict__ scales, float4 *__restrict__ x,
+                                                    long long positions)
+{
+    constexpr int kTimes = 4;
+    const long long at0 = (long long)blockIdx.x * kTimes * 256 + threadIdx.x;
+    unsigned w[kTimes], sc[kTimes];
+#pragma unroll
+    for (int i = 0; i < kTimes; ++i) {
+        const long long at = min(at0 + i * 256, positions - 1);
+        w[i] = codes[at];
+        sc[i] = scales[at / kPackGroup];
+    }
+#pragma unroll
+    for (int i = 0; i < kTimes; ++i) {
+        float f[4];
+        unpack4_finite(w[i], f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] *= pack_step((sc[i] >> (8 * k)) & 0xffu);
+        if (unpack_odd(w[i])) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[k] = unpack_special(f[k], (w[i] >> (8 * k)) & 0xffu);
+        }
+        if (at0 + i * 256 < positions) x[at0 + i * 256] = make_float4(f[0], f[1], f[2], f[3]);
+    }
+}
+
+size_t il4_packed_bytes(int Q, long long P) { return ((size_t)Q * P * 4 + (size_t)Q * (P / kPackGroup) * 4 + 255) / 256 * 256; }
+
+int launch_pack_il4(const float *x, void *packed, int Q, long long P, cudaStream_t st)
+{
+    const long long groups = Q * (P / kPackGroup);
+    unsigned *const codes = (unsigned *)packed;
+    pack_il4_k<<<(unsigned)((groups + 31) / 32), 256, 0, st>>>((const float4 *)x, codes, codes + Q * P, groups);
+    return check_launch("pack_il4");
+}
+
+int launch_unpack_il4(const void *packed, float *x, int Q, long long P, cudaStream_t st)
+{
+    const unsigned *const codes = (const unsigned *)packed;
+    unpack_il4_k<<<(unsigned)((Q * P + 1023) / 1024), 256, 0, st>>>(codes, codes + Q * P, (float4 *)x, Q * P);
+    return check_launch("unpack_il4");
+}
+
 }  // namespace gn
 
 using namespace gn;

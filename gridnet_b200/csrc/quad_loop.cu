@@ -13,6 +13,14 @@
 
 namespace gn {
 
+// With `packed` (packed_loop.cu), the tensors that the passes hand over (input and raw outputs) are 8-bit copies: forward, two tensors take turns and
+// each is packed when its step is done; backward, they are unpacked when their step is walked back, into two tensors that take turns as well: the
+// input of step k, which is the output of step k - 1, into turns[k & 1].
+struct Packed {
+    LoopPacked by;  // by.of nullptr: not packed
+    float *x_il4, *turns[2];
+};
+
 static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 struct LoopDims {
@@ -141,6 +149,293 @@ static int gated_step(const GatedWs &w, const LoopDims &d, const float *in, cons
     return launch_quad_gated_fwd(a, act, st);
 }
 
+static int loop_forward(const float *const *weights, const float *const *biases, const float *const *scales, int nparams, const float *gamma,
+                        const float *beta, const float *x, float *y, float *x_il4, float *const *outs, const Packed &packed, float *stats,
+                        float *const *stashes, const LoopDims &d, const LoopWs &w, float ln_eps, int act, cudaStream_t st)
+{
+    const int B = d.B, M = d.M, N = d.N, K = d.K, inner = d.inner, outer = d.outer, block = d.block, residual = d.residual;
+    float2 *const mr = reinterpret_cast<float2 *>(stats);
+    const int S = 4 * d.Q;  // statistics of one step
+    auto out = [&](int k) { return packed.by.of ? packed.turns[k & 1] : outs[k]; };
+    {
+        QuadPrepare a{};
+        a.w = weights[0]; a.b = biases[0]; a.s = scales[0]; a.packed = w.packed; a.ordered = true;
+        a.gamma = gamma; a.beta = beta; a.gbt = w.gbt;
+        a.x = x; a.il = x_il4; a.B = B;
+        TRY_(launch_quad_prepare(a, M, N, K, block, st));
+    }
+    if (packed.by.of) TRY_(packed.by.pack(x_il4, packed.by.of[0], d.Q, d.P, st));
+    if (residual) {
+        TRY_(launch_quad_residual_combine(x_il4, nullptr, nullptr, nullptr, nullptr, nullptr, w.partials, d.Q, d.P, st));
+        TRY_(launch_norm_finalize(w.partials, quad_combine_parts(d.P), mr, S, d.P, ln_eps, st));
+    }
+    for (int k = 0; k < outer; ++k) {
+        if (k > 0 && nparams > 1) {
+            QuadPrepare a{};
+            a.w = weights[k]; a.b = biases[k]; a.s = scales[k]; a.packed = w.packed; a.ordered = true;
+            TRY_(launch_quad_prepare(a, M, N, K, block, st));
+        }
+        const float *in = k ? out(k - 1) : x_il4;
+        QuadStep a{};
+        a.packed = w.packed; a.gbt = w.gbt;
+        a.in_il4 = in;
+        a.out_il4 = residual ? w.tmp : out(k);
+        a.in_stats = residual ? mr + (size_t)k * S : (k ? mr + (size_t)(k - 1) * S : nullptr);
+        a.out_partials = residual ? nullptr : w.partials;
+        a.nparts = d.regions;
+        a.params_old = k > 0 && nparams == 1;
+        if (stashes) a.save_h = stashes[k];
+        a.M = M; a.N = N; a.K = K; a.Q = d.Q; a.inner = inner; a.block = block;
+        TRY_(launch_step_fwd_quad(a, act, st));
+        if (residual) {
+            TRY_(launch_quad_residual_combine(in, w.tmp, gamma, beta, mr + (size_t)k * S, out(k), w.partials, d.Q, d.P, st));
+            if (k + 1 < outer) TRY_(launch_norm_finalize(w.partials, quad_combine_parts(d.P), mr + (size_t)(k + 1) * S, S, d.P, ln_eps, st));
+        } else {
+            TRY_(launch_norm_finalize(w.partials, d.regions, mr + (size_t)k * S, S, d.P, ln_eps, st));
+        }
+        if (packed.by.of && !(residual && k + 1 == outer)) TRY_(packed.by.pack(out(k), packed.by.of[k + 1], d.Q, d.P, st));
+    }
+    return launch_from_il4(out(outer - 1), residual ? nullptr : mr + (size_t)(outer - 1) * S, gamma, beta, y, B, d.P, st);
+}
+
+static int loop_backward(const float *const *weights, const float *const *biases, const float *const *scales, int nparams, const float *gamma,
+                         const float *beta, const float *x_il4, float *const *outs, const Packed &packed, const float *stats, float *const *stashes,
+                         const float *gy, float *const *gw, float *const *gb, float *const *gs, float *ggamma, float *gbeta, float *gx,
+                         const LoopDims &d, const LoopWs &w, bool replay, int act, cudaStream_t st)
+{
+    const int B = d.B, M = d.M, N = d.N, K = d.K, inner = d.inner, outer = d.outer, block = d.block, residual = d.residual;
+    const float2 *const mr = reinterpret_cast<const float2 *>(stats);
+    const int S = 4 * d.Q;
+    const bool with_border = !residual && quad_border_takes_sums(M, N, K, block);
+    auto raw = [&](int k) { return packed.by.of ? packed.turns[(k + 1) & 1] : outs[k]; };
+    if (packed.by.of && !residual) TRY_(packed.by.unpack(packed.by.of[outer], packed.turns[outer & 1], d.Q, d.P, st));
+    int cur = 0;
+    for (int k = outer - 1; k >= 0; --k) {
+        if (packed.by.of) TRY_(packed.by.unpack(packed.by.of[k], packed.turns[k & 1], d.Q, d.P, st));
+        const int kp = nparams > 1 ? k : 0;
+        const bool first = k == outer - 1;  // first to be walked back
+        const float *in = packed.by.of ? packed.turns[k & 1] : (k ? outs[k - 1] : x_il4);
+        const float2 *in_stats = residual ? mr + (size_t)k * S : (k ? mr + (size_t)(k - 1) * S : nullptr);
+        const bool kept = stashes && stashes[k];
+        bool fresh = false;  // the kernel queued last has re-ordered parameters
+        if (first || nparams > 1) {
+            QuadPrepare a{};
+            a.w = weights[kp]; a.b = biases[kp]; a.s = scales[kp]; a.b_t = gamma; a.packed_t = w.packed_t;
+            if (replay) a.packed = w.packed;
+            a.ordered = true;
+            if (first) {
+                a.gamma = gamma; a.beta = beta; a.gbt = w.gbt;
+                a.x = gy; a.il = w.g[0]; a.B = B; a.gradient = true;
+            }
+            TRY_(launch_quad_prepare(a, M, N, K, block, st));
+            fresh = true;
+        }
+        if (!residual && (first || !with_border)) {  // else taken with the border of the step after
+            TRY_(launch_quad_norm_sums(raw(k), w.g[cur], nullptr, gamma, mr + (size_t)k * S, w.partials, ggamma, gbeta, !first, w.ac, d.Q, d.P, st));
+            fresh = false;
+        }
+        float *const h = kept ? stashes[k] : w.replay;
+        if (!kept) {
+            QuadStep a{};
+            a.packed = w.packed; a.gbt = w.gbt;
+            a.in_il4 = in; a.in_stats = in_stats;
+            a.save_h = h;
+            a.M = M; a.N = N; a.K = K; a.Q = d.Q; a.inner = inner; a.block = block;
+            TRY_(launch_step_fwd_quad(a, act, st));
+            fresh = false;
+        }
+        QuadReverse r{};
+        r.packed_t = w.packed_t; r.g = w.g[cur];
+        r.params_old = !fresh;
+        if (!residual) {
+            r.raw = raw(k); r.stats = mr + (size_t)k * S; r.ac = w.ac;
+        }
+        r.h = h; r.delta = w.delta; r.dsum = w.dsum; r.gx = w.g[cur ^ 1]; r.dsq = w.dsq;
+        r.M = M; r.N = N; r.K = K; r.Q = d.Q; r.inner = inner; r.block = block;
+        TRY_(launch_quad_reverse(r, act, st));
+        QuadWgrad g{};
+        g.in_il4 = in; g.gbt = w.gbt; g.in_stats = in_stats;
+        g.delta = w.delta; g.h = h; g.scale = scales[kp]; g.dsq = w.dsq; g.gpk = w.gpk;
+        g.accumulate = nparams == 1 && !first;
+        g.M = M; g.N = N; g.K = K; g.Q = d.Q; g.inner = inner; g.block = block;
+        TRY_(launch_quad_wgrad(g, act, st));
+        if (nparams > 1 && k > 0) TRY_(launch_quad_finish(w.gpk, gw[kp], gb[kp], gs[kp], nullptr, nullptr, B, M, N, K, block, 1, st));
+        QuadBorder o{};
+        o.w = weights[kp]; o.dsum = w.dsum; o.gx = w.g[cur ^ 1];
+        if (with_border && k > 0) {  // with the sums of the norm that made this step's input
+            o.x_il4 = in; o.stats = in_stats; o.gamma = gamma; o.partials = w.partials; o.ggamma = ggamma; o.gbeta = gbeta; o.ac = w.ac;
+            o.accumulate = 1;
+        }
+        o.M = M; o.N = N; o.K = K; o.Q = d.Q; o.block = block;
+        TRY_(launch_quad_border(o, st));
+        if (residual) {
+            TRY_(launch_quad_norm_sums(in, w.g[cur ^ 1], w.g[cur], gamma, in_stats, w.partials, ggamma, gbeta, !first, w.ac, d.Q, d.P, st));
+            TRY_(launch_quad_norm_residual_apply(in, w.g[cur ^ 1], w.g[cur], gamma, in_stats, w.ac, w.g[cur], d.Q, d.P, st));
+        } else {
+            cur ^= 1;
+        }
+    }
+    return launch_quad_finish(w.gpk, gw[0], gb[0], gs[0], w.g[cur], gx, B, M, N, K, block, 1, st);
+}
+
+static int gated_loop_forward(const float *weight, const float *bias, const float *gamma, const float *beta, const float *x, float *y, float *x_il4,
+                              float *const *outs, const Packed &packed, float *stats, float *const *stashes, const LoopDims &d, const GatedWs &w,
+                              float ln_eps, int act, cudaStream_t st)
+{
+    const int B = d.B, M = d.M, N = d.N, K = d.K, outer = d.outer;
+    float2 *const mr = reinterpret_cast<float2 *>(stats);
+    const int S = 4 * d.Q;
+    auto out = [&](int k) { return packed.by.of ? packed.turns[k & 1] : outs[k]; };
+    QuadPrepare a{};
+    a.w = weight; a.b = bias; a.s = weight; a.gated = true; a.packed = w.packed;
+    a.gamma = gamma; a.beta = beta; a.gbt = w.gbt;
+    a.x = x; a.il = x_il4; a.B = B;
+    TRY_(launch_quad_prepare(a, M, N, K, 8, st));
+    if (packed.by.of) TRY_(packed.by.pack(x_il4, packed.by.of[0], d.Q, d.P, st));
+    for (int k = 0; k < outer; ++k) {
+        TRY_(gated_step(w, d, k ? out(k - 1) : x_il4, k ? mr + (size_t)(k - 1) * S : nullptr, out(k), w.partials, stashes ? stashes[k] : nullptr,
+                        k > 0, act, st));
+        TRY_(launch_norm_finalize(w.partials, 2 * d.regions, mr + (size_t)k * S, S, d.P, ln_eps, st));
+        if (packed.by.of) TRY_(packed.by.pack(out(k), packed.by.of[k + 1], d.Q, d.P, st));
+    }
+    return launch_from_il4(out(outer - 1), mr + (size_t)(outer - 1) * S, gamma, beta, y, B, d.P, st);
+}
+
+static int gated_loop_backward(const float *weight, const float *bias, const float *gamma, const float *beta, const float *x_il4, float *const *outs,
+                               const Packed &packed, const float *stats, float *const *stashes, const float *gy, float *gw, float *gb, float *ggamma,
+                               float *gbeta, float *gx, const LoopDims &d, const GatedWs &w, bool replay, int act, cudaStream_t st)
+{
+    const int B = d.B, M = d.M, N = d.N, K = d.K, inner = d.inner, outer = d.outer;
+    const float2 *const mr = reinterpret_cast<const float2 *>(stats);
+    const int S = 4 * d.Q;
+    {
+        QuadPrepare a{};
+        a.w = weight; a.b = bias; a.s = weight; a.b_t = bias; a.gated = true; a.packed_t = w.packed_t;
+        if (replay) a.packed = w.packed;
+        a.gamma = gamma; a.beta = beta; a.gbt = w.gbt;
+        a.x = gy; a.il = w.g[0]; a.B = B; a.gradient = true;
+        TRY_(launch_quad_prepare(a, M, N, K, 8, st));
+    }
+    const bool with_border = quad_border_takes_sums(M, N, K, 8);
+    float *const delta_v = w.delta, *const delta_g = w.delta + inner * d.T4, *const dsum_v = w.dsum, *const dsum_g = w.dsum + d.T4;
+    auto raw = [&](int k) { return packed.by.of ? packed.turns[(k + 1) & 1] : outs[k]; };
+    if (packed.by.of) TRY_(packed.by.unpack(packed.by.of[outer], packed.turns[outer & 1], d.Q, d.P, st));
+    int cur = 0;
+    for (int k = outer - 1; k >= 0; --k, cur ^= 1) {
+        if (packed.by.of) TRY_(packed.by.unpack(packed.by.of[k], packed.turns[k & 1], d.Q, d.P, st));
+        const bool first = k == outer - 1;
+        const float *in = packed.by.of ? packed.turns[k & 1] : (k ? outs[k - 1] : x_il4);
+        const float2 *in_stats = k ? mr + (size_t)(k - 1) * S : nullptr;
+        if (first || !with_border)  // else taken with the border of the step after
+            TRY_(launch_quad_norm_sums(raw(k), w.g[cur], nullptr, gamma, mr + (size_t)k * S, w.partials, ggamma, gbeta, !first, w.ac, d.Q, d.P, st));
+        float *kept = stashes ? stashes[k] : nullptr;
+        if (!kept) {
+            // the step's output is computed once more, into the buffer that receives the gradient afterwards
+            kept = w.replay;
+            TRY_(gated_step(w, d, in, in_stats, w.g[cur ^ 1], nullptr, kept, 1, act, st));
+        }
+        QuadGatedReverse r{};
+        r.packed_t = w.packed_t; r.gamma = gamma; r.g = w.g[cur]; r.raw = raw(k); r.stats = mr + (size_t)k * S; r.ac = w.ac;
+        r.hv = kept; r.hg = kept + inner * d.T4; r.x = kept + 2 * inner * d.T4;
+        r.delta_v = delta_v; r.delta_g = delta_g; r.dsum_v = dsum_v; r.dsum_g = dsum_g; r.gx = w.g[cur ^ 1];
+        r.M = M; r.N = N; r.K = K; r.Q = d.Q; r.inner = inner;
+        TRY_(launch_quad_gated_reverse(r, act, st));
+        QuadWgrad g{};
+        g.in_il4 = in; g.gbt = w.gbt; g.in_stats = in_stats;
+        g.delta = delta_v; g.delta2 = delta_g; g.h = r.x + d.T4; g.gpk = w.gpk;
+        g.accumulate = !first;
+        g.M = M; g.N = N; g.K = K; g.Q = d.Q; g.inner = inner; g.block = 8;
+        TRY_(launch_quad_wgrad(g, act, st));
+        QuadBorder o{};
+        o.w = weight; o.dsum = dsum_v; o.dsum2 = dsum_g; o.gx = w.g[cur ^ 1];
+        if (with_border && k > 0) {  // with the sums of the norm that made this step's input
+            o.x_il4 = in; o.stats = in_stats; o.gamma = gamma; o.partials = w.partials; o.ggamma = ggamma; o.gbeta = gbeta; o.ac = w.ac;
+            o.accumulate = 1;
+        }
+        o.M = M; o.N = N; o.K = K; o.Q = d.Q; o.block = 8;
+        TRY_(launch_quad_border(o, st));
+    }
+    return launch_quad_finish(w.gpk, gw, gb, nullptr, w.g[cur], gx, B, M, N, K, 8, 2, st);
+}
+
+// The workspace of a packed pass: that of the loop, then the tensors that take turns (forward the input too). Returns its size
+static size_t packed_ws(void *base, const LoopDims &d, bool gated, bool backward, Packed *p)
+{
+    const size_t loop = up256(gated ? carve_gated(nullptr, d, backward, backward).bytes : carve_loop(nullptr, d, backward, backward).bytes);
+    const size_t t = up256(sizeof(float) * d.T4);
+    if (p) {
+        unsigned char *const at = static_cast<unsigned char *>(base) + loop;
+        p->turns[0] = reinterpret_cast<float *>(at);
+        p->turns[1] = reinterpret_cast<float *>(at + t);
+        if (!backward) p->x_il4 = reinterpret_cast<float *>(at + 2 * t);
+    }
+    return loop + (backward ? 2 : 3) * t;
+}
+
+size_t loop_packed_workspace(int B, int M, int N, int K, int inner, int outer, int block, int residual, bool gated, bool backward)
+{
+    if (loop_check(B, M, N, K, inner, outer, block, GN_ACT_RELU, 1) != GN_OK) return 0;
+    return packed_ws(nullptr, loop_dims(B, M, N, K, inner, outer, block, 1, residual), gated, backward, nullptr);
+}
+
+int loop_forward_packed(const LoopPacked &packed, const float *const *weights, const float *const *biases, const float *const *scales, int nparams,
+                                      const float *gamma, const float *beta, const float *x, float *y, float *stats, int B, int M,
+                                      int N, int K, int inner, int outer, int block, float ln_eps, int act, int residual, void *workspace,
+                                      size_t workspace_bytes, cudaStream_t st)
+{
+    TRY_(loop_check(B, M, N, K, inner, outer, block, act, nparams));
+    if (!weights || !biases || !scales || !gamma || !beta || !x || !y || !packed.of || !stats || !workspace) return GN_ERR_NULL_POINTER;
+    const LoopDims d = loop_dims(B, M, N, K, inner, outer, block, nparams, residual);
+    Packed p{packed, nullptr, {nullptr, nullptr}};
+    if (workspace_bytes < packed_ws(workspace, d, false, false, &p) || reinterpret_cast<uintptr_t>(workspace) % 256) return GN_ERR_WORKSPACE;
+    return loop_forward(weights, biases, scales, nparams, gamma, beta, x, y, p.x_il4, nullptr, p, stats, nullptr, d,
+                        carve_loop(workspace, d, false, false), ln_eps, act, st);
+}
+
+int loop_backward_packed(const LoopPacked &packed, const float *const *weights, const float *const *biases, const float *const *scales, int nparams,
+                                       const float *gamma, const float *beta, const float *stats, const float *gy,
+                                       float *const *gw, float *const *gb, float *const *gs, float *ggamma, float *gbeta, float *gx, int B, int M,
+                                       int N, int K, int inner, int outer, int block, int act, int residual, void *workspace,
+                                       size_t workspace_bytes, cudaStream_t st)
+{
+    TRY_(loop_check(B, M, N, K, inner, outer, block, act, nparams));
+    if (!weights || !biases || !scales || !gamma || !beta || !packed.of || !stats || !gy || !gw || !gb || !gs || !ggamma || !gbeta || !gx || !workspace)
+        return GN_ERR_NULL_POINTER;
+    const LoopDims d = loop_dims(B, M, N, K, inner, outer, block, nparams, residual);
+    Packed p{packed, nullptr, {nullptr, nullptr}};
+    if (workspace_bytes < packed_ws(workspace, d, false, true, &p) || reinterpret_cast<uintptr_t>(workspace) % 256) return GN_ERR_WORKSPACE;
+    return loop_backward(weights, biases, scales, nparams, gamma, beta, nullptr, nullptr, p, stats, nullptr, gy, gw, gb, gs, ggamma, gbeta, gx, d,
+                         carve_loop(workspace, d, true, true), true, act, st);
+}
+
+int gated_loop_forward_packed(const LoopPacked &packed, const float *weight, const float *bias, const float *gamma, const float *beta, const float *x, float *y,
+                                            float *stats, int B, int M, int N, int K, int inner, int outer, float ln_eps,
+                                            int act, void *workspace, size_t workspace_bytes, cudaStream_t st)
+{
+    TRY_(loop_check(B, M, N, K, inner, outer, 8, act, 1));
+    if (!weight || !bias || !gamma || !beta || !x || !y || !packed.of || !stats || !workspace) return GN_ERR_NULL_POINTER;
+    const LoopDims d = loop_dims(B, M, N, K, inner, outer, 8, 1, 0);
+    Packed p{packed, nullptr, {nullptr, nullptr}};
+    if (workspace_bytes < packed_ws(workspace, d, true, false, &p) || reinterpret_cast<uintptr_t>(workspace) % 256) return GN_ERR_WORKSPACE;
+    return gated_loop_forward(weight, bias, gamma, beta, x, y, p.x_il4, nullptr, p, stats, nullptr, d, carve_gated(workspace, d, false, false), ln_eps,
+                              act, st);
+}
+
+int gated_loop_backward_packed(const LoopPacked &packed, const float *weight, const float *bias, const float *gamma, const float *beta,
+                               const float *stats, const float *gy, float *gw, float *gb, float *ggamma, float *gbeta, float *gx, int B,
+                                             int M, int N, int K, int inner, int outer, int act, void *workspace, size_t workspace_bytes,
+                                             cudaStream_t st)
+{
+    TRY_(loop_check(B, M, N, K, inner, outer, 8, act, 1));
+    if (!weight || !bias || !gamma || !beta || !packed.of || !stats || !gy || !gw || !gb || !ggamma || !gbeta || !gx || !workspace)
+        return GN_ERR_NULL_POINTER;
+    const LoopDims d = loop_dims(B, M, N, K, inner, outer, 8, 1, 0);
+    Packed p{packed, nullptr, {nullptr, nullptr}};
+    if (workspace_bytes < packed_ws(workspace, d, true, true, &p) || reinterpret_cast<uintptr_t>(workspace) % 256) return GN_ERR_WORKSPACE;
+    return gated_loop_backward(weight, bias, gamma, beta, nullptr, nullptr, p, stats, nullptr, gy, gw, gb, ggamma, gbeta, gx, d,
+                               carve_gated(workspace, d, true, true), true, act, st);
+}
+
 }  // namespace gn
 
 using namespace gn;
@@ -180,46 +475,8 @@ GN_API int gn_loop_forward_f32(const float *const *weights, const float *const *
     const LoopDims d = loop_dims(B, M, N, K, inner, outer, block, nparams, residual);
     const LoopWs w = carve_loop(workspace, d, false, false);
     if (workspace_bytes < w.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return GN_ERR_WORKSPACE;
-    cudaStream_t st = (cudaStream_t)stream;
-    float2 *const mr = reinterpret_cast<float2 *>(stats);
-    const int S = 4 * d.Q;  // statistics of one step
-    {
-        QuadPrepare a{};
-        a.w = weights[0]; a.b = biases[0]; a.s = scales[0]; a.packed = w.packed; a.ordered = true;
-        a.gamma = gamma; a.beta = beta; a.gbt = w.gbt;
-        a.x = x; a.il = x_il4; a.B = B;
-        TRY_(launch_quad_prepare(a, M, N, K, block, st));
-    }
-    if (residual) {
-        TRY_(launch_quad_residual_combine(x_il4, nullptr, nullptr, nullptr, nullptr, nullptr, w.partials, d.Q, d.P, st));
-        TRY_(launch_norm_finalize(w.partials, quad_combine_parts(d.P), mr, S, d.P, ln_eps, st));
-    }
-    for (int k = 0; k < outer; ++k) {
-        if (k > 0 && nparams > 1) {
-            QuadPrepare a{};
-            a.w = weights[k]; a.b = biases[k]; a.s = scales[k]; a.packed = w.packed; a.ordered = true;
-            TRY_(launch_quad_prepare(a, M, N, K, block, st));
-        }
-        const float *in = k ? outs[k - 1] : x_il4;
-        QuadStep a{};
-        a.packed = w.packed; a.gbt = w.gbt;
-        a.in_il4 = in;
-        a.out_il4 = residual ? w.tmp : outs[k];
-        a.in_stats = residual ? mr + (size_t)k * S : (k ? mr + (size_t)(k - 1) * S : nullptr);
-        a.out_partials = residual ? nullptr : w.partials;
-        a.nparts = d.regions;
-        a.params_old = k > 0 && nparams == 1;
-        if (stashes) a.save_h = stashes[k];
-        a.M = M; a.N = N; a.K = K; a.Q = d.Q; a.inner = inner; a.block = block;
-        TRY_(launch_step_fwd_quad(a, act, st));
-        if (residual) {
-            TRY_(launch_quad_residual_combine(in, w.tmp, gamma, beta, mr + (size_t)k * S, outs[k], w.partials, d.Q, d.P, st));
-            if (k + 1 < outer) TRY_(launch_norm_finalize(w.partials, quad_combine_parts(d.P), mr + (size_t)(k + 1) * S, S, d.P, ln_eps, st));
-        } else {
-            TRY_(launch_norm_finalize(w.partials, d.regions, mr + (size_t)k * S, S, d.P, ln_eps, st));
-        }
-    }
-    return launch_from_il4(outs[outer - 1], residual ? nullptr : mr + (size_t)(outer - 1) * S, gamma, beta, y, B, d.P, st);
+    return loop_forward(weights, biases, scales, nparams, gamma, beta, x, y, x_il4, outs, Packed{}, stats, stashes, d, w, ln_eps, act,
+                        (cudaStream_t)stream);
 }
 
 GN_API int gn_loop_backward_f32(const float *const *weights, const float *const *biases, const float *const *scales, int nparams,
@@ -237,76 +494,8 @@ GN_API int gn_loop_backward_f32(const float *const *weights, const float *const 
     for (int k = 0; k < outer; ++k) replay |= !stashes || !stashes[k];
     const LoopWs w = carve_loop(workspace, d, true, replay);
     if (workspace_bytes < w.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return GN_ERR_WORKSPACE;
-    cudaStream_t st = (cudaStream_t)stream;
-    const float2 *const mr = reinterpret_cast<const float2 *>(stats);
-    const int S = 4 * d.Q;
-    const bool with_border = !residual && quad_border_takes_sums(M, N, K, block);
-    int cur = 0;
-    for (int k = outer - 1; k >= 0; --k) {
-        const int kp = nparams > 1 ? k : 0;
-        const bool first = k == outer - 1;  // first to be walked back
-        const float *in = k ? outs[k - 1] : x_il4;
-        const float2 *in_stats = residual ? mr + (size_t)k * S : (k ? mr + (size_t)(k - 1) * S : nullptr);
-        const bool kept = stashes && stashes[k];
-        bool fresh = false;  // the kernel queued last has re-ordered parameters
-        if (first || nparams > 1) {
-            QuadPrepare a{};
-            a.w = weights[kp]; a.b = biases[kp]; a.s = scales[kp]; a.b_t = gamma; a.packed_t = w.packed_t;
-            if (replay) a.packed = w.packed;
-            a.ordered = true;
-            if (first) {
-                a.gamma = gamma; a.beta = beta; a.gbt = w.gbt;
-                a.x = gy; a.il = w.g[0]; a.B = B; a.gradient = true;
-            }
-            TRY_(launch_quad_prepare(a, M, N, K, block, st));
-            fresh = true;
-        }
-        if (!residual && (first || !with_border)) {  // else taken with the border of the step after
-            TRY_(launch_quad_norm_sums(outs[k], w.g[cur], nullptr, gamma, mr + (size_t)k * S, w.partials, ggamma, gbeta, !first, w.ac, d.Q, d.P, st));
-            fresh = false;
-        }
-        float *const h = kept ? stashes[k] : w.replay;
-        if (!kept) {
-            QuadStep a{};
-            a.packed = w.packed; a.gbt = w.gbt;
-            a.in_il4 = in; a.in_stats = in_stats;
-            a.save_h = h;
-            a.M = M; a.N = N; a.K = K; a.Q = d.Q; a.inner = inner; a.block = block;
-            TRY_(launch_step_fwd_quad(a, act, st));
-            fresh = false;
-        }
-        QuadReverse r{};
-        r.packed_t = w.packed_t; r.g = w.g[cur];
-        r.params_old = !fresh;
-        if (!residual) {
-            r.raw = outs[k]; r.stats = mr + (size_t)k * S; r.ac = w.ac;
-        }
-        r.h = h; r.delta = w.delta; r.dsum = w.dsum; r.gx = w.g[cur ^ 1]; r.dsq = w.dsq;
-        r.M = M; r.N = N; r.K = K; r.Q = d.Q; r.inner = inner; r.block = block;
-        TRY_(launch_quad_reverse(r, act, st));
-        QuadWgrad g{};
-        g.in_il4 = in; g.gbt = w.gbt; g.in_stats = in_stats;
-        g.delta = w.delta; g.h = h; g.scale = scales[kp]; g.dsq = w.dsq; g.gpk = w.gpk;
-        g.accumulate = nparams == 1 && !first;
-        g.M = M; g.N = N; g.K = K; g.Q = d.Q; g.inner = inner; g.block = block;
-        TRY_(launch_quad_wgrad(g, act, st));
-        if (nparams > 1 && k > 0) TRY_(launch_quad_finish(w.gpk, gw[kp], gb[kp], gs[kp], nullptr, nullptr, B, M, N, K, block, 1, st));
-        QuadBorder o{};
-        o.w = weights[kp]; o.dsum = w.dsum; o.gx = w.g[cur ^ 1];
-        if (with_border && k > 0) {  // with the sums of the norm that made this step's input
-            o.x_il4 = in; o.stats = in_stats; o.gamma = gamma; o.partials = w.partials; o.ggamma = ggamma; o.gbeta = gbeta; o.ac = w.ac;
-            o.accumulate = 1;
-        }
-        o.M = M; o.N = N; o.K = K; o.Q = d.Q; o.block = block;
-        TRY_(launch_quad_border(o, st));
-        if (residual) {
-            TRY_(launch_quad_norm_sums(in, w.g[cur ^ 1], w.g[cur], gamma, in_stats, w.partials, ggamma, gbeta, !first, w.ac, d.Q, d.P, st));
-            TRY_(launch_quad_norm_residual_apply(in, w.g[cur ^ 1], w.g[cur], gamma, in_stats, w.ac, w.g[cur], d.Q, d.P, st));
-        } else {
-            cur ^= 1;
-        }
-    }
-    return launch_quad_finish(w.gpk, gw[0], gb[0], gs[0], w.g[cur], gx, B, M, N, K, block, 1, st);
+    return loop_backward(weights, biases, scales, nparams, gamma, beta, x_il4, outs, Packed{}, stats, stashes, gy, gw, gb, gs, ggamma, gbeta, gx, d, w,
+                         replay, act, (cudaStream_t)stream);
 }
 
 GN_API size_t gn_gated_loop_workspace_bytes(int B, int M, int N, int K, int inner, int outer, int backward, int replay)
@@ -324,20 +513,7 @@ GN_API int gn_gated_loop_forward_f32(const float *weight, const float *bias, con
     const LoopDims d = loop_dims(B, M, N, K, inner, outer, 8, 1, 0);
     const GatedWs w = carve_gated(workspace, d, false, false);
     if (workspace_bytes < w.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return GN_ERR_WORKSPACE;
-    cudaStream_t st = (cudaStream_t)stream;
-    float2 *const mr = reinterpret_cast<float2 *>(stats);
-    const int S = 4 * d.Q;
-    QuadPrepare a{};
-    a.w = weight; a.b = bias; a.s = weight; a.gated = true; a.packed = w.packed;
-    a.gamma = gamma; a.beta = beta; a.gbt = w.gbt;
-    a.x = x; a.il = x_il4; a.B = B;
-    TRY_(launch_quad_prepare(a, M, N, K, 8, st));
-    for (int k = 0; k < outer; ++k) {
-        TRY_(gated_step(w, d, k ? outs[k - 1] : x_il4, k ? mr + (size_t)(k - 1) * S : nullptr, outs[k], w.partials, stashes ? stashes[k] : nullptr,
-                        k > 0, act, st));
-        TRY_(launch_norm_finalize(w.partials, 2 * d.regions, mr + (size_t)k * S, S, d.P, ln_eps, st));
-    }
-    return launch_from_il4(outs[outer - 1], mr + (size_t)(outer - 1) * S, gamma, beta, y, B, d.P, st);
+    return gated_loop_forward(weight, bias, gamma, beta, x, y, x_il4, outs, Packed{}, stats, stashes, d, w, ln_eps, act, (cudaStream_t)stream);
 }
 
 GN_API int gn_gated_loop_backward_f32(const float *weight, const float *bias, const float *gamma, const float *beta, const float *x_il4,
@@ -353,54 +529,8 @@ GN_API int gn_gated_loop_backward_f32(const float *weight, const float *bias, co
     for (int k = 0; k < outer; ++k) replay |= !stashes || !stashes[k];
     const GatedWs w = carve_gated(workspace, d, true, replay);
     if (workspace_bytes < w.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return GN_ERR_WORKSPACE;
-    cudaStream_t st = (cudaStream_t)stream;
-    const float2 *const mr = reinterpret_cast<const float2 *>(stats);
-    const int S = 4 * d.Q;
-    {
-        QuadPrepare a{};
-        a.w = weight; a.b = bias; a.s = weight; a.b_t = bias; a.gated = true; a.packed_t = w.packed_t;
-        if (replay) a.packed = w.packed;
-        a.gamma = gamma; a.beta = beta; a.gbt = w.gbt;
-        a.x = gy; a.il = w.g[0]; a.B = B; a.gradient = true;
-        TRY_(launch_quad_prepare(a, M, N, K, 8, st));
-    }
-    const bool with_border = quad_border_takes_sums(M, N, K, 8);
-    float *const delta_v = w.delta, *const delta_g = w.delta + inner * d.T4, *const dsum_v = w.dsum, *const dsum_g = w.dsum + d.T4;
-    int cur = 0;
-    for (int k = outer - 1; k >= 0; --k, cur ^= 1) {
-        const bool first = k == outer - 1;
-        const float *in = k ? outs[k - 1] : x_il4;
-        const float2 *in_stats = k ? mr + (size_t)(k - 1) * S : nullptr;
-        if (first || !with_border)  // else taken with the border of the step after
-            TRY_(launch_quad_norm_sums(outs[k], w.g[cur], nullptr, gamma, mr + (size_t)k * S, w.partials, ggamma, gbeta, !first, w.ac, d.Q, d.P, st));
-        float *kept = stashes ? stashes[k] : nullptr;
-        if (!kept) {
-            // the step's output is computed once more, into the buffer that receives the gradient afterwards
-            kept = w.replay;
-            TRY_(gated_step(w, d, in, in_stats, w.g[cur ^ 1], nullptr, kept, 1, act, st));
-        }
-        QuadGatedReverse r{};
-        r.packed_t = w.packed_t; r.gamma = gamma; r.g = w.g[cur]; r.raw = outs[k]; r.stats = mr + (size_t)k * S; r.ac = w.ac;
-        r.hv = kept; r.hg = kept + inner * d.T4; r.x = kept + 2 * inner * d.T4;
-        r.delta_v = delta_v; r.delta_g = delta_g; r.dsum_v = dsum_v; r.dsum_g = dsum_g; r.gx = w.g[cur ^ 1];
-        r.M = M; r.N = N; r.K = K; r.Q = d.Q; r.inner = inner;
-        TRY_(launch_quad_gated_reverse(r, act, st));
-        QuadWgrad g{};
-        g.in_il4 = in; g.gbt = w.gbt; g.in_stats = in_stats;
-        g.delta = delta_v; g.delta2 = delta_g; g.h = r.x + d.T4; g.gpk = w.gpk;
-        g.accumulate = !first;
-        g.M = M; g.N = N; g.K = K; g.Q = d.Q; g.inner = inner; g.block = 8;
-        TRY_(launch_quad_wgrad(g, act, st));
-        QuadBorder o{};
-        o.w = weight; o.dsum = dsum_v; o.dsum2 = dsum_g; o.gx = w.g[cur ^ 1];
-        if (with_border && k > 0) {  // with the sums of the norm that made this step's input
-            o.x_il4 = in; o.stats = in_stats; o.gamma = gamma; o.partials = w.partials; o.ggamma = ggamma; o.gbeta = gbeta; o.ac = w.ac;
-            o.accumulate = 1;
-        }
-        o.M = M; o.N = N; o.K = K; o.Q = d.Q; o.block = 8;
-        TRY_(launch_quad_border(o, st));
-    }
-    return launch_quad_finish(w.gpk, gw, gb, nullptr, w.g[cur], gx, B, M, N, K, 8, 2, st);
+    return gated_loop_backward(weight, bias, gamma, beta, x_il4, outs, Packed{}, stats, stashes, gy, gw, gb, ggamma, gbeta, gx, d, w, replay, act,
+                               (cudaStream_t)stream);
 }
 
 }  // extern "C"

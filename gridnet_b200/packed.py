@@ -23,10 +23,12 @@ _keep_packed = False
 
 
 def keep_packed(enabled: bool) -> bool:
-    """Whether differentiated calls keep 8-bit copies of activations for their backward pass, and compute their gradients at those copies:
-    the input of :class:`GridNorm`; gate and value of :func:`gated_scan`. Outputs are the
-    same with and without. Off by default. Holds for forward passes that start afterwards; a backward pass goes by what its forward
-    pass kept. Returns the previous setting."""
+    """Whether differentiated float32 calls keep 8-bit copies of activations for their backward passes, and compute their gradients at those copies:
+    the input of :class:`GridNorm`; the input of a step (:class:`Gridnet`, :class:`GatedGridnet`, with and without per-block normalisation);
+    of the loops of the models the input and every step's output; and, whatever the type, gate and value of :func:`gated_scan`. Steps and loops then
+    run their inner iterations again, from the copies, and keep none of them (:func:`keep_forward_stash`). Outputs are the same with and without.
+    Off by default. Holds for forward passes that start afterwards; a backward pass goes by what its forward pass kept. Returns the previous
+    setting."""
     global _keep_packed
     previous, _keep_packed = _keep_packed, bool(enabled)
     return previous

@@ -24,9 +24,10 @@ def stash_bytes(x, inner: int, block: int) -> int:
 
 
 def forward(plist, norm_weight, norm_bias, x, inner: int, outer: int, block: int, activation: str, ln_eps: float, residual: bool,
-            outs, stats, stashes):
+            outs, stats, stashes, done=None):
     """Runs the loop; ``outs``: a tensor like x per step for its raw output (residual: the next h), ``stats`` [outer, B, 2] for
-    the (mean, rstd) of outs[k] (residual: of the input of step k), ``stashes``: per step ``stash_bytes`` bytes or None."""
+    the (mean, rstd) of outs[k] (residual: of the input of step k), ``stashes``: per step ``stash_bytes`` bytes or None;
+    ``done``: called with every step's output when it is there."""
     B, M, N, K = x.shape
     P, act, st = M * N * K, activation_id(activation), torch.cuda.current_stream().cuda_stream
     y = torch.empty_like(x)
@@ -53,6 +54,8 @@ def forward(plist, norm_weight, norm_bias, x, inner: int, outer: int, block: int
         else:
             check(lib.gn_norm_finalize_f32(partials.data_ptr(), nparts, stats[k].data_ptr(), B, P, ln_eps, st))
         h = outs[k]
+        if done is not None:
+            done(h)
     if residual:
         return y.copy_(h)
     check(lib.gn_norm_apply_f32(h.data_ptr(), norm_weight.data_ptr(), norm_bias.data_ptr(), stats[outer - 1].data_ptr(), y.data_ptr(), B, P, st))

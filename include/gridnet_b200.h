@@ -546,6 +546,31 @@ GN_API int gn_norm_backward_packed_f32(const void *codes, const void *scales, co
                                        float *gx, float *ggamma, float *gbeta, int B, long long P, void *workspace,
                                        size_t workspace_bytes, void *stream);
 
+/* The loops with gradients (gn_loop_forward_f32, gn_gated_loop_forward_f32 and their backward calls) with 8-bit copies between the passes:
+ * packed is a host array of outer + 1 device pointers, gn_loop_packed_bytes each, 256-byte aligned: the input and the output of each
+ * step, groups of 32 neighbouring neurons of a sample (with residual the last one is not touched and may be NULL). The forward call
+ * computes what the other one does. The backward call computes the gradients with every step's input, and every norm's, as unpacked; the statistics
+ * are those of the forward pass, the inner iterations are run again. Other arguments as there. */
+GN_API size_t gn_loop_packed_bytes(int B, int M, int N, int K);
+GN_API size_t gn_loop_packed_workspace_bytes(int B, int M, int N, int K, int inner, int outer, int block, int residual, int gated,
+                                             int backward);
+GN_API int gn_loop_forward_packed_f32(const float *const *weights, const float *const *biases, const float *const *scales, int nparams,
+                                      const float *gamma, const float *beta, const float *x, float *y, void *const *packed, float *stats,
+                                      int B, int M, int N, int K, int inner, int outer, int block, float ln_eps, int activation,
+                                      int residual, void *workspace, size_t workspace_bytes, void *stream);
+GN_API int gn_loop_backward_packed_f32(const float *const *weights, const float *const *biases, const float *const *scales, int nparams,
+                                       const float *gamma, const float *beta, void *const *packed, const float *stats, const float *gy,
+                                       float *const *gw, float *const *gb, float *const *gs, float *ggamma, float *gbeta, float *gx,
+                                       int B, int M, int N, int K, int inner, int outer, int block, int activation, int residual,
+                                       void *workspace, size_t workspace_bytes, void *stream);
+GN_API int gn_gated_loop_forward_packed_f32(const float *weight, const float *bias, const float *gamma, const float *beta, const float *x,
+                                            float *y, void *const *packed, float *stats, int B, int M, int N, int K, int inner, int outer,
+                                            float ln_eps, int act, void *workspace, size_t workspace_bytes, void *stream);
+GN_API int gn_gated_loop_backward_packed_f32(const float *weight, const float *bias, const float *gamma, const float *beta,
+                                             void *const *packed, const float *stats, const float *gy, float *gw, float *gb,
+                                             float *ggamma, float *gbeta, float *gx, int B, int M, int N, int K, int inner, int outer,
+                                             int act, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------ gated scan
  * The update of the gated cell (gridnet/backend_torch.py:241-265) along a sequence, gate z and value u given, s the logistic function:
  *     h_t = s(z_t) h_{t-1} + s(-z_t) u_t,   h_0 = state (NULL: zeros)

@@ -150,3 +150,34 @@ def test_python_refusals_of_tensors_on_the_device():
         with pytest.raises((RuntimeError, AssertionError)) as e:
             call()
         assert "not refused" not in str(e.value)
+
+
+def test_packed_loop_errors():
+    from gridnet_b200._lib import lib
+
+    one = 256
+    assert lib.gn_loop_packed_bytes(5, 8, 8, 8) == 2 * 512 * 4 + 2 * 16 * 4 + 128 and lib.gn_loop_packed_bytes(0, 8, 8, 8) == 0
+    assert lib.gn_loop_packed_workspace_bytes(1, 8, 8, 12, 1, 1, 4, 0, 0, 0) == 0  # no multiple of 8
+    assert lib.gn_loop_forward_packed_f32(*[one] * 3, 1, *[one] * 6, 5, 8, 8, 8, 2, 3, 3, 1e-5, 2, 0, one, 1 << 40, None) == -2
+    assert lib.gn_loop_backward_packed_f32(*[one] * 3, 2, *[one] * 11, 5, 8, 8, 8, 2, 3, 8, 2, 0, one, 1 << 40, None) == -3  # sets of parameters
+    assert lib.gn_gated_loop_forward_packed_f32(*[one] * 8, 5, 8, 8, 8, 0, 3, 1e-5, 3, one, 1 << 40, None) == -5
+    assert lib.gn_gated_loop_backward_packed_f32(*[one] * 12, 5, 8, 8, 8, 2, 3, 9, one, 1 << 40, None) == -4
+
+
+@pytest.mark.gpu
+def test_packed_loop_workspaces():
+    """The library asks the device whether its kernels apply, so these need one; nothing is launched."""
+    from gridnet_b200._lib import lib
+
+    one = 256
+    need = lib.gn_loop_packed_workspace_bytes(5, 8, 8, 8, 2, 3, 8, 0, 0, 0)
+    fwd = lambda *work, packed=one: lib.gn_loop_forward_packed_f32(  # noqa: E731
+        one, one, one, 1, one, one, one, one, packed, one, 5, 8, 8, 8, 2, 3, 8, 1e-5, 2, 0, *work, None)
+    assert need > 0 and fwd(one, need - 1) == -6 and fwd(one + 8, need) == -6 and fwd(None, need) == -1 and fwd(one, need, packed=None) == -1
+    need = lib.gn_loop_packed_workspace_bytes(5, 8, 8, 8, 2, 3, 8, 0, 0, 1)
+    assert lib.gn_loop_backward_packed_f32(*[one] * 3, 1, *[one] * 11, 5, 8, 8, 8, 2, 3, 8, 2, 0, one, need - 1, None) == -6
+    need = lib.gn_loop_packed_workspace_bytes(5, 8, 8, 8, 2, 3, 8, 0, 1, 0)
+    assert lib.gn_gated_loop_forward_packed_f32(*[one] * 8, 5, 8, 8, 8, 2, 3, 1e-5, 3, one, need - 1, None) == -6
+    assert lib.gn_gated_loop_forward_packed_f32(*[one] * 6, None, one, 5, 8, 8, 8, 2, 3, 1e-5, 3, one, need, None) == -1
+    need = lib.gn_loop_packed_workspace_bytes(5, 8, 8, 8, 2, 3, 8, 0, 1, 1)
+    assert lib.gn_gated_loop_backward_packed_f32(*[one] * 12, 5, 8, 8, 8, 2, 3, 3, one, need - 1, None) == -6
