@@ -778,9 +778,10 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
     const bool vec = p.vec;
     auto rows_at = [&](long long t) { return (int)min((long long)S, max(0LL, now.q.len - t)); };
     auto ask_now = [&] {
-        from.turn_to(now.seq, now.q);
+        if (CHUNK) from.turn_to(now.seq, now.q);
         from.ask_for((now.tile << kFwdLog2) + warp * S, rows_at((now.tile << kFwdLog2) + warp * S));
     };
+    if (!CHUNK) from.turn_to(now.seq, now.q);
     if (more_to_come) ask_now();
     float2 carry = two(0.0f);
     if constexpr (CHUNK) {
@@ -886,9 +887,10 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
     const bool vec = p.vec;
     auto rows_at = [&](long long t) { return (int)min((long long)S, max(0LL, now.q.len - t)); };
     auto ask_now = [&] {
-        from.turn_to(now.seq, now.q);
+        if (CHUNK) from.turn_to(now.seq, now.q);
         from.ask_for((now.tile << kBwdLog2) + warp * S, rows_at((now.tile << kBwdLog2) + warp * S));
     };
+    if (!CHUNK) from.turn_to(now.seq, now.q);
     if (more_to_come) ask_now();
     float2 carry = two(0.0f);  // gradient of the state behind the steps in hand
     if constexpr (CHUNK) {
@@ -900,18 +902,19 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
         const long long t0 = (now.tile << kBwdLog2) + warp * S, at = (now.q.first + t0) * p.width + ch;
         const int cnt = rows_at(t0);
         float2 a[S], n[S], u[S], g[S], h = two(0.0f);
-        if constexpr (CHUNK) {
-            h = *plane(p, 1, now.row, slab);
-            carry = *plane(p, 2, now.row, slab);
-        } else {
-            if (now.tile > 0)
-                h = load2(p.bounds + tile_row<kBwdLog2>(p, now.seq, now.q, now.tile) * p.width + ch, vec, nch);
-            else if (p.state)
-                h = load2(p.state + (long long)now.seq * p.width + ch, vec, nch);
-        }
         from.take_from(t0, cnt, a, u, g);
+        const Cursor<kBwdLog2, CHUNK, true> here = now;
         more_to_come = now.next(p);
         if (more_to_come) ask_now();
+        if constexpr (CHUNK) {
+            h = *plane(p, 1, here.row, slab);
+            carry = *plane(p, 2, here.row, slab);
+        } else {
+            if (here.tile > 0)
+                h = load2(p.bounds + tile_row<kBwdLog2>(p, here.seq, here.q, here.tile) * p.width + ch, vec, nch);
+            else if (p.state)
+                h = load2(p.state + (long long)here.seq * p.width + ch, vec, nch);
+        }
         float2 A = two(1.0f), H = two(0.0f), C = two(0.0f);
         const bool special = farthest(a) >= kFar;
         if (!special) {
