@@ -22,7 +22,7 @@ from torch.autograd.function import once_differentiable
 
 from . import gridnet_cuda, patch_loop
 from ._lib import activation_id, check, lib
-from .packed import PackedActivations, empty_packed, keeps_packed, pack_activations, stream_of, unpack_activations
+from .packed import PackedActivations, keeps_packed, pack_activations, stream_of, unpack_activations
 
 
 def _assert_step_args(weight, bias, residual_scale, init_activations, block_size, gated):
@@ -200,7 +200,7 @@ class GridnetCudaOp(_Op):
         return (*grads, None, None, None, None, None)
 
 
-class GatedGridnetCudaOp(torch.autograd.Function):
+class GatedGridnetCudaOp(_Op):
     """One outer-loop step of the gated gridnet (gridnet/backend_cuda.py:111-190)."""
 
     @staticmethod
@@ -280,6 +280,17 @@ class GridNormOp(torch.autograd.Function):
         return gx, gg, gb, None
 
 
+@functools.lru_cache(maxsize=512)
+def _packed_norm_layout(B: int, P: int):
+    """Where scales, statistics and scratch start behind the codes, bytes in all, and those of the scratch."""
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    scales = up(B * P)
+    stats = scales + up(B * ((P + 31) // 32))
+    ws = stats + up(8 * B)
+    work = max(256, int(lib.gn_norm_packed_workspace_bytes(B, P)))
+    return (scales, stats, ws), ws + work, work
+
+
 class PackedGridNormOp(_Op):
     """:class:`GridNormOp` whose backward pass reads x from 8 bits (:func:`pack_activations`, groups along the grid of a sample): a
     quarter of the memory between the passes. The output is that of :class:`GridNormOp`; mean and deviation in the gradients are
@@ -295,28 +306,28 @@ class PackedGridNormOp(_Op):
             return GridNormOp.apply(x, gamma, beta, eps)
         B, P = x.shape[0], gamma.numel()
         y = torch.empty_like(x)
-        packed = empty_packed(x.shape, 1, x.dtype, x.device)
-        stats = torch.empty(B, 2, dtype=torch.float32, device=x.device)
-        ws = _workspace(lib.gn_norm_packed_workspace_bytes(B, P), x.device)
+        at, kept_bytes, work = _packed_norm_layout(B, P)
+        # codes, scales, statistics and the forward pass's scratch in one allocation
+        kept = torch.empty(kept_bytes, dtype=torch.uint8, device=x.device)
+        codes = kept.data_ptr()
         with torch.cuda.device(x.device):
-            check(lib.gn_norm_forward_packed_f32(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), stats.data_ptr(),
-                                                 packed.codes.data_ptr(), packed.scales.data_ptr(), B, P, float(eps), ws.data_ptr(), ws.numel(),
-                                                 stream_of(x)))
-        ctx.save_for_backward(packed.codes, packed.scales, stats, gamma)
+            check(lib.gn_norm_forward_packed_f32(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), codes + at[1], codes, codes + at[0],
+                                                 B, P, float(eps), codes + at[2], work, stream_of(x)))
+        ctx.save_for_backward(kept, gamma)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        codes, scales, stats, gamma = ctx.saved_tensors
+        kept, gamma = ctx.saved_tensors
         grad_y = grad_y.contiguous()
-        B, P = codes.shape[0], gamma.numel()
+        B, P = grad_y.shape[0], gamma.numel()
         gx, gg, gb = torch.empty_like(grad_y), torch.empty_like(gamma), torch.empty_like(gamma)
-        ws = _workspace(lib.gn_norm_packed_workspace_bytes(B, P), grad_y.device)
+        at, _, work = _packed_norm_layout(B, P)
+        codes, ws = kept.data_ptr(), torch.empty(work, dtype=torch.uint8, device=grad_y.device)
         with torch.cuda.device(grad_y.device):
-            check(lib.gn_norm_backward_packed_f32(codes.data_ptr(), scales.data_ptr(), stats.data_ptr(), gamma.data_ptr(), grad_y.data_ptr(),
-                                                  gx.data_ptr(), gg.data_ptr(), gb.data_ptr(), B, P, ws.data_ptr(), ws.numel(),
-                                                  stream_of(grad_y)))
+            check(lib.gn_norm_backward_packed_f32(codes, codes + at[0], codes + at[1], gamma.data_ptr(), grad_y.data_ptr(), gx.data_ptr(),
+                                                  gg.data_ptr(), gb.data_ptr(), B, P, ws.data_ptr(), work, stream_of(grad_y)))
         return gx, gg, gb, None
 
 

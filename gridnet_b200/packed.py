@@ -60,16 +60,6 @@ def stream_of(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
-def empty_packed(shape, rows: int, dtype: torch.dtype, device) -> PackedActivations:
-    """Room for the packed copy of a tensor of this shape, groups along what is behind its first ``rows`` dimensions."""
-    cols = 1
-    for n in shape[rows:]:
-        cols *= n
-    return PackedActivations(torch.empty(shape, dtype=torch.int8, device=device),
-                             torch.empty(*shape[:rows], (cols + GROUP - 1) // GROUP, dtype=torch.uint8, device=device), dtype)
-
-
-@torch.no_grad()
 def pack_activations(x: torch.Tensor, rows: int = 1) -> PackedActivations:
     """The packed copy of ``x`` (float32, bfloat16 or float16, on a CUDA device). The first ``rows`` dimensions count rows (a sample, a
     step of a sequence); groups of 32 run along the others taken together and never across a row's end."""
@@ -77,16 +67,15 @@ def pack_activations(x: torch.Tensor, rows: int = 1) -> PackedActivations:
         raise GridnetB200Error("x must be a CUDA tensor")
     dtype = dtype_id(x, "x")
     assert 0 <= rows <= x.dim(), f"{rows=} invalid for {x.shape=}"
-    x = x.contiguous()
-    packed = empty_packed(x.shape, rows, x.dtype, x.device)
-    nrows = x.shape[:rows].numel()
+    x = x.detach().contiguous()
+    nrows, cols = x.shape[:rows].numel(), x.shape[rows:].numel()
+    codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scales = torch.empty((*x.shape[:rows], (cols + GROUP - 1) // GROUP), dtype=torch.uint8, device=x.device)
     with torch.cuda.device(x.device):
-        check(lib.gn_pack8(x.data_ptr(), packed.codes.data_ptr(), packed.scales.data_ptr(), nrows, x.numel() // nrows if nrows else 0, dtype,
-                           stream_of(x)))
-    return packed
+        check(lib.gn_pack8(x.data_ptr(), codes.data_ptr(), scales.data_ptr(), nrows, cols, dtype, stream_of(x)))
+    return PackedActivations(codes, scales, x.dtype)
 
 
-@torch.no_grad()
 def unpack_activations(packed: PackedActivations, out: torch.Tensor | None = None) -> torch.Tensor:
     """What the packed copy stands for, in the tensor's own type or in ``out``'s (contiguous, any of the three types)."""
     codes, scales, dtype = packed

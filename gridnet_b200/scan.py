@@ -13,7 +13,7 @@ from torch.autograd.function import once_differentiable
 
 from ._lib import GridnetB200Error, check, lib
 from .backend_cuda import _Op
-from .packed import DTYPES, dtype_id, empty_packed, keeps_packed, stream_of
+from .packed import DTYPES, GROUP, dtype_id, keeps_packed, stream_of
 
 
 def _rows(t: torch.Tensor, lead: int) -> torch.Tensor:
@@ -84,6 +84,19 @@ def _device_offsets(offsets, total: int, device):
     return offsets.to(device=device, dtype=torch.int64).contiguous()
 
 
+def _packed_at(total: int, width: int):
+    """Codes of the gate, of the value, scales of the gate, of the value in one allocation: where each starts, and the end."""
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    codes, scales = up(total * width), up(total * ((width + GROUP - 1) // GROUP))
+    return 0, codes, 2 * codes, 2 * codes + scales, 2 * (codes + scales)
+
+
+def _packed_places(memory: torch.Tensor, total: int, width: int):
+    """Addresses of the gate's codes and scales and the value's."""
+    base, at = memory.data_ptr(), _packed_at(total, width)
+    return base, base + at[2], base + at[1], base + at[3]
+
+
 def _forward(gate, value, state, offsets, kept_packed: bool, need_grad: bool):
     """(h, last), and what the backward pass needs: the tensors to save and the sizes."""
     n, steps, total = _check_scan(gate, value, state, offsets)
@@ -97,19 +110,20 @@ def _forward(gate, value, state, offsets, kept_packed: bool, need_grad: bool):
     left, scratch = _sizes(dev.index, *size)[:2]
     h = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
     last = torch.empty((n, *gate.shape[lead:]), dtype=torch.float32, device=dev)
-    codes, bounds = (None, None, None, None), None
+    codes, bounds, packed = (None,) * 4, None, None
     if need_grad and kept_packed:
-        codes = [t for x in (z, u) for t in empty_packed(x.shape, lead, x.dtype, dev)[:2]]
+        packed = torch.empty(max(1, _packed_at(total, width)[-1]), dtype=torch.uint8, device=dev)
+        codes = _packed_places(packed, total, width)
     elif need_grad:
         bounds = _scratch(left, dev)
     work = _scratch(scratch, dev)
     with torch.cuda.device(dev):
-        check(lib.gn_gated_scan_forward(z.data_ptr(), u.data_ptr(), _ptr(s), _ptr(offsets), h.data_ptr(), last.data_ptr(), *map(_ptr, codes),
+        check(lib.gn_gated_scan_forward(z.data_ptr(), u.data_ptr(), _ptr(s), _ptr(offsets), h.data_ptr(), last.data_ptr(), *codes,
                                         _ptr(bounds), n, steps, total, width, *_strides(z), *_strides(u), dtype, _ptr(work), scratch,
                                         stream_of(gate)))
-    if codes[0] is not None:
-        return h, last, (codes[0], codes[2], codes[1], codes[3], s, offsets, None), size
-    return h, last, (z, u, None, None, s, offsets, bounds), size
+    if packed is not None:
+        return h, last, (packed, None, s, offsets, None), size
+    return h, last, (z, u, s, offsets, bounds), size
 
 
 class GatedScanOp(_Op):
@@ -126,17 +140,22 @@ class GatedScanOp(_Op):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_h, grad_last):
-        z, u, z_scales, u_scales, s, offsets, bounds = ctx.saved_tensors
-        size, dev, packed = ctx.size, z.device, z_scales is not None
+        z, u, s, offsets, bounds = ctx.saved_tensors
+        size, dev, packed = ctx.size, z.device, u is None
         grad_h = torch.zeros(ctx.shape, dtype=ctx.dtype, device=dev) if grad_h is None else grad_h.contiguous()
         grad_last = None if grad_last is None else grad_last.contiguous()
         dz, du = torch.empty(ctx.shape, dtype=ctx.dtype, device=dev), torch.empty(ctx.shape, dtype=ctx.dtype, device=dev)
         ds = torch.empty_like(s) if s is not None and ctx.needs_input_grad[2] else None
-        strides = (0, 0, 0, 0) if packed else (*_strides(z), *_strides(u))
+        if packed:
+            z_at, z_scales, u_at, u_scales = _packed_places(z, size[2], size[3])
+            strides = (0, 0, 0, 0)
+        else:
+            z_at, u_at, z_scales, u_scales = z.data_ptr(), u.data_ptr(), None, None
+            strides = (*_strides(z), *_strides(u))
         scratch = _sizes(dev.index, *size)[2 + packed]
         work = _scratch(scratch, dev)
         with torch.cuda.device(dev):
-            check(lib.gn_gated_scan_backward(z.data_ptr(), u.data_ptr(), _ptr(z_scales), _ptr(u_scales), _ptr(s), _ptr(offsets), _ptr(bounds),
+            check(lib.gn_gated_scan_backward(z_at, u_at, z_scales, u_scales, _ptr(s), _ptr(offsets), _ptr(bounds),
                                              grad_h.data_ptr(), _ptr(grad_last), dz.data_ptr(), du.data_ptr(), _ptr(ds), *size[:4], *strides,
                                              size[4], _ptr(work), scratch, stream_of(z)))
         return dz, du, ds, None, None

@@ -89,6 +89,12 @@ def test_shapes_and_rows():
     # an odd address
     flat = torch.randn(1 + 6 * 40, device="cuda")[1:].view(6, 40)
     assert np.array_equal(gb.pack_activations(flat).codes.cpu().numpy(), pack(flat.cpu().numpy())[0])
+    for kind in TYPES.values():
+        flat = torch.randn(1 + 6 * 64, device="cuda").to(kind)[1:].view(6, 64)
+        p = gb.pack_activations(flat)
+        assert np.array_equal(p.codes.cpu().numpy(), pack(flat.float().cpu().numpy())[0])
+        out = torch.zeros(1 + 6 * 64, device="cuda", dtype=kind)[1:].view(6, 64)
+        assert torch.equal(gb.unpack_activations(p, out=out), gb.unpack_activations(p))
     for shape in ((0, 5), (5, 0)):
         e = torch.empty(shape, device="cuda")
         assert gb.unpack_activations(gb.pack_activations(e)).shape == shape

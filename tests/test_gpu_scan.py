@@ -313,6 +313,68 @@ def test_captured_replayed_and_on_another_stream():
             assert all(torch.equal(a, b) and torch.equal(b, c) for a, b, c in zip(outs, want, beside))
 
 
+@pytest.mark.parametrize("shape,ragged", [((2, 2100, 40), None), ((1, 3000, 72), [0, 5, 5, 1900, 3000]), ((160, 300, 64), None)])
+def test_captured_by_chunks_and_as_a_walk(shape, ragged):
+    """Long sequences in three kernels, many in one: replayed twice in a row, the second time on other inputs."""
+    import gridnet_b200 as gb
+
+    gen = torch.Generator().manual_seed(5)
+    total = shape[0] * shape[1]
+    offsets = None if ragged is None else torch.tensor(ragged, device="cuda")
+    kind = shape if ragged is None else (total, shape[2])
+    n = shape[0] if ragged is None else len(ragged) - 1
+    make = lambda: [torch.randn(*s, generator=gen).cuda() for s in (kind, kind, (n, shape[2]), kind, (n, shape[2]))]  # noqa: E731
+
+    def run(z, u, h0, g, gl, packed):
+        z, u, h0 = (t.detach().requires_grad_(True) for t in (z, u, h0))
+        h, last = gb.gated_scan(z, u, h0, offsets, packed=packed)
+        return [h, last, *torch.autograd.grad([h, last], (z, u, h0), [g, gl])]
+
+    for packed in (False, True):
+        static, new = make(), make()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(*static, packed)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = run(*static, packed)
+        graph.replay()
+        for a, b in zip(static, new):
+            a.copy_(b)
+        graph.replay()
+        want = run(*new, packed)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("n,steps", [(1, 600000), (4, 150000)])
+def test_places_past_32_bits(n, steps):
+    """2.4e9 values, as chunks and as a walk: the last sequence's end, behind a reset, is what the end alone is."""
+    import gridnet_b200 as gb
+
+    width, tail = 4096, 200
+    z = torch.zeros(n, steps, width, dtype=torch.bfloat16, device="cuda")
+    u = torch.ones_like(z)
+    g = torch.zeros_like(z)
+    z[-1, -tail:], u[-1, -tail:], g[-1, -tail:] = (torch.randn(tail, width, device="cuda") for _ in range(3))
+    z[-1, -tail] = float("-inf")
+    for packed in (False, True):
+        leaves, short = ([t.detach().requires_grad_(True) for t in pair] for pair in ((z, u), (z[-1:, -tail:].clone(), u[-1:, -tail:].clone())))
+        h, last = gb.gated_scan(*leaves, packed=packed)
+        grads = torch.autograd.grad(h, leaves, g)
+        h2, last2 = gb.gated_scan(*short, packed=packed)
+        grads2 = torch.autograd.grad(h2, short, g[-1:, -tail:])
+        # runs of steps are put together in other places: a few units of float32 each, then at most one step of bfloat16 apart
+        for a, b in ((h[-1, -tail:], h2[0]), *((x[-1, -tail:], y[0]) for x, y in zip(grads, grads2))):
+            assert ((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 1e-6).all()
+        assert torch.allclose(last[-1], last2[0], rtol=1e-5, atol=1e-5)
+        assert (h[0, 1000].float() - 1).abs().max() < 1e-2 or n == 1
+        del h, last, grads, leaves
+    del z, u, g
+
+
 def test_the_same_bits_every_time_and_two_graphs_alive():
     import gridnet_b200 as gb
 
