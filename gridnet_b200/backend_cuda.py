@@ -22,7 +22,7 @@ from torch.autograd.function import once_differentiable
 
 from . import gridnet_cuda, patch_loop
 from ._lib import activation_id, check, lib
-from .packed import PackedActivations, keeps_packed, pack_activations, stream_of, unpack_activations
+from .packed import PackedActivations, keeps_packed, on_device, pack_activations, stream_of, unpack_activations
 
 
 def _assert_step_args(weight, bias, residual_scale, init_activations, block_size, gated):
@@ -310,7 +310,7 @@ class PackedGridNormOp(_Op):
         # codes, scales, statistics and the forward pass's scratch in one allocation
         kept = torch.empty(kept_bytes, dtype=torch.uint8, device=x.device)
         codes = kept.data_ptr()
-        with torch.cuda.device(x.device):
+        with on_device(x.device):
             check(lib.gn_norm_forward_packed_f32(x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), codes + at[1], codes, codes + at[0],
                                                  B, P, float(eps), codes + at[2], work, stream_of(x)))
         ctx.save_for_backward(kept, gamma)
@@ -325,7 +325,7 @@ class PackedGridNormOp(_Op):
         gx, gg, gb = torch.empty_like(grad_y), torch.empty_like(gamma), torch.empty_like(gamma)
         at, _, work = _packed_norm_layout(B, P)
         codes, ws = kept.data_ptr(), torch.empty(work, dtype=torch.uint8, device=grad_y.device)
-        with torch.cuda.device(grad_y.device):
+        with on_device(grad_y.device):
             check(lib.gn_norm_backward_packed_f32(codes, codes + at[0], codes + at[1], gamma.data_ptr(), grad_y.data_ptr(), gx.data_ptr(),
                                                   gg.data_ptr(), gb.data_ptr(), B, P, ws.data_ptr(), work, stream_of(grad_y)))
         return gx, gg, gb, None

@@ -19,9 +19,9 @@
 // a round of tiles, slower than the chunks (4 x 4097 x 1024 float32, backward from packed copies, 157 us).
 //
 // Steps whose n_t is 0 (gates from about 104 up, and +inf) do not look at their value, which may be NaN; steps whose a_t is 0 do not look
-// at the state. Anything else that is not finite stays in the state. Threads that hold such a step (the smaller of a_t and n_t is 0) go
-// through the steps with selections, all others with products and sums alone. A run with a reset has the sign bit in A (-0): an A that became
-// +0 by underflow still passes on a state that is not finite.
+// at the state. Anything else that is not finite stays in the state. Threads that hold a gate beyond 80 select while they compute the gates,
+// those that hold a reset (a_t = 0) also while they go through the steps; all others have products and sums alone. A run with a reset has the
+// sign bit in A (-0): an A that became +0 by underflow still passes on a state that is not finite.
 //
 // A thread has two channels, so that a row is read 64 channels at a time and arithmetic is on pairs (f32x2); a warp has a run of steps
 // of its own, no lane has to know another lane's.
@@ -86,7 +86,7 @@ __device__ __forceinline__ long long tile_row(const Scan &p, int seq, const Plac
     if (!p.offsets) return seq * ((p.steps + (1 << LOG2) - 1) >> LOG2) + k;
     return (s.first >> LOG2) + seq + k;  // a sequence has at most one tile more than its rows have multiples of a tile
 }
-// and the other way round; false where the row belongs to no tile
+// and the other way round; false where the row belongs to no tile. All lanes of a warp call with the same row
 template <int LOG2>
 __device__ __forceinline__ bool tile_of_row(const Scan &p, long long row, int &seq, Place &s, long long &k)
 {
@@ -97,13 +97,15 @@ __device__ __forceinline__ bool tile_of_row(const Scan &p, long long row, int &s
         k = row - seq * tiles;
         return true;
     }
-    int lo = 0, hi = p.n;  // the last sequence that starts at this row or before
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if ((min(max(p.offsets[mid], 0LL), p.total) >> LOG2) + mid <= row)
-            lo = mid;
-        else
-            hi = mid;
+    // the last sequence that starts at this row or before: 32 places at a time, a lane each (n <= 1024: two loads one after the other)
+    const int lane = threadIdx.x & 31;
+    int lo = 0;
+    for (int left = p.n; left > 1;) {
+        const int step = (left + 31) / 32, at = lo + lane * step;
+        const bool before = lane * step < left && (min(max(p.offsets[min(at, p.n)], 0LL), p.total) >> LOG2) + at <= row;
+        const int found = max(__popc(__ballot_sync(0xffffffffu, before)) - 1, 0);
+        lo += found * step;
+        left = min(step, left - found * step);
     }
     seq = lo;
     s = sequence(p, seq);
@@ -493,6 +495,32 @@ __device__ __forceinline__ void take_packed(const Rows<unsigned char, S> &gates,
         }
 }
 
+// All gates of a thread's steps: z becomes s(z), and a value that is not looked at 0. Returns what there is
+enum { kNear, kFarGates, kResets };
+template <int S>
+__device__ __forceinline__ int gates_of(float2 (&z)[S], float2 (&n)[S], float2 (&u)[S])
+{
+    if (farthest(z) < kFar) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            float2 a;
+            gates(z[s], a, n[s]);
+            z[s] = a;
+        }
+        return kNear;
+    }
+    float least = 1.0f;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        float2 a;
+        gates_any(z[s], a, n[s]);
+        z[s] = a;
+        u[s] = looked_at(n[s], u[s]);
+        least = fminf(least, fminf(a.x, a.y));
+    }
+    return least == 0.0f ? kResets : kFarGates;
+}
+
 // What a warp's, a CTA's steps amount to: (A, H) and, backward, (A, C) of a channel pair; two copies, so that one barrier lies between
 // writing and writing again
 __device__ __forceinline__ float4 map_of(float2 A, float2 H) { return make_float4(A.x, A.y, H.x, H.y); }
@@ -642,22 +670,19 @@ __global__ void __launch_bounds__(kScanThreads, 7) scan_maps_k(const Scan p)
         float2 z[S], u[S], g[BACKWARD ? S : 1];
         from.take_from(t, min(S, rows), z, u, g);
         from.ask_for(t + S, min(S, rows - S));
-        if (farthest(z) < kFar) {
+        float2 n[S];
+        if (gates_of(z, n, u) != kResets && !resets(A.x) && !resets(A.y)) {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                float2 a, n;
-                gates(z[s], a, n);
-                H = fma2(a, H, mul2(n, u[s]));
-                A = product(A, a);
-                if constexpr (BACKWARD) C = make_float2(resets(A.x) ? C.x : fmaf(A.x, g[s].x, C.x), resets(A.y) ? C.y : fmaf(A.y, g[s].y, C.y));
+                H = fma2(z[s], H, mul2(n[s], u[s]));
+                A = mul2(A, z[s]);
+                if constexpr (BACKWARD) C = fma2(A, g[s], C);
             }
         } else {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                float2 a, n;
-                gates_any(z[s], a, n);
-                H = after(a, H, mul2(n, looked_at(n, u[s])));
-                A = more(A, a);
+                H = after(z[s], H, mul2(n[s], u[s]));
+                A = more(A, z[s]);
                 if constexpr (BACKWARD) C = make_float2(resets(A.x) ? C.x : fmaf(A.x, g[s].x, C.x), resets(A.y) ? C.y : fmaf(A.y, g[s].y, C.y));
             }
         }
@@ -804,27 +829,25 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
             const PackTo to = {p.pack_gate, p.pack_value, p.pack_gate_scales, p.pack_value_scales};
             pack_rows(a, b, to, first + t0, p.width, ch, vec && from.left >= kSlab && cnt == S, cnt, nch);
         }
-        const bool special = farthest(a) >= kFar;
         float2 A = two(1.0f), H = two(0.0f);
+        bool special;
+        {
+            float2 n[S];
+            special = gates_of(a, n, b) == kResets;
+#pragma unroll
+            for (int s = 0; s < S; ++s) b[s] = mul2(n[s], b[s]);
+        }
         if (!special) {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                float2 w, n;
-                gates(a[s], w, n);
-                a[s] = w;
-                b[s] = mul2(n, b[s]);
-                H = fma2(w, H, b[s]);
-                A = mul2(A, w);
+                H = fma2(a[s], H, b[s]);
+                A = mul2(A, a[s]);
             }
         } else {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                float2 w, n;
-                gates_any(a[s], w, n);
-                a[s] = w;
-                b[s] = mul2(n, looked_at(n, b[s]));
-                H = after(w, H, b[s]);
-                A = more(A, w);
+                H = after(a[s], H, b[s]);
+                A = more(A, a[s]);
             }
         }
         ex.warp[par][0][warp][lane] = map_of(A, H);
@@ -916,26 +939,20 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
                 h = load2(p.state + (long long)here.seq * p.width + ch, vec, nch);
         }
         float2 A = two(1.0f), H = two(0.0f), C = two(0.0f);
-        const bool special = farthest(a) >= kFar;
+        const int kind = gates_of(a, n, u);
+        const bool special = kind == kResets;
         if (!special) {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                float2 w;
-                gates(a[s], w, n[s]);
-                a[s] = w;
-                H = fma2(w, H, mul2(n[s], u[s]));
-                A = mul2(A, w);
+                H = fma2(a[s], H, mul2(n[s], u[s]));
+                A = mul2(A, a[s]);
                 C = fma2(A, g[s], C);
             }
         } else {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
-                float2 w;
-                gates_any(a[s], w, n[s]);
-                a[s] = w;
-                u[s] = looked_at(n[s], u[s]);
-                H = after(w, H, mul2(n[s], u[s]));
-                A = more(A, w);
+                H = after(a[s], H, mul2(n[s], u[s]));
+                A = more(A, a[s]);
                 C = make_float2(resets(A.x) ? C.x : fmaf(A.x, g[s].x, C.x), resets(A.y) ? C.y : fmaf(A.y, g[s].y, C.y));
             }
         }
@@ -959,7 +976,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
             for (int w = 0; w < warp; ++w) h = through(ex.warp[par][0][w][lane], h);
         }
         // u becomes a n (h before the step - u), then both gradients in place of g and u
-        if (!special) {
+        if (kind == kNear) {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
                 const float2 d = fma2(u[s], two(-1.0f), h);
@@ -1008,21 +1025,30 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
 }
 
 // ------------------------------------------------------------------ one step
+// Four channels of a thread; quads: vectors of four lie on whole vectors' addresses
 template <typename T>
 __global__ void __launch_bounds__(256) scan_step_k(const T *__restrict__ gate, const T *__restrict__ value, const float *state, T *__restrict__ h,
-                                                   float *out_state, long long rows, int width, long long gate_row, long long value_row, int vec)
+                                                   float *out_state, long long rows, int width, long long gate_row, long long value_row, int quads)
 {
-    const int pairs = (width + 1) / 2;
+    const int of_row = (width + 3) / 4;
     const long long stride = (long long)gridDim.x * blockDim.x;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < rows * pairs; i += stride) {
-        const long long row = i / pairs;
-        const int ch = (int)(i - row * pairs) * 2, nch = min(2, width - ch);
-        float2 a, n;
-        gates_any(load2(gate + row * gate_row + ch, vec, nch), a, n);
-        const float2 u = looked_at(n, load2(value + row * value_row + ch, vec, nch));
-        const float2 s = after(a, load2(state + row * width + ch, vec, nch), mul2(n, u));
-        store2(h + row * width + ch, vec, nch, s);
-        store2(out_state + row * width + ch, vec, nch, s);
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < rows * of_row; i += stride) {
+        const long long row = rows * of_row <= 0xffffffffLL ? (long long)((unsigned)i / (unsigned)of_row) : i / of_row;
+        const int ch = (int)(i - row * of_row) * 4, nch = min(4, width - ch);
+        float z[4], u[4], s[4];
+        load4(gate + row * gate_row + ch, quads, nch, z);
+        load4(value + row * value_row + ch, quads, nch, u);
+        load4(state + row * width + ch, quads, nch, s);
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+            float2 a, n;
+            gates_any(make_float2(z[k], z[k + 1]), a, n);
+            const float2 r = after(a, make_float2(s[k], s[k + 1]), mul2(n, looked_at(n, make_float2(u[k], u[k + 1]))));
+            s[k] = r.x;
+            s[k + 1] = r.y;
+        }
+        store4(h + row * width + ch, quads, nch, s);
+        store4(out_state + row * width + ch, quads, nch, s);
     }
 }
 
@@ -1233,20 +1259,20 @@ GN_API int gn_gated_scan_step(const void *gate, const void *value, const float *
     if (rows == 0) return GN_OK;
     if (!gate || !value || !state || !h || !out_state) return GN_ERR_NULL_POINTER;
     const int size = dtype == GN_F32 ? 4 : 2;
-    const int vec = width % 2 == 0 && gate_row % 2 == 0 && value_row % 2 == 0 && aligned(gate, 2 * size) && aligned(value, 2 * size) &&
-                    aligned(h, 2 * size) && aligned(state, 8) && aligned(out_state, 8);
-    const long long want = (rows * ((width + 1) / 2) + 255) / 256, most = 16LL * sm_count();
+    const int quads = width % 4 == 0 && gate_row % 4 == 0 && value_row % 4 == 0 && aligned(gate, 4 * size) && aligned(value, 4 * size) &&
+                      aligned(h, 4 * size) && aligned(state, 16) && aligned(out_state, 16);
+    const long long want = (rows * ((width + 3) / 4) + 255) / 256, most = 32LL * sm_count();
     const unsigned blocks = (unsigned)(want < most ? want : most);
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == GN_F32)
         scan_step_k<float><<<blocks, 256, 0, st>>>((const float *)gate, (const float *)value, state, (float *)h, out_state, rows, width, gate_row,
-                                                   value_row, vec);
+                                                   value_row, quads);
     else if (dtype == GN_BF16)
         scan_step_k<__nv_bfloat16><<<blocks, 256, 0, st>>>((const __nv_bfloat16 *)gate, (const __nv_bfloat16 *)value, state, (__nv_bfloat16 *)h,
-                                                           out_state, rows, width, gate_row, value_row, vec);
+                                                           out_state, rows, width, gate_row, value_row, quads);
     else
         scan_step_k<__half><<<blocks, 256, 0, st>>>((const __half *)gate, (const __half *)value, state, (__half *)h, out_state, rows, width,
-                                                    gate_row, value_row, vec);
+                                                    gate_row, value_row, quads);
     return check_launch("gated_scan_step");
 }
 

@@ -13,7 +13,7 @@ from torch.autograd.function import once_differentiable
 
 from ._lib import GridnetB200Error, check, lib
 from .backend_cuda import _Op
-from .packed import DTYPES, GROUP, dtype_id, keeps_packed, stream_of
+from .packed import DTYPES, GROUP, dtype_id, keeps_packed, on_device, stream_of
 
 
 def _rows(t: torch.Tensor, lead: int) -> torch.Tensor:
@@ -117,7 +117,7 @@ def _forward(gate, value, state, offsets, kept_packed: bool, need_grad: bool):
     elif need_grad:
         bounds = _scratch(left, dev)
     work = _scratch(scratch, dev)
-    with torch.cuda.device(dev):
+    with on_device(dev):
         check(lib.gn_gated_scan_forward(z.data_ptr(), u.data_ptr(), _ptr(s), _ptr(offsets), h.data_ptr(), last.data_ptr(), *codes,
                                         _ptr(bounds), n, steps, total, width, *_strides(z), *_strides(u), dtype, _ptr(work), scratch,
                                         stream_of(gate)))
@@ -154,7 +154,7 @@ class GatedScanOp(_Op):
             strides = (*_strides(z), *_strides(u))
         scratch = _sizes(dev.index, *size)[2 + packed]
         work = _scratch(scratch, dev)
-        with torch.cuda.device(dev):
+        with on_device(dev):
             check(lib.gn_gated_scan_backward(z_at, u_at, z_scales, u_scales, _ptr(s), _ptr(offsets), _ptr(bounds),
                                              grad_h.data_ptr(), _ptr(grad_last), dz.data_ptr(), du.data_ptr(), _ptr(ds), *size[:4], *strides,
                                              size[4], _ptr(work), scratch, stream_of(z)))
@@ -180,14 +180,13 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor | No
     if offsets is not None and not isinstance(offsets, torch.Tensor):
         offsets = torch.as_tensor(offsets, dtype=torch.int64)
     if not (torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or (state is not None and state.requires_grad))):
-        return _forward(gate.detach(), value.detach(), state, offsets, False, False)[:2]
+        return _forward(gate, value, state, offsets, False, False)[:2]
     return GatedScanOp.apply(gate, value, state, offsets, keeps_packed() if packed is None else bool(packed))
 
 
 def gated_scan_step(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor, out_state: torch.Tensor | None = None):
     """One step of :func:`gated_scan` without gradients: ``gate`` and ``value`` [batch, ...], ``state`` [batch, ...] float32. Returns
     ``(h, new_state)``; ``out_state`` (which may be ``state``) receives the new state."""
-    gate, value, state = gate.detach(), value.detach(), state.detach()
     for name, t in (("gate", gate), ("value", value), ("state", state)):
         if not t.is_cuda:
             raise GridnetB200Error(f"{name} must be a CUDA tensor")
@@ -208,7 +207,7 @@ def gated_scan_step(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor
         if not out_state.is_contiguous():
             raise GridnetB200Error("out_state must be contiguous")
     h = torch.empty(shape, dtype=gate.dtype, device=dev)
-    with torch.cuda.device(dev):
+    with on_device(dev):
         check(lib.gn_gated_scan_step(z.data_ptr(), u.data_ptr(), s.data_ptr(), h.data_ptr(), out_state.data_ptr(), rows, width, z.stride(0),
                                      u.stride(0), dtype, stream_of(gate)))
     return h, out_state
