@@ -718,44 +718,42 @@ __global__ void __launch_bounds__(8 * kStartRuns) scan_starts_k(const Scan p)
     const long long state_at = (long long)seq * p.width + ch, tiles = (q.len + (1 << kLog2) - 1) >> kLog2, row = tile_row<kLog2>(p, seq, q, 0);
     const long long per = (tiles + all_runs - 1) / all_runs, lo = min(tiles, run * per), hi = min(tiles, lo + per);
     auto at = [&](int way, long long k) { return reinterpret_cast<float2 *>(p.maps + (way * p.map_rows + row + k) * p.padded + ch); };
-    float2 A = two(1.0f), H = two(0.0f), C = two(0.0f);
-    for (long long k = lo; k < hi; k += kBatch) {
-        float2 a[kBatch], h[kBatch], c[kBatch];
+    float2 a[kBatch], b[kBatch], c[kBatch];  // maps of eight tiles at a time
+    auto load = [&](long long k) {
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             const long long j = min(k + i, hi - 1);
             a[i] = *at(0, j);
-            h[i] = *at(1, j);
+            b[i] = *at(1, j);
             if (BACKWARD) c[i] = *at(2, j);
         }
+    };
+    const bool one_batch = per <= kBatch;  // loaded once
+    float2 A = two(1.0f), H = two(0.0f), C = two(0.0f);
+    for (long long k = lo; k < hi; k += kBatch) {
+        load(k);
 #pragma unroll
         for (int i = 0; i < kBatch; ++i)
             if (k + i < hi) {
                 if (BACKWARD) C = make_float2(resets(A.x) ? C.x : fmaf(A.x, c[i].x, C.x), resets(A.y) ? C.y : fmaf(A.y, c[i].y, C.y));
-                H = through(a[i], H, h[i]);
+                H = through(a[i], H, b[i]);
                 A = product(A, a[i]);
             }
     }
     runs[0][run][lane] = map_of(A, H);
     if (BACKWARD) runs[BACKWARD][run][lane] = map_of(A, C);
     __syncthreads();
-    float2 h = two(0.0f), c = two(0.0f);
+    float2 h = two(0.0f), g = two(0.0f);  // the state ahead of the run, the gradient behind it
     if (p.state) h = load2(p.state + state_at, p.vec, nch);
     if (!BACKWARD && tiles == 0 && run == 0 && p.last) store2(p.last + state_at, p.vec, nch, h);
     const int used = per > 0 ? (int)((tiles + per - 1) / per) : 0;  // runs that have tiles
     for (int r = 0; r < min(run, used); ++r) h = through(runs[0][r][lane], h);
     if (BACKWARD) {
-        if (p.glast) c = load2(p.glast + state_at, p.vec, nch);
-        for (int r = used - 1; r > run; --r) c = through(runs[BACKWARD][r][lane], c);
+        if (p.glast) g = load2(p.glast + state_at, p.vec, nch);
+        for (int r = used - 1; r > run; --r) g = through(runs[BACKWARD][r][lane], g);
     }
     for (long long k = lo; k < hi; k += kBatch) {
-        float2 a[kBatch], b[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const long long j = min(k + i, hi - 1);
-            a[i] = *at(0, j);
-            b[i] = *at(1, j);
-        }
+        if (!one_batch) load(k);
 #pragma unroll
         for (int i = 0; i < kBatch; ++i)
             if (k + i < hi) {
@@ -764,22 +762,16 @@ __global__ void __launch_bounds__(8 * kStartRuns) scan_starts_k(const Scan p)
             }
     }
     if (BACKWARD) {
-        for (long long k = hi - 1; k >= lo; k -= kBatch) {
-            float2 a[kBatch], b[kBatch];
+        for (long long k = lo + (hi - 1 - lo) / kBatch * kBatch; k >= lo && lo < hi; k -= kBatch) {
+            if (!one_batch) load(k);  // the states have gone into plane 1 by now, and b is not looked at any more
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const long long j = max(k - i, lo);
-                a[i] = *at(0, j);
-                b[i] = *at(2, j);
-            }
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i)
-                if (k - i >= lo) {
-                    *at(2, k - i) = c;
-                    c = through(a[i], c, b[i]);
+            for (int i = kBatch - 1; i >= 0; --i)
+                if (k + i < hi) {
+                    *at(2, k + i) = g;
+                    g = through(a[i], g, c[i]);
                 }
         }
-        if (p.dstate && run == 0) store2(p.dstate + state_at, p.vec, nch, c);
+        if (p.dstate && run == 0) store2(p.dstate + state_at, p.vec, nch, g);
     }
 }
 
