@@ -316,7 +316,7 @@ __device__ __forceinline__ unsigned rows_to_lanes(unsigned (&m)[kFwdSteps])
 struct PackTo {
     unsigned char *gate, *value, *gate_scales, *value_scales;
 };
-// whole: all rows and channels are there, and pairs of codes lie on even addresses
+// whole: all rows are there, and pairs of codes lie on even addresses (a lane has two channels or none)
 __device__ __forceinline__ void pack_rows(const float2 (&z)[kFwdSteps], const float2 (&u)[kFwdSteps], const PackTo &to, long long row, int width, int ch,
                                           bool whole, int cnt, int nch)
 {
@@ -357,8 +357,10 @@ __device__ __forceinline__ void pack_rows(const float2 (&z)[kFwdSteps], const fl
         for (int s = 0; s < kFwdSteps; ++s, zc += width, uc += width) {
             const unsigned both = __shfl_sync(0xffffffffu, inverses, (lane & 16) | s);
             const float2 c = fma2(z[s], two(__uint_as_float(both << 16)), magic), d = fma2(u[s], two(__uint_as_float(both & 0xffff0000u)), magic);
-            *reinterpret_cast<unsigned short *>(zc) = (unsigned short)__byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x0040);
-            *reinterpret_cast<unsigned short *>(uc) = (unsigned short)__byte_perm(__float_as_uint(d.x), __float_as_uint(d.y), 0x0040);
+            if (nch == 2) {
+                *reinterpret_cast<unsigned short *>(zc) = (unsigned short)__byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x0040);
+                *reinterpret_cast<unsigned short *>(uc) = (unsigned short)__byte_perm(__float_as_uint(d.x), __float_as_uint(d.y), 0x0040);
+            }
         }
         return;
     }
@@ -819,7 +821,7 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
         if (more_to_come) ask_now();
         if constexpr (KEEP) {
             const PackTo to = {p.pack_gate, p.pack_value, p.pack_gate_scales, p.pack_value_scales};
-            pack_rows(a, b, to, first + t0, p.width, ch, vec && from.left >= kSlab && cnt == S, cnt, nch);
+            pack_rows(a, b, to, first + t0, p.width, ch, vec && cnt == S, cnt, nch);
         }
         float2 A = two(1.0f), H = two(0.0f);
         bool special;
@@ -1069,10 +1071,10 @@ static int scan_check(const ScanDims &d)
     return GN_OK;
 }
 
-// Whether the forward pass (backward: the backward pass) walks or goes by chunks. A walk's tile takes 1.2 to 1.4 us however few CTAs there
-// are, chunks cost two more kernels (10 us) and a second reading. us, walk / chunks, forward and backward: 64 CTAs, 8 x 1024 x 512 float32
-// 21.5 / 17.5 and 45 / 31, 4 x 4097 x 1024 90 / 61 and 203 / 108; 256 CTAs, 16 x 1024 x 1000 float32 44 / 62 and 78 / 118, 16 x 512 x 1024
-// bfloat16 13 / 24 and 25 / 41; 16 CTAs, 1 x 300 x 1024 float32 14 / 18 and 17 / 15. So: a CTA per SM, or few tiles one after the other.
+// Whether the forward pass (backward: the backward pass) walks or goes by chunks. A walk's tile takes 1.2 to 1.8 us however few CTAs there
+// are, chunks cost two more kernels (8 to 10 us) and a second reading. us, walk / chunks, forward and backward: 64 CTAs, 8 x 1024 x 512 float32
+// 24 / 18 and 58 / 31, 4 x 4097 x 1024 95 / 58 and 236 / 107; 256 CTAs, 16 x 1024 x 1000 float32 45 / 59 and 93 / 109, 16 x 512 x 1024
+// bfloat16 14 / 25 and 26 / 40; 16 CTAs, 1 x 300 x 1024 float32 10 / 13 and 15 / 13. So: a CTA per SM, or few tiles one after the other.
 // How long the longest of ragged sequences is is not known here: eight rounds of CTAs, so that one of eight times the mean takes no longer
 // than all (37 of mean 300, the longest 2380, x 1000 bfloat16: a walk takes 118 and 183 us, chunks 50 and 75).
 static bool scan_walks(const ScanDims &d, bool backward, bool packed)
