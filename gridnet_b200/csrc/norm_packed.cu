@@ -11,13 +11,27 @@
 
 namespace gn {
 
-// y and the packed copy. A thread has four positions of four samples, with gamma and beta read once for them; eight lanes have a group. Later
-// samples first: of them, what the sums were taken from is still in L2.
-constexpr int kTogether = 4;
-__global__ void __launch_bounds__(256) norm_apply_pack_k(const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta,
-                                                         const float2 *stats, float *__restrict__ y, unsigned char *__restrict__ codes,
-                                                         unsigned char *__restrict__ scales, int B, int slices, long long per_row, long long P, int vec)
+constexpr int kTogether = 4;     // samples that a thread loads at a time
+constexpr int kFoldParts = 128;  // partial sums that a CTA may add up itself (703, 40 x 56 x 72 x 37: 26 us instead of 16 + 3.5)
+
+// Sum of up to 64 partial sums by a warp, in the order in which a block of threads adds them up (block_sum)
+__device__ __forceinline__ double2 sum_of_parts(const double2 *partials, int parts)
 {
+    static_assert(kNormMaxParts == 64, "two to a lane");
+    const int lane = threadIdx.x & 31;
+    const double2 none = make_double2(0.0, 0.0), a = lane < parts ? partials[lane] : none, b = lane + 32 < parts ? partials[lane + 32] : none;
+    return make_double2(warp_sum(a.x) + warp_sum(b.x), warp_sum(a.y) + warp_sum(b.y));
+}
+
+// y and the packed copy. With partial sums a CTA finishes the statistics of its four samples itself, a launch
+// less; without them stats has them. A thread has four positions of four samples, with gamma and beta read once for them; eight lanes have a group. Later
+// samples first: of them, what the sums were taken from is still in L2.
+__global__ void __launch_bounds__(256) norm_apply_pack_k(const float *__restrict__ x, const float *__restrict__ gamma, const float *__restrict__ beta,
+                                                         const double2 *partials, int parts, float eps, float2 *stats, float *__restrict__ y,
+                                                         unsigned char *__restrict__ codes, unsigned char *__restrict__ scales, int B, int slices,
+                                                         long long per_row, long long P, int vec)
+{
+    __shared__ float2 of_sample[kTogether];
     const int chunk = blockIdx.x / slices, last = B - 1 - chunk * kTogether;
     const long long col = ((long long)(blockIdx.x - chunk * slices) * 256 + threadIdx.x) * 4;
     const int n = (int)min(4LL, max(0LL, P - col));
@@ -27,6 +41,21 @@ __global__ void __launch_bounds__(256) norm_apply_pack_k(const float *__restrict
     load4(gamma + col, vec, n, ga);
     load4(beta + col, vec, n, be);
     previous_done();
+    const int warp = threadIdx.x >> 5;
+    if (!partials) {
+        if (threadIdx.x < kTogether && last - (int)threadIdx.x >= 0) of_sample[threadIdx.x] = stats[last - threadIdx.x];
+    } else if (warp < kTogether && last - warp >= 0) {
+        const double2 sums = sum_of_parts(partials + (size_t)(last - warp) * parts, parts);
+        const double mean = sums.x / (double)P;
+        double var = sums.y / (double)P - mean * mean;
+        if (var < 0.0) var = 0.0;
+        const float2 mr = make_float2((float)mean, (float)(1.0 / sqrt(var + (double)eps)));
+        if ((threadIdx.x & 31) == 0) {
+            of_sample[warp] = mr;
+            if (blockIdx.x == chunk * slices) stats[last - warp] = mr;
+        }
+    }
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < kTogether; ++i) {
         const int b = last - i;
@@ -37,7 +66,7 @@ __global__ void __launch_bounds__(256) norm_apply_pack_k(const float *__restrict
             const long long at = b * P + col;
             store_codes(codes + at, vec, n, w);
             if ((threadIdx.x & 7) == 0) scales[b * per_row + col / kPackGroup] = (unsigned char)scale;
-            const float2 mr = stats[b];
+            const float2 mr = of_sample[i];
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[i][k] = fmaf((v[i][k] - mr.x) * mr.y, ga[k], be[k]);
             store4(y + at, vec, n, v[i]);
@@ -101,19 +130,17 @@ __global__ void __launch_bounds__(256) norm_packed_sums_k(const unsigned char *_
     if (threadIdx.x == 0) partials[blockIdx.x] = make_double2(sq, sp);
 }
 
-// one CTA per sample: means of q and q p
-__global__ void __launch_bounds__(64) norm_packed_means_k(const double2 *partials, int parts, float2 *__restrict__ ac, long long P)
+// one warp per sample: means of q and q p
+__device__ __forceinline__ float2 means_of(const double2 *partials, int parts, long long P)
 {
-    __shared__ double red[33];
+    const double2 sums = sum_of_parts(partials, parts);
+    return make_float2((float)(sums.x / (double)P), (float)(sums.y / (double)P));
+}
+__global__ void __launch_bounds__(32) norm_packed_means_k(const double2 *partials, int parts, float2 *ac, long long P)
+{
     previous_done();
-    double q = 0.0, p = 0.0;
-    for (int i = threadIdx.x; i < parts; i += blockDim.x) {
-        q += partials[(size_t)blockIdx.x * parts + i].x;
-        p += partials[(size_t)blockIdx.x * parts + i].y;
-    }
-    q = block_sum(q, red);
-    p = block_sum(p, red);
-    if (threadIdx.x == 0) ac[blockIdx.x] = make_float2((float)(q / (double)P), (float)(p / (double)P));
+    const float2 m = means_of(partials + (size_t)blockIdx.x * parts, parts, P);
+    if (threadIdx.x == 0) ac[blockIdx.x] = m;
 }
 
 // A thread has four positions and every PARTS-th sample, 256 / PARTS threads side by side; the parts' sums are added up in a fixed order. Four
@@ -121,18 +148,28 @@ __global__ void __launch_bounds__(64) norm_packed_means_k(const double2 *partial
 // eight (40 x 56 x 72 x 37 37 -> 19 us, 32^3 x 8 10.6 -> 4.5).
 template <int PARTS>
 __global__ void __launch_bounds__(256) norm_packed_apply_k(const unsigned char *__restrict__ codes, const unsigned char *__restrict__ scales,
-                                                           const float2 *stats, const float2 *ac, const float *__restrict__ gamma,
+                                                           const float2 *stats, const float2 *ac, const double2 *partials, int parts,
+                                                           const float *__restrict__ gamma,
                                                            const float *__restrict__ gy, float *__restrict__ gx, float *__restrict__ ggamma,
                                                            float *__restrict__ gbeta, int B, long long P, long long per_row, int vec)
 {
     constexpr int kSide = 256 / PARTS;
     __shared__ float4 sums[2][PARTS][PARTS > 1 ? kSide : 1];
+    __shared__ float2 means[kFoldParts];
     const int place = threadIdx.x % kSide, part = threadIdx.x / kSide;
     const long long col = ((long long)blockIdx.x * kSide + place) * 4;
     const int n = (int)min(4LL, max(0LL, P - col));
     float ga[4], sg[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sb[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     load4(gamma + col, vec, n, ga);
     previous_done();
+    if (!ac) {  // few enough: every CTA adds them up itself, a launch less
+        for (int b = threadIdx.x >> 5; b < B; b += 8) {
+            const float2 m = means_of(partials + (size_t)b * parts, parts, P);
+            if ((threadIdx.x & 31) == 0) means[b] = m;
+        }
+        __syncthreads();
+        ac = means;
+    }
     if (n > 0) {
         for (int b0 = part; b0 < B; b0 += PARTS * kTogether) {
             float g[kTogether][4];
@@ -229,12 +266,15 @@ GN_API int gn_norm_forward_packed_f32(const float *x, const float *gamma, const 
     float2 *const stats = reinterpret_cast<float2 *>(mean_rstd);
     const int parts = norm_pick_parts(P);
     rc = launch_norm_partial_stats(x, ws.partials, B, P, parts, st);
-    if (rc == GN_OK) rc = launch_norm_finalize(ws.partials, parts, stats, B, P, eps, st);
     if (rc != GN_OK) return rc;
-    const long long per_row = (P + kPackGroup - 1) / kPackGroup, slices = (P + 1023) / 1024;
+    const long long per_row = (P + kPackGroup - 1) / kPackGroup, slices = (P + 1023) / 1024, ctas = slices * ((B + kTogether - 1) / kTogether);
+    // two rounds of CTAs: 40 x 56 x 72 x 37 13.2 us instead of 10.9 + 3.6; 128^3 x 32, seven rounds, 113 instead of 103 + 3.8
+    const bool fold = ctas <= 16LL * sm_count();
+    if (!fold) rc = launch_norm_finalize(ws.partials, parts, stats, B, P, eps, st);
+    if (rc != GN_OK) return rc;
     const int vec = P % 4 == 0 && aligned(x, 16) && aligned(gamma, 16) && aligned(beta, 16) && aligned(y, 16) && aligned(codes, 4);
-    launch_after(norm_apply_pack_k, dim3((unsigned)(slices * ((B + kTogether - 1) / kTogether))), dim3(256), 0, st, x, gamma, beta, stats, y,
-                 (unsigned char *)codes, (unsigned char *)scales, B, (int)slices, per_row, P, vec);
+    launch_after(norm_apply_pack_k, dim3((unsigned)ctas), dim3(256), 0, st, x, gamma, beta, fold ? ws.partials : nullptr, parts,
+                 eps, stats, y, (unsigned char *)codes, (unsigned char *)scales, B, (int)slices, per_row, P, vec);
     return check_launch("norm_apply_pack");
 }
 
@@ -255,18 +295,20 @@ GN_API int gn_norm_backward_packed_f32(const void *codes, const void *scales, co
     const long long per_row = (P + kPackGroup - 1) / kPackGroup;
     const int vec = P % 4 == 0 && aligned(gamma, 16) && aligned(gy, 16) && aligned(gx, 16) && aligned(ggamma, 16) && aligned(gbeta, 16) &&
                     aligned(codes, 4);
+    const int parts = norm_pick_parts(P);
+    const bool fold = (long long)B * parts <= kFoldParts;
+    const float2 *const ac = fold ? nullptr : ws.ac;
     if (B > 0) {
-        const int parts = norm_pick_parts(P);
         const long long slice = ((P + parts - 1) / parts + kPackGroup - 1) / kPackGroup * kPackGroup;
         norm_packed_sums_k<<<(unsigned)B * parts, 256, 0, st>>>(c, s, stats, gamma, gy, ws.partials, P, slice, per_row, parts, vec);
-        launch_after(norm_packed_means_k, dim3(B), dim3(64), 0, st, ws.partials, parts, ws.ac, P);
+        if (!fold) launch_after(norm_packed_means_k, dim3(B), dim3(32), 0, st, ws.partials, parts, ws.ac, P);
     }
     if (P >= 2048LL * sm_count())
-        launch_after(norm_packed_apply_k<1>, dim3((unsigned)((P + 1023) / 1024)), dim3(256), 0, st, c, s, stats, ws.ac, gamma, gy, gx, ggamma, gbeta,
-                     B, P, per_row, vec);
+        launch_after(norm_packed_apply_k<1>, dim3((unsigned)((P + 1023) / 1024)), dim3(256), 0, st, c, s, stats, ac, ws.partials, parts, gamma, gy, gx,
+                     ggamma, gbeta, B, P, per_row, vec);
     else
-        launch_after(norm_packed_apply_k<8>, dim3((unsigned)((P + 127) / 128)), dim3(256), 0, st, c, s, stats, ws.ac, gamma, gy, gx, ggamma, gbeta, B,
-                     P, per_row, vec);
+        launch_after(norm_packed_apply_k<8>, dim3((unsigned)((P + 127) / 128)), dim3(256), 0, st, c, s, stats, ac, ws.partials, parts, gamma, gy, gx,
+                     ggamma, gbeta, B, P, per_row, vec);
     return check_launch("norm_backward_packed");
 }
 

@@ -142,7 +142,7 @@ def _norm_want(x, gamma, beta, g, eps=1e-5):
     return out
 
 
-@pytest.mark.parametrize("B,grid", [(1, (4, 4, 4)), (3, (8, 8, 8)), (2, (1, 1, 1)), (5, (3, 5, 7)), (4, (2, 9, 18)), (9, (16, 24, 16)), (2, (32, 32, 40)), (130, (8, 8, 4))])
+@pytest.mark.parametrize("B,grid", [(1, (4, 4, 4)), (3, (8, 8, 8)), (2, (1, 1, 1)), (5, (3, 5, 7)), (4, (2, 9, 18)), (9, (16, 24, 16)), (2, (32, 32, 40)), (130, (8, 8, 4)), (1100, (4, 4, 4)), (9600, (2, 2, 2)), (2, (64, 72, 72))])
 def test_norm(B, grid):
     import gridnet_b200 as gb
 
@@ -170,6 +170,7 @@ def test_norm_module_and_setting():
     assert gb.keep_packed(True) is False
     try:
         ours = norm(x)
+        assert torch.equal(plain, ours)
         a, b = torch.autograd.grad(plain, x, g)[0], torch.autograd.grad(ours, x, g)[0]
         direct = torch.autograd.grad(gb.PackedGridNormOp.apply(x, norm.weight, norm.bias, norm.eps), x, g)[0]
         assert torch.equal(b, direct) and not torch.equal(a, b)
