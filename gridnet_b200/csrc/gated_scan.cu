@@ -1105,10 +1105,12 @@ static int launch_chunks(Scan &p, const ScanDims &d, size_t work_smem, const cha
     p.map_rows = d.tile_rows(kLog2);
     const size_t smem = p.wide ? kScanWarps * Source<T, PACKED, BACKWARD, kSumSteps>::kBytes : 0;
     const long long warps = p.map_rows * p.slabs;
-    // More than one tile to a CTA, the next asked for while one is worked on, where six rounds of CTAs are left (four fit an SM): 2 x 20000 x
-    // 2048 bfloat16 backward 335 -> 291 us; with fewer rounds the last one costs more (4 x 4097 x 1024 float32 forward 61 -> 67 us)
+    // More than one tile to a CTA, the next asked for while one is worked on: 2 x 20000 x 2048 bfloat16 forward 191 -> 174 us, backward 356 ->
+    // 298. Forward where six rounds of CTAs are left (four fit an SM), with fewer the last one costs as much (4 x 4097 x 1024 float32 58.1 -> 58.4
+    // us, and 71.2 -> 73.9 with packing); backward, whose tiles are half as long, where two are (one to four tiles: 6 x 3000 x 640 bfloat16 55.4 ->
+    // 51.4 us, 37 ragged sequences of mean 300 x 1000 69 -> 64; 8 x 1024 x 512 float32, one round, stays at one tile: 31)
     p.tiles_per_cta = 1;
-    while (p.tiles_per_cta < 8 && warps / (2 * p.tiles_per_cta) >= 24LL * sm_count()) p.tiles_per_cta *= 2;
+    while (p.tiles_per_cta < 8 && warps / (2 * p.tiles_per_cta) >= (BACKWARD ? 8LL : 24LL) * sm_count()) p.tiles_per_cta *= 2;
     const long long ctas = (p.map_rows + p.tiles_per_cta - 1) / p.tiles_per_cta * p.slabs;
     scan_maps_k<T, PACKED, BACKWARD><<<(unsigned)((warps + kScanWarps - 1) / kScanWarps), kScanThreads, smem, st>>>(p);
     // eight tiles to a run (they are read together), 64 runs at most and four at least, a warp; ragged: for twice the mean sequence
