@@ -48,6 +48,39 @@ def test_dense(n, steps, width, packed, dtype):
     _check(want, h, last, grads, kind, (n * steps, width))
 
 
+def _far_values(seed, rows, cols):
+    """Rows of every scale, zeros, the largest numbers; what is not finite in every third group only, so that both ways of packing are taken."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g) * torch.exp2(torch.randint(-140, 122, (rows, 1), generator=g).float())
+    x[::5] = 0
+    x[1::7] = torch.randn(x[1::7].shape, generator=g) * 2.0**125
+    for v in (float("inf"), float("-inf"), float("nan")):
+        x[torch.randint(0, rows, (1 + rows // 40,), generator=g), torch.randint(0, cols, (1 + rows // 40,), generator=g)] = v
+    return x
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("lengths,width", [([1], 1), ([16, 15, 17, 0, 1], 64), ([37, 70], 33), ([64, 129, 3], 63), ([300], 100), ([700, 5], 34), ([2000], 65),
+                                           ([40] * 9, 128)])
+def test_copies_are_those_of_packing(lengths, width, dtype):
+    """What the forward pass keeps of gate and value has the codes and scales of the format, whole tiles, last rows and odd widths alike."""
+    import gridnet_b200 as gb
+    from gridnet_b200.scan import _packed_at
+
+    total = sum(lengths)
+    offsets = torch.tensor([0, *lengths]).cumsum(0).cuda()
+    z, u = (_far_values(seed + width, total, width).to(TYPES[dtype]) for seed in (1, 1000))
+    leaves = [t.cuda().requires_grad_(True) for t in (z, u)]
+    for one, spans in ((leaves, offsets), ([t.detach()[None].requires_grad_(True) for t in leaves], None)):
+        h, _ = gb.gated_scan(*one, None, spans, packed=True)
+        kept, places = h.grad_fn.saved_tensors[0], _packed_at(total, width)
+        for i, x in enumerate((z, u)):
+            codes, scales, _ = pack(x.float().numpy())
+            got = kept[places[i]:][:total * width].view(torch.int8).cpu()
+            assert torch.equal(got, torch.from_numpy(codes).reshape(-1))
+            assert torch.equal(kept[places[i + 2]:][:scales.size].cpu(), torch.from_numpy(scales).reshape(-1))
+
+
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("packed", [False, True])
 @pytest.mark.parametrize("lengths,width", [([0, 1, 0, 5, 130, 0], 36), ([700, 3, 64, 65, 1], 7), ([0, 0], 4), ([1] * 40, 64), ([2100, 0, 9], 20)])
