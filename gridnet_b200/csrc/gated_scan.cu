@@ -243,39 +243,26 @@ __device__ __forceinline__ void load_rows(const T *x, long long step, bool vec, 
     }
 }
 
+// the codes of two channels of each row; rows behind the end have the last one's
 template <int S>
-__device__ __forceinline__ void load_packed(const unsigned char *codes, const unsigned char *scales, long long row, int width, int ch, bool vec,
-                                            int cnt, int nch, float end, float2 (&v)[S])
+__device__ __forceinline__ void load_codes(const unsigned char *c, long long width, bool vec, int cnt, int nch, unsigned (&w)[S])
 {
     if (cnt <= 0 || nch <= 0) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) v[s] = s < cnt ? two(0.0f) : two(end);
-        return;
-    }
-    const int per_row = (width + kPackGroup - 1) / kPackGroup;
-    const unsigned char *const c = codes + row * width + ch, *const g = scales + row * per_row + ch / kPackGroup;
-    unsigned w[S], sc[S];
-    if (vec && nch == 2) {
+        for (int s = 0; s < S; ++s) w[s] = 0u;
+    } else if (vec && nch == 2) {
 #pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const long long i = min(s, cnt - 1);
-            w[s] = *reinterpret_cast<const unsigned short *>(c + i * width);
-            sc[s] = g[i * per_row];
-        }
+        for (int s = 0; s < S; ++s) w[s] = *reinterpret_cast<const unsigned short *>(c + min(s, cnt - 1) * width);
     } else {
+        unsigned other[S];
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-            const long long i = min(s, cnt - 1);
-            w[s] = c[i * width] | (nch > 1 ? (unsigned)c[i * width + 1] << 8 : 0u);
-            sc[s] = g[i * per_row];
+            const unsigned char *const at = c + min(s, cnt - 1) * width;
+            w[s] = at[0];
+            other[s] = at[nch - 1];
         }
-    }
 #pragma unroll
-    for (int s = 0; s < S; s += 2) {  // the codes of two steps in a word
-        float f[4];
-        unpack4(w[s] | w[s + 1] << 16, 1.0f, f);
-        v[s] = s < cnt ? make_float2(f[0] * pack_step(sc[s]), f[1] * pack_step(sc[s])) : two(end);
-        v[s + 1] = s + 1 < cnt ? make_float2(f[2] * pack_step(sc[s + 1]), f[3] * pack_step(sc[s + 1])) : two(end);
+        for (int s = 0; s < S; ++s) w[s] |= nch > 1 ? other[s] << 8 : 0u;
     }
 }
 
@@ -470,18 +457,13 @@ __device__ __forceinline__ Scales ask_scales(const Scan &p, long long row, int s
     const long long at = there ? (row + r) * per_row + g : 0;
     return {p.gate_scales[at], p.value_scales[at]};
 }
-// gate and value as their codes give them
-template <int S>
-__device__ __forceinline__ void take_packed(const Rows<unsigned char, S> &gates, const Rows<unsigned char, S> &values, Scales scales, int cnt, int nch,
-                                            float end, float2 (&z)[S], float2 (&u)[S])
+// gate and value as their codes give them; word(value, s): the codes of steps s and s + 1
+template <int S, typename Word>
+__device__ __forceinline__ void take_packed(Word word, Scales scales, int cnt, int nch, float end, float2 (&z)[S], float2 (&u)[S])
 {
     const int lane = threadIdx.x & 31;
     unsigned wz[S / 2], wu[S / 2];
     float far = 0.0f;
-    auto word = [&](const Rows<unsigned char, S> &from, int s) {  // the codes of two steps
-        return __byte_perm(*reinterpret_cast<const unsigned short *>(&from.v[s][lane * 2]), *reinterpret_cast<const unsigned short *>(&from.v[s + 1][lane * 2]),
-                           0x5410);
-    };
     auto whole = [&](unsigned w, float2 &a, float2 &b) {
         float f[4];
         unpack4_finite(w, f);
@@ -491,8 +473,8 @@ __device__ __forceinline__ void take_packed(const Rows<unsigned char, S> &gates,
     };
 #pragma unroll
     for (int s = 0; s < S; s += 2) {
-        whole(wz[s / 2] = word(gates, s), z[s], z[s + 1]);
-        whole(wu[s / 2] = word(values, s), u[s], u[s + 1]);
+        whole(wz[s / 2] = word(false, s), z[s], z[s + 1]);
+        whole(wu[s / 2] = word(true, s), u[s], u[s + 1]);
     }
     const unsigned steps = (scales.gate | (unsigned)scales.value << 16) << 7;  // the upper halves of both 2^e (the lower ones are 0)
 #pragma unroll
@@ -594,12 +576,13 @@ struct Source {
     // cnt rows from step t of the sequence on (none: nothing)
     __device__ __forceinline__ void ask_for(long long t, int cnt)
     {
-        if (!p.wide || cnt <= 0) return;
+        if (cnt <= 0) return;
+        if constexpr (PACKED) scales = ask_scales(p, first + t, slab, cnt);
+        if (!p.wide) return;
         ask(*zs, asks_from<V, S>(gate + t * gate_step, gate_step), gate_step, cnt, left);
         ask(*us, asks_from<V, S>(value + t * value_step, value_step), value_step, cnt, left);
         if constexpr (GRAD) ask(*gs, asks_from<T, S>(grad + t * p.width, p.width), (long long)p.width, cnt, left);
         copies_on_their_way();
-        if constexpr (PACKED) scales = ask_scales(p, first + t, slab, cnt);
     }
     // What was asked for; a step behind the end holds the state and has no gradient of its own. Then `ask_for` may ask for other rows
     __device__ __forceinline__ void take_from(long long t, int cnt, float2 (&z)[S], float2 (&u)[S], float2 (&g)[GRAD ? S : 1])
@@ -608,7 +591,11 @@ struct Source {
         if (p.wide) {
             copies_there();
             if constexpr (PACKED) {
-                take_packed<S>(*zs, *us, scales, cnt, nch, inf, z, u);
+                auto word = [&](bool value, int s) {
+                    const unsigned char *const at = &(value ? us : zs)->v[s][(threadIdx.x & 31) * 2];
+                    return __byte_perm(*reinterpret_cast<const unsigned short *>(at), *reinterpret_cast<const unsigned short *>(at + kSlab), 0x5410);
+                };
+                take_packed<S>(word, scales, cnt, nch, inf, z, u);
             } else {
                 take(*zs, cnt, nch, inf, z);
                 take(*us, cnt, nch, 0.0f, u);
@@ -618,8 +605,10 @@ struct Source {
         } else {
             const int lane = threadIdx.x & 31;
             if constexpr (PACKED) {
-                load_packed<S>((const unsigned char *)p.gate, p.gate_scales, first + t, p.width, ch, p.vec, cnt, nch, inf, z);
-                load_packed<S>((const unsigned char *)p.value, p.value_scales, first + t, p.width, ch, p.vec, cnt, nch, 0.0f, u);
+                unsigned wz[S], wu[S];
+                load_codes<S>(gate + lane * 2 + t * p.width, p.width, p.vec, cnt, nch, wz);
+                load_codes<S>(value + lane * 2 + t * p.width, p.width, p.vec, cnt, nch, wu);
+                take_packed<S>([&](bool value, int s) { return value ? wu[s] | wu[s + 1] << 16 : wz[s] | wz[s + 1] << 16; }, scales, cnt, nch, inf, z, u);
             } else {
                 load_rows<T, S>(gate + lane * 2 + t * gate_step, gate_step, p.vec, cnt, nch, inf, z);
                 load_rows<T, S>(value + lane * 2 + t * value_step, value_step, p.vec, cnt, nch, 0.0f, u);
