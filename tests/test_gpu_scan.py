@@ -106,6 +106,29 @@ def test_ragged_with_held_and_reset_steps(lengths, width, packed, dtype):
 
 
 @pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("lengths", [[9000, 0, 3, 40], [20000], [2500, 2500]])
+def test_long_sequences_with_few_resets(lengths, packed):
+    """Many tiles to a run of tiles: a reset in some of the channels of some of them, not finite values ahead of one."""
+    import gridnet_b200 as gb
+
+    n, total, width = len(lengths), sum(lengths), 34
+    z, u, h0, g, gl = _inputs(total, total, n, width, torch.float32)
+    for at, ch in ((1700, 3), (1701, 3), (2111, 20), (4444 % total, 33), (total - 70, 0)):
+        z[at, ch] = float("-inf")
+    ends = torch.tensor([0] + lengths).cumsum(0)
+    want = _want(z, u, h0, list(zip(ends.tolist(), ends.tolist()[1:])), g, gl, packed)
+    leaves = [t.cuda().requires_grad_(True) for t in (z, u, h0)]
+    h, last = gb.gated_scan(*leaves, ends, packed=packed)
+    grads = torch.autograd.grad([h, last], leaves, [g.cuda(), gl.cuda()])
+    _check(want, h, last, grads, torch.float32, (total, width))
+    # a state that is not finite ends at the next reset: from there on nothing has changed
+    u[900:905, 3], u[2100, 20] = float("nan"), float("inf")
+    spoilt, _ = gb.gated_scan(z.cuda(), u.cuda(), h0.cuda(), ends)
+    assert not spoilt[905:1700, 3].isfinite().any() and not spoilt[2100:2111, 20].isfinite().any()
+    assert torch.equal(spoilt[1700:, 3], h[1700:, 3]) and torch.equal(spoilt[2111:, 20], h[2111:, 20])
+
+
+@pytest.mark.parametrize("packed", [False, True])
 def test_rows_of_no_sequence_are_zero(packed):
     import gridnet_b200 as gb
 
