@@ -1121,10 +1121,10 @@ static int scan_check(const ScanDims &d)
 
 // Whether the forward pass (backward: the backward pass) walks or goes by chunks. A walk's tile takes 1.2 to 1.8 us however few CTAs there
 // are, chunks cost two more kernels (8 to 10 us) and a second reading. us, walk / chunks, forward and backward: 64 CTAs, 8 x 1024 x 512 float32
-// 24 / 18 and 58 / 31, 4 x 4097 x 1024 95 / 58 and 236 / 107; 256 CTAs, 16 x 1024 x 1000 float32 45 / 59 and 93 / 109, 16 x 512 x 1024
+// 24 / 18 and 58 / 31, 4 x 4097 x 1024 95 / 58 and 236 / 106; 256 CTAs, 16 x 1024 x 1000 float32 45 / 59 and 93 / 109, 16 x 512 x 1024
 // bfloat16 14 / 25 and 26 / 40; 16 CTAs, 1 x 300 x 1024 float32 10 / 13 and 15 / 13. So: a CTA per SM, or few tiles one after the other.
 // How long the longest of ragged sequences is is not known here: eight rounds of CTAs, so that one of eight times the mean takes no longer
-// than all (37 of mean 300, the longest 2380, x 1000 bfloat16: a walk takes 118 and 183 us, chunks 50 and 75).
+// than all (37 of mean 300, the longest 2380, x 1000 bfloat16: a walk takes 118 and 183 us, chunks 41 and 61).
 static bool scan_walks(const ScanDims &d, bool backward, bool packed)
 {
     const int log2 = backward ? kBwdLog2 : kFwdLog2;
