@@ -69,6 +69,16 @@ def stream_of(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
+def check_written(t: torch.Tensor, name: str) -> None:
+    """What torch asks of a tensor that is written in place."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise GridnetB200Error(f"{name} requires a gradient: what is written in place here has none")
+
+
+# After the library has written to a tensor of the caller's: autograd counts it like an in-place operation of torch's own
+written = torch.autograd.graph.increment_version
+
+
 def pack_activations(x: torch.Tensor, rows: int = 1) -> PackedActivations:
     """The packed copy of ``x`` (float32, bfloat16 or float16, on a CUDA device). The first ``rows`` dimensions count rows (a sample, a
     step of a sequence); groups of 32 run along the others taken together and never across a row's end."""

@@ -13,7 +13,7 @@ from torch.autograd.function import once_differentiable
 
 from ._lib import GridnetB200Error, check, lib
 from .backend_cuda import _Op
-from .packed import DTYPES, GROUP, dtype_id, keeps_packed, on_device, stream_of
+from .packed import DTYPES, GROUP, check_written, dtype_id, keeps_packed, on_device, stream_of, written
 
 
 def _rows(t: torch.Tensor, lead: int) -> torch.Tensor:
@@ -186,7 +186,7 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor | No
 
 def gated_scan_step(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor, out_state: torch.Tensor | None = None):
     """One step of :func:`gated_scan` without gradients: ``gate`` and ``value`` [batch, ...], ``state`` [batch, ...] float32. Returns
-    ``(h, new_state)``; ``out_state`` (which may be ``state``) receives the new state."""
+    ``(h, new_state)``; ``out_state`` (which may be ``state``) receives the new state, which autograd sees as a change in place."""
     for name, t in (("gate", gate), ("value", value), ("state", state)):
         if not t.is_cuda:
             raise GridnetB200Error(f"{name} must be a CUDA tensor")
@@ -199,17 +199,21 @@ def gated_scan_step(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor
     z, u, s = _rows(gate, 1), _rows(value, 1), state.contiguous()
     rows, width = z.shape
     assert width > 0, f"{gate.shape=}: steps of no values"
-    if out_state is None:
+    given = out_state is not None
+    if not given:
         out_state = torch.empty_like(s)
     else:
         assert out_state.shape == shape and out_state.dtype == torch.float32 and out_state.device == dev, (
             f"{out_state.shape=} {out_state.dtype=} {out_state.device=} invalid for a state of {state.shape}")
         if not out_state.is_contiguous():
             raise GridnetB200Error("out_state must be contiguous")
+        check_written(out_state, "out_state")
     h = torch.empty(shape, dtype=gate.dtype, device=dev)
     with on_device(dev):
         check(lib.gn_gated_scan_step(z.data_ptr(), u.data_ptr(), s.data_ptr(), h.data_ptr(), out_state.data_ptr(), rows, width, z.stride(0),
                                      u.stride(0), dtype, stream_of(gate)))
+    if given:
+        written(out_state)
     return h, out_state
 
 
