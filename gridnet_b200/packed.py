@@ -96,7 +96,8 @@ def pack_activations(x: torch.Tensor, rows: int = 1) -> PackedActivations:
 
 
 def unpack_activations(packed: PackedActivations, out: torch.Tensor | None = None) -> torch.Tensor:
-    """What the packed copy stands for, in the tensor's own type or in ``out``'s (contiguous, any of the three types)."""
+    """What the packed copy stands for, in the tensor's own type or in ``out``'s (contiguous, any of the three types). Autograd sees a
+    change in place of ``out``."""
     codes, scales, dtype = packed
     for name, t in (("codes", codes), ("scales", scales)):
         if not t.is_cuda:
@@ -109,12 +110,16 @@ def unpack_activations(packed: PackedActivations, out: torch.Tensor | None = Non
     nrows, cols = codes.shape[:rows].numel(), codes.shape[rows:].numel()
     assert 0 <= rows <= codes.dim() and scales.shape == (*codes.shape[:rows], (cols + GROUP - 1) // GROUP), (
         f"{scales.shape=} invalid for {codes.shape=}")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
     assert out.shape == codes.shape, f"{out.shape=} invalid for {codes.shape=}"
     assert out.device == codes.device, f"mismatching devices: {codes.device=} {out.device=}"
     if not out.is_contiguous():
         raise GridnetB200Error("out must be contiguous")
+    check_written(out, "out")
     with on_device(codes.device):
         check(lib.gn_unpack8(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), nrows, cols, dtype_id(out, "out"), stream_of(codes)))
+    if given:
+        written(out)
     return out
