@@ -75,6 +75,26 @@ def check_written(t: torch.Tensor, name: str) -> None:
         raise GridnetB200Error(f"{name} requires a gradient: what is written in place here has none")
 
 
+def overlaps(out: torch.Tensor, t: torch.Tensor) -> bool:
+    """Whether ``out``, contiguous, has bytes of ``t``, which is [rows, values] with the values of a row side by side and rows at any
+    distance."""
+    rows, row = t.shape[0], t.shape[1] * t.element_size()
+    lo, nbytes, base = out.data_ptr(), out.numel() * out.element_size(), t.data_ptr()
+    if not rows or not row or not nbytes or base >= lo + nbytes:
+        return False
+    distance = t.stride(0) * t.element_size()
+    # the first row that ends behind the start of out
+    first = max(0, (lo - row - base) // distance + 1) if distance else 0
+    return first < rows and base + first * distance < lo + nbytes and base + first * distance + row > lo
+
+
+def refuse_overlap(out: torch.Tensor, name: str, **inputs: torch.Tensor) -> None:
+    """The kernels read and write in no order that a caller could count on."""
+    for other, t in inputs.items():
+        if overlaps(out, t):
+            raise GridnetB200Error(f"{name} shares memory with {other}")
+
+
 # After the library has written to a tensor of the caller's: autograd counts it like an in-place operation of torch's own
 written = torch.autograd.graph.increment_version
 
@@ -96,8 +116,8 @@ def pack_activations(x: torch.Tensor, rows: int = 1) -> PackedActivations:
 
 
 def unpack_activations(packed: PackedActivations, out: torch.Tensor | None = None) -> torch.Tensor:
-    """What the packed copy stands for, in the tensor's own type or in ``out``'s (contiguous, any of the three types). Autograd sees a
-    change in place of ``out``."""
+    """What the packed copy stands for, in the tensor's own type or in ``out``'s (contiguous, any of the three types; no memory of the
+    copy's). Autograd sees a change in place of ``out``."""
     codes, scales, dtype = packed
     for name, t in (("codes", codes), ("scales", scales)):
         if not t.is_cuda:
@@ -118,6 +138,8 @@ def unpack_activations(packed: PackedActivations, out: torch.Tensor | None = Non
     if not out.is_contiguous():
         raise GridnetB200Error("out must be contiguous")
     check_written(out, "out")
+    if given:
+        refuse_overlap(out, "out", codes=codes.view(1, -1), scales=scales.view(1, -1))
     with on_device(codes.device):
         check(lib.gn_unpack8(codes.data_ptr(), scales.data_ptr(), out.data_ptr(), nrows, cols, dtype_id(out, "out"), stream_of(codes)))
     if given:

@@ -13,7 +13,7 @@ from torch.autograd.function import once_differentiable
 
 from ._lib import GridnetB200Error, check, lib
 from .backend_cuda import _Op
-from .packed import DTYPES, GROUP, check_written, dtype_id, keeps_packed, on_device, stream_of, written
+from .packed import DTYPES, GROUP, check_written, dtype_id, keeps_packed, on_device, refuse_overlap, stream_of, written
 
 
 def _rows(t: torch.Tensor, lead: int) -> torch.Tensor:
@@ -186,7 +186,8 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor | No
 
 def gated_scan_step(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor, out_state: torch.Tensor | None = None):
     """One step of :func:`gated_scan` without gradients: ``gate`` and ``value`` [batch, ...], ``state`` [batch, ...] float32. Returns
-    ``(h, new_state)``; ``out_state`` (which may be ``state``) receives the new state, which autograd sees as a change in place."""
+    ``(h, new_state)``; ``out_state`` (which may be ``state``, and otherwise shares no memory with the inputs) receives the new state, which
+    autograd sees as a change in place."""
     for name, t in (("gate", gate), ("value", value), ("state", state)):
         if not t.is_cuda:
             raise GridnetB200Error(f"{name} must be a CUDA tensor")
@@ -208,6 +209,9 @@ def gated_scan_step(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor
         if not out_state.is_contiguous():
             raise GridnetB200Error("out_state must be contiguous")
         check_written(out_state, "out_state")
+        refuse_overlap(out_state, "out_state", gate=z, value=u)
+        if out_state.data_ptr() != s.data_ptr():
+            refuse_overlap(out_state, "out_state", state=s.view(rows, width))
     h = torch.empty(shape, dtype=gate.dtype, device=dev)
     with on_device(dev):
         check(lib.gn_gated_scan_step(z.data_ptr(), u.data_ptr(), s.data_ptr(), h.data_ptr(), out_state.data_ptr(), rows, width, z.stride(0),
