@@ -22,7 +22,7 @@ from torch.autograd.function import once_differentiable
 
 from . import gridnet_cuda, patch_loop
 from ._lib import activation_id, check, lib
-from .packed import PackedActivations, keeps_packed, on_device, pack_activations, stream_of, unpack_activations
+from .packed import PackedActivations, keeps_packed, on_device, pack_activations, stream_of, unpack_activations, written
 
 
 def _assert_step_args(weight, bias, residual_scale, init_activations, block_size, gated):
@@ -870,7 +870,7 @@ def outer_forward(weight, bias, residual_scale, norm_weight, norm_bias, init_act
             h = gridnet_step(weight, bias, residual_scale, h, inner_iters, block_size, normalize=False, ...)
             h = layer_norm(h, (M, N, K), norm_weight, norm_bias, ln_eps)
 
-    (gridnet/scripts/train_mnist.py:62-64). float32, no autograd.
+    (gridnet/scripts/train_mnist.py:62-64). float32, no autograd; a change of ``out`` in place counts as one.
     """
     batch_size = _assert_step_args(weight, bias, residual_scale, init_activations, block_size, False)
     assert norm_weight.shape == bias.shape == norm_bias.shape, f"{norm_weight.shape=} invalid for {bias.shape=}"
@@ -905,6 +905,8 @@ def outer_forward(weight, bias, residual_scale, norm_weight, norm_bias, init_act
                                              gridnet_cuda._stream(weight)))
     if workspace is not None:
         ws._gn_packed_for = None if key is None else (key, ws._version)
+    if out is not None:
+        written(out)
     return y
 
 

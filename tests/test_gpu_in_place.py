@@ -40,3 +40,17 @@ def test_a_state_that_requires_a_gradient_is_not_overwritten():
     with torch.no_grad():  # as torch's own operations
         gb.gated_scan_step(z, u, leaf, out_state=leaf)
     assert leaf._version > version and not torch.equal(leaf, before)
+
+
+def test_the_loop_without_gradients_into_a_tensor_that_a_graph_keeps():
+    import gridnet_b200 as gb
+
+    model = gb.GridnetModel((8, 8, 8), 1, 1, 8, "cuda")
+    net, norm = model.network, model.norm
+    x, out = torch.randn(1, 8, 8, 8, device="cuda"), torch.randn(1, 8, 8, 8, device="cuda")
+    w = torch.randn(1, 8, 8, 8, device="cuda", requires_grad=True)
+    loop = lambda out: gb.outer_forward(net.weight, net.bias, net.residual_scale, norm.weight, norm.bias, x, 1, 1, 8, out=out)  # noqa: E731
+    product = w * out
+    loop(out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
