@@ -18,6 +18,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import gridnet_cuda, patch_loop
@@ -127,14 +128,23 @@ def _quad_step(weight, x, inner_iters: int, block_size: int, normalize: bool):
     return gridnet_cuda.step_bytes(weight, x, inner_iters, block_size, normalize)
 
 
+def has_tangent(*of) -> bool:
+    """Whether one of these tensors, or a parameter of one of these modules, carries a forward-mode derivative, which no op here has: they go
+    to the autograd functions, which say so. ``requires_grad`` does not tell, and turning gradients off does not turn these off."""
+    if forward_ad._current_level < 0:  # outside of every dual_level, as nearly always
+        return False
+    tensors = [t for o in of for t in (o.parameters() if isinstance(o, torch.nn.Module) else (o,)) if isinstance(t, torch.Tensor)]
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _Op(torch.autograd.Function):
     """An op that keeps things for its backward pass. Where gradients are off there is none, but a parameter still says that it
-    requires one (``ctx.needs_input_grad``), so it comes detached."""
+    requires one (``ctx.needs_input_grad``), so it comes detached. A tensor with a tangent does not: detached it would lose that unseen."""
 
     @classmethod
     def apply(cls, *args):
         if not torch.is_grad_enabled():
-            args = [a.detach() if isinstance(a, torch.Tensor) else a for a in args]
+            args = [a.detach() if isinstance(a, torch.Tensor) and not has_tangent(a) else a for a in args]
         return super().apply(*args)
 
 

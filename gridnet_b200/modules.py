@@ -13,7 +13,8 @@ from typing import Tuple
 import torch
 import torch.nn as nn
 
-from .backend_cuda import FusedGatedLoopTrainOp, FusedLoopTrainOp, GatedGridnetCudaOp, GridnetCudaOp, GridNormOp, PackedGridNormOp, outer_forward
+from .backend_cuda import (FusedGatedLoopTrainOp, FusedLoopTrainOp, GatedGridnetCudaOp, GridnetCudaOp, GridNormOp, PackedGridNormOp, has_tangent,
+                           outer_forward)
 from .packed import keeps_packed
 
 
@@ -139,6 +140,7 @@ class GridnetModel(nn.Module):
         net = self.network
         plain = isinstance(net, Gridnet) and not net.normalize and h.dtype == torch.float32
         with_grad = torch.is_grad_enabled() and (h.requires_grad or any(p.requires_grad for p in self.parameters()))
+        with_grad = with_grad or has_tangent(h, self)
         if plain and not with_grad:
             return outer_forward(net.weight, net.bias, net.residual_scale, self.norm.weight, self.norm.bias,
                                  h.contiguous(), net.inner_iterations, self.outer_iters, net.block_size, net.activation,

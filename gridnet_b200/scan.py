@@ -12,7 +12,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from ._lib import GridnetB200Error, check, lib
-from .backend_cuda import _Op
+from .backend_cuda import _Op, has_tangent
 from .packed import DTYPES, GROUP, check_written, dtype_id, keeps_packed, on_device, refuse_overlap, stream_of, written
 
 
@@ -173,13 +173,15 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor | No
     ``(h, last)``: h like gate, and the state behind the last step, float32.
 
     A step whose s(-gate) is 0 (gate = inf) holds the state and does not look at its value, one whose s(gate) is 0
-    (gate = -inf) takes its value and does not look at the state. Differentiable once in gate, value and state. ``packed``: keep gate and
+    (gate = -inf) takes its value and does not look at the state. Differentiable once in gate, value and state, backward only: tensors with a
+    tangent of torch.autograd.forward_ad are refused. ``packed``: keep gate and
     value in 8 bits for the backward pass, which then takes the gradients at the packed copies; default as
     :func:`keep_packed` says. A step's values have to lie side by side, otherwise they are copied; steps and sequences may lie anywhere, so the
     halves of a wider projection are read where they are."""
     if offsets is not None and not isinstance(offsets, torch.Tensor):
         offsets = torch.as_tensor(offsets, dtype=torch.int64)
-    if not (torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or (state is not None and state.requires_grad))):
+    if not (torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or (state is not None and state.requires_grad))
+            or has_tangent(gate, value, state)):
         return _forward(gate, value, state, offsets, False, False)[:2]
     return GatedScanOp.apply(gate, value, state, offsets, keeps_packed() if packed is None else bool(packed))
 

@@ -16,14 +16,14 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from .backend_cuda import (FusedGatedLoopTrainOp, FusedLoopResidualTrainOp, FusedLoopSeparateTrainOp, FusedLoopTrainOp, fused_loop_forward,
+from .backend_cuda import (FusedGatedLoopTrainOp, FusedLoopResidualTrainOp, FusedLoopSeparateTrainOp, FusedLoopTrainOp, fused_loop_forward, has_tangent,
                            outer_forward)
 from .modules import GatedGridnet, Gridnet, GridNorm, Readout, fused_gated_applies
 
 
 def _wants_grad(module: nn.Module, *tensors: torch.Tensor) -> bool:
-    return torch.is_grad_enabled() and (any(t.requires_grad for t in tensors)
-                                        or any(p.requires_grad for p in module.parameters()))
+    return (torch.is_grad_enabled() and (any(t.requires_grad for t in tensors) or any(p.requires_grad for p in module.parameters()))
+            or has_tangent(*tensors, module))
 
 
 def _plain_loop(network: nn.Module, norm: GridNorm, h: torch.Tensor, outer_iters: int, owner: nn.Module) -> torch.Tensor:
