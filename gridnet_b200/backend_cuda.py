@@ -412,15 +412,14 @@ class _PackedPatches:
 
     def __init__(self, stats: torch.Tensor, packed):
         self.stats, self.packed = stats, packed
-        self.at_hand = {}
+        self.k, self.at_hand = None, None
 
-    def __getitem__(self, k: int) -> torch.Tensor:
-        """The output of step k (-1: the input), unpacked; the two asked for last are kept."""
-        if k not in self.at_hand:
-            while len(self.at_hand) > 1:
-                self.at_hand.pop(next(iter(self.at_hand)))
-            self.at_hand[k] = unpack_activations(self.packed[k + 1])
-        return self.at_hand[k]
+    def input_of(self, k: int) -> torch.Tensor:
+        """The input of step k, which is the output of step k - 1, unpacked; the one asked for last is kept."""
+        if k != self.k:
+            self.at_hand = None  # its memory is free for the next one
+            self.k, self.at_hand = k, unpack_activations(self.packed[k])
+        return self.at_hand
 
 
 def _kept_steps(nbytes_out: int, nbytes_stash: int, outer: int, device) -> int:
@@ -471,8 +470,14 @@ def _patch_forward(plist, norm_weight, norm_bias, x, inner: int, outer: int, blo
             stats = torch.empty(outer, x.shape[0], 2, dtype=torch.float32, device=dev)
             turns = [torch.empty_like(x) for _ in range(min(2, outer))]
             packed = [pack_activations(x)]
+            read_again = outer - int(residual)  # with residual nothing is taken from the last output
+
+            def keep(out):
+                if len(packed) <= read_again:
+                    packed.append(pack_activations(out))
+
             y = patch_loop.forward(plist, norm_weight, norm_bias, x, inner, outer, block, activation, ln_eps, residual,
-                                   [turns[k & 1] for k in range(outer)], stats, [None] * outer, lambda out: packed.append(pack_activations(out)))
+                                   [turns[k & 1] for k in range(outer)], stats, [None] * outer, keep)
         return y, _PackedPatches(stats, packed)
     with torch.cuda.device(dev):
         stash = patch_loop.stash_bytes(x, inner, block)
@@ -575,14 +580,15 @@ def _loop_backward(plist, norm_weight, norm_bias, saved, grad_y, inner: int, out
     dev = g.device
     if isinstance(saved, _PackedPatches):
         with torch.cuda.device(dev):
-            return patch_loop.backward(plist, norm_weight, norm_bias, saved[-1], saved, saved.stats, [None] * outer, g, inner, outer, block, activation,
+            return patch_loop.backward(plist, norm_weight, norm_bias, saved.input_of, saved.stats, [None] * outer, g, inner, outer, block, activation,
                                        residual)
     if isinstance(saved, _PackedLoop):
         return _packed_loop_backward(plist, norm_weight, norm_bias, saved, g, inner, outer, block, activation, residual, gated)
     x_il4, stats, outs, stashes = saved
     if x_il4.dtype == torch.float32:  # _patch_forward
         with torch.cuda.device(dev):
-            return patch_loop.backward(plist, norm_weight, norm_bias, x_il4, outs, stats, stashes, g, inner, outer, block, activation, residual)
+            return patch_loop.backward(plist, norm_weight, norm_bias, lambda k: outs[k - 1] if k else x_il4, stats, stashes, g, inner, outer, block,
+                                       activation, residual)
     grads = [tuple(torch.empty_like(t) for t in params) for params in plist]
     gg, gb, gx = torch.empty_like(norm_weight), torch.empty_like(norm_bias), torch.empty_like(g)
     with torch.cuda.device(dev):

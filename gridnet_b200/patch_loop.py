@@ -90,12 +90,14 @@ def _step_backward(params, grads, h, mr, norm_weight, norm_bias, gy, gx, inner: 
         gridnet_cuda.backward(*params, h, gy, *grads, gx, inner, block, 1e-5, False, activation)
 
 
-def backward(plist, norm_weight, norm_bias, x, outs, stats, stashes, grad_y, inner: int, outer: int, block: int, activation: str, residual: bool):
-    """One (weight, bias, scale) gradient per entry of ``plist``, those of the norm's weight and bias, and that of x."""
-    B, M, N, K = x.shape
+def backward(plist, norm_weight, norm_bias, input_of, stats, stashes, grad_y, inner: int, outer: int, block: int, activation: str, residual: bool):
+    """One (weight, bias, scale) gradient per entry of ``plist``, those of the norm's weight and bias, and that of x. ``input_of(k)``: the
+    input of step k, which is the output of step k - 1. They are asked for from the last (``outer``, with residual ``outer - 1``) down to 0,
+    and none is held when the next one is asked for."""
+    B, M, N, K = grad_y.shape
     P, st = M * N * K, torch.cuda.current_stream().cuda_stream
-    nws = _workspace(lib.gn_norm_workspace_bytes(B, P), x.device)
-    sums = torch.empty(B, 2, dtype=torch.float64, device=x.device)
+    nws = _workspace(lib.gn_norm_workspace_bytes(B, P), grad_y.device)
+    sums = torch.empty(B, 2, dtype=torch.float64, device=grad_y.device)
     grads, gg, gb = [None] * len(plist), None, None
 
     def norm_backward(h, mr, g):
@@ -109,11 +111,12 @@ def backward(plist, norm_weight, norm_bias, x, outs, stats, stashes, grad_y, inn
     g = grad_y
     for k in reversed(range(outer)):
         kp = k % len(plist)
-        h = outs[k - 1] if k else x
         mr = stats[k] if residual else (stats[k - 1] if k else None)
         if not residual:
-            g, gg, gb = norm_backward(outs[k], stats[k], g)
-        here, gx = [torch.empty_like(t) for t in plist[kp]], torch.empty_like(x)
+            g, gg, gb = norm_backward(input_of(k + 1), stats[k], g)
+        h = None  # that of the step after
+        h = input_of(k)
+        here, gx = [torch.empty_like(t) for t in plist[kp]], torch.empty_like(grad_y)
         _step_backward(plist[kp], here, h, mr, norm_weight, norm_bias, g, gx, inner, block, activation, stashes[k])
         if residual:
             gx -= g  # h' = h + net(n) - n: n also enters with a minus sign
