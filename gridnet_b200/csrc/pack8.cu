@@ -29,11 +29,12 @@ __global__ void __launch_bounds__(256) pack8_k(const T *__restrict__ x, unsigned
     }
 }
 
-// a half holds no more than 65504: what stands for 65536 next to it is not made an infinity
+// The largest halves have codes that stand for 65536, which is no half and would be rounded to an infinity: 65504 again. Codes for more than that are
+// not of halves, and rounded like any float
 template <typename T>
 __device__ __forceinline__ float held_by(float v) { return v; }
 template <>
-__device__ __forceinline__ float held_by<__half>(float v) { return magnitude_bits(v) < 0x7f800000u ? fminf(fmaxf(v, -65504.0f), 65504.0f) : v; }
+__device__ __forceinline__ float held_by<__half>(float v) { return fabsf(v) == 65536.0f ? copysignf(65504.0f, v) : v; }
 
 template <typename T>
 __global__ void __launch_bounds__(256) unpack8_k(const unsigned char *__restrict__ codes, const unsigned char *__restrict__ scales,

@@ -117,7 +117,7 @@ def pack_activations(x: torch.Tensor, rows: int = 1) -> PackedActivations:
 
 def unpack_activations(packed: PackedActivations, out: torch.Tensor | None = None) -> torch.Tensor:
     """What the packed copy stands for, in the tensor's own type or in ``out``'s (contiguous, any of the three types; no memory of the
-    copy's). Autograd sees a change in place of ``out``."""
+    copy's), rounded to it. Autograd sees a change in place of ``out``."""
     codes, scales, dtype = packed
     for name, t in (("codes", codes), ("scales", scales)):
         if not t.is_cuda:

@@ -533,7 +533,8 @@ GN_API int gn_gated_loop_backward_f32(const float *weight, const float *bias, co
  * are +inf, -inf and NaN (at e = 122 codes end at 63: what is finite stays so). scales [rows][ceil(cols / 32)]: e + 127 as a byte. A value is off by at most 2^(e-1). */
 typedef enum gn_dtype { GN_F32 = 0, GN_BF16 = 1, GN_F16 = 2 } gn_dtype;
 GN_API int gn_pack8(const void *x, void *codes, void *scales, long long rows, long long cols, int dtype, void *stream);
-/* A half that the codes put at 65536 comes out as 65504. */
+/* Values are rounded to the type of x. Halves: 65536, where the codes put the largest of them, comes out as 65504; what is beyond is of another
+ * type and becomes an infinity. */
 GN_API int gn_unpack8(const void *codes, const void *scales, void *x, long long rows, long long cols, int dtype, void *stream);
 
 /* gn_norm_forward_f32 that leaves what its backward pass needs in 8 bits: codes [B][P], scales [B][ceil(P / 32)] of x, and
