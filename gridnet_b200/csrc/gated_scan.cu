@@ -21,7 +21,8 @@
 // Steps whose n_t is 0 (gates from about 104 up, and +inf) do not look at their value, which may be NaN; steps whose a_t is 0 do not look
 // at the state. Anything else that is not finite stays in the state. Threads that hold a gate beyond 80 select while they compute the gates,
 // those that hold a reset (a_t = 0) also while they go through the steps; all others have products and sums alone. A run with a reset has the
-// sign bit in A (-0): an A that became +0 by underflow still passes on a state that is not finite.
+// sign bit in A (-0). One without, whose factors' product is too small for a float, has the smallest one there is: off by no more than a
+// product that is rounded, and a state that is infinite stays so, where 0 * inf would be no number.
 //
 // A thread has two channels, so that a row is read 64 channels at a time and arithmetic is on pairs (f32x2); a warp has a run of steps
 // of its own, no lane has to know another lane's.
@@ -196,6 +197,14 @@ __device__ __forceinline__ float product(float a, float b)
     return __uint_as_float(__float_as_uint(a * b) | ((__float_as_uint(a) | __float_as_uint(b)) & 0x80000000u));
 }
 __device__ __forceinline__ float2 product(float2 a, float2 b) { return make_float2(product(a.x, b.x), product(a.y, b.y)); }
+__device__ __forceinline__ float at_least(float a)  // a >= 0 or NaN
+{
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(__uint_as_float(1u)));
+    return m;
+}
+__device__ __forceinline__ float2 at_least(float2 a) { return make_float2(at_least(a.x), at_least(a.y)); }
+__device__ __forceinline__ float2 kept(float2 a) { return make_float2(resets(a.x) ? a.x : at_least(a.x), resets(a.y) ? a.y : at_least(a.y)); }
 // one step with a_t = 0 or n_t = 0 among those of the thread
 __device__ __forceinline__ float after(float a, float h, float b) { return a == 0.0f ? b : fmaf(a, h, b); }
 __device__ __forceinline__ float2 after(float2 a, float2 h, float2 b) { return make_float2(after(a.x, h.x, b.x), after(a.y, h.y, b.y)); }
@@ -204,6 +213,11 @@ __device__ __forceinline__ float2 more(float2 A, float2 a)
     return make_float2(a.x == 0.0f ? -0.0f : product(A.x, a.x), a.y == 0.0f ? -0.0f : product(A.y, a.y));
 }
 __device__ __forceinline__ float2 looked_at(float2 n, float2 v) { return make_float2(n.x == 0.0f ? 0.0f : v.x, n.y == 0.0f ? 0.0f : v.y); }
+
+// Gradient term of a run with another step (or run) behind it: A of all of them, g of that one; nothing passes a reset
+__device__ __forceinline__ float behind(float A, float g, float c) { return resets(A) ? c : fmaf(A, g, c); }
+__device__ __forceinline__ float2 behind(float2 A, float2 g, float2 c) { return make_float2(behind(A.x, g.x, c.x), behind(A.y, g.y, c.y)); }
+__device__ __forceinline__ bool not_a_number(float2 v) { return v.x != v.x || v.y != v.y; }
 
 // Rows outside of every sequence of a ragged call: zeros
 template <typename T>
@@ -657,6 +671,42 @@ struct Cursor {
 };
 
 // ------------------------------------------------------------------ chunks: what each tile amounts to, a warp per tile
+// C of a tile as products and sums do not give it, where a gradient that is infinite has met a product of 0: step by step, from memory. Threads come here
+// by themselves, so the search is another; and from the row alone, so that the kernel holds nothing more for it (selections in the loop above,
+// with what they start from held: 4 x 4097 x 1024 float32 backward 105.7 -> 110.8 us, this way 106.7)
+template <typename T, bool PACKED>
+__device__ float2 once_more(const Scan &p, long long row, int slab)
+{
+    int seq = 0, end = p.n;
+    if (!p.offsets)
+        seq = (int)(row / ((p.steps + kBwdTile - 1) >> kBwdLog2));
+    else
+        while (end - seq > 1) {
+            const int middle = seq + (end - seq) / 2;
+            (tile_row<kBwdLog2>(p, middle, sequence(p, middle), 0) <= row ? seq : end) = middle;
+        }
+    const Place q = sequence(p, seq);
+    const long long t0 = (row - tile_row<kBwdLog2>(p, seq, q, 0)) << kBwdLog2;
+    const int ch = slab * kSlab + (threadIdx.x & 31) * 2, per_row = (p.width + kPackGroup - 1) / kPackGroup;
+    float2 A = two(1.0f), C = two(0.0f);
+    for (long long t = max(t0, 0LL); t < min(t0 + kBwdTile, q.len); ++t) {  // whatever stands in the offsets, rows of the sequence
+        const long long r = q.first + t;
+        float z[2] = {0.0f, 0.0f}, g[2] = {0.0f, 0.0f};
+        for (int k = 0; k < 2 && ch + k < p.width; ++k) {
+            if constexpr (PACKED)
+                z[k] = unpack1(((const unsigned char *)p.gate)[r * p.width + ch + k], pack_step(p.gate_scales[r * per_row + (ch + k) / kPackGroup]));
+            else
+                z[k] = to_float<T>(((const T *)p.gate)[(p.offsets ? r * p.gate_step : seq * p.gate_seq + t * p.gate_step) + ch + k]);
+            g[k] = to_float<T>(((const T *)p.gh)[r * p.width + ch + k]);
+        }
+        float2 a, n;
+        gates_any(make_float2(z[0], z[1]), a, n);
+        A = kept(more(A, a));
+        C = behind(A, make_float2(g[0], g[1]), C);
+    }
+    return C;
+}
+
 template <typename T, bool PACKED, bool BACKWARD>
 __global__ void __launch_bounds__(kScanThreads, 7) scan_maps_k(const Scan p)
 {
@@ -689,18 +739,22 @@ __global__ void __launch_bounds__(kScanThreads, 7) scan_maps_k(const Scan p)
                 A = mul2(A, z[s]);
                 if constexpr (BACKWARD) C = fma2(A, g[s], C);
             }
+            A = at_least(A);
         } else {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
                 H = after(z[s], H, mul2(n[s], u[s]));
-                A = more(A, z[s]);
-                if constexpr (BACKWARD) C = make_float2(resets(A.x) ? C.x : fmaf(A.x, g[s].x, C.x), resets(A.y) ? C.y : fmaf(A.y, g[s].y, C.y));
+                A = kept(more(A, z[s]));
+                if constexpr (BACKWARD) C = behind(A, g[s], C);
             }
         }
     }
     *plane(p, 0, row, slab) = A;
     *plane(p, 1, row, slab) = H;
-    if (BACKWARD) *plane(p, 2, row, slab) = C;
+    if (BACKWARD) {
+        if (not_a_number(C)) C = once_more<T, PACKED>(p, row, slab);
+        *plane(p, 2, row, slab) = C;
+    }
 }
 
 // ------------------------------------------------------------------ chunks: where each tile starts. A CTA has 16 channels of a sequence; 8 lanes, two
@@ -755,15 +809,15 @@ __global__ void __launch_bounds__(8 * kStartRuns) scan_starts_k(const Scan p)
             for (int i = 0; i < kBatch; ++i) {
                 if (BACKWARD) C = fma2(A, c[i], C);
                 H = fma2(a[i], H, b[i]);
-                A = mul2(A, a[i]);
+                A = at_least(mul2(A, a[i]));
             }
         } else {
 #pragma unroll
             for (int i = 0; i < kBatch; ++i)
                 if (k + i < count) {
-                    if (BACKWARD) C = make_float2(resets(A.x) ? C.x : fmaf(A.x, c[i].x, C.x), resets(A.y) ? C.y : fmaf(A.y, c[i].y, C.y));
+                    if (BACKWARD) C = behind(A, c[i], C);
                     H = through(a[i], H, b[i]);
-                    A = product(A, a[i]);
+                    A = kept(product(A, a[i]));
                 }
         }
     }
@@ -885,12 +939,14 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_forward_k(const Scan p)
                 H = fma2(a[s], H, b[s]);
                 A = mul2(A, a[s]);
             }
+            A = at_least(A);
         } else {
 #pragma unroll
             for (int s = 0; s < S; ++s) {
                 H = after(a[s], H, b[s]);
                 A = more(A, a[s]);
             }
+            A = kept(A);
         }
         ex.warp[par][0][warp][lane] = map_of(A, H);
         const bool any = __syncthreads_or(special);
@@ -990,12 +1046,16 @@ __global__ void __launch_bounds__(kScanThreads, 4) scan_backward_k(const Scan p)
                 A = mul2(A, a[s]);
                 C = fma2(A, g[s], C);
             }
-        } else {
+            A = at_least(A);
+        }
+        if (special || not_a_number(C)) {  // or where a gradient that is infinite has met a product of 0
+            A = two(1.0f);
+            H = C = two(0.0f);
 #pragma unroll
             for (int s = 0; s < S; ++s) {
                 H = after(a[s], H, mul2(n[s], u[s]));
-                A = more(A, a[s]);
-                C = make_float2(resets(A.x) ? C.x : fmaf(A.x, g[s].x, C.x), resets(A.y) ? C.y : fmaf(A.y, g[s].y, C.y));
+                A = kept(more(A, a[s]));
+                C = behind(A, g[s], C);
             }
         }
         ex.warp[par][0][warp][lane] = map_of(A, H);
