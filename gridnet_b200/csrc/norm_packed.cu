@@ -5,7 +5,8 @@
 //     gx = r (q - mean(q) - p mean(q p)),  ggamma = sum over the batch of g p,  gbeta = sum over the batch of g
 //
 // HBM-bound: forward 8 bytes for a value (and 4 more where its second reading does not hit L2) and 1.03 for its packed
-// copy, backward 5.03 twice and 4. Sums are in double, in a fixed order.
+// copy, backward 5.03 twice and 4. Sums over a sample are in double (backward of four products at a time, those added up as floats), sums over the
+// batch, which ggamma and gbeta are, in float; all in a fixed order.
 #include "kernels.h"
 #include "packed8.cuh"
 

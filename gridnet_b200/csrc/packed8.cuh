@@ -5,7 +5,8 @@
 // code depends on x alone, not on the order or kind of any arithmetic. Codes 127, -127 and -128 stand for +inf, -inf and NaN:
 // what is not finite stays what it is and touches no neighbour. The group's scale byte is e + 127, the exponent field
 // of the float 2^e, in [1, 249]. At the largest e, 122, codes end at 63: 64 * 2^122 is no float, and what is
-// finite stays so. 33 bytes hold 32 values; a value is off by at most 2^(e-1) <= m / 125 (m / 250 where m is just below 125 * 2^e).
+// finite stays so. 33 bytes hold 32 values; a value is off by at most 2^(e-1) < m / 125 (m / 250 where m is just below 125 * 2^e), but for the two
+// ends: at e = 122 a value beyond 63.5 * 2^122 is off by up to 2^122, and at e = -126 the bound 2^-127 may be all of a value.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

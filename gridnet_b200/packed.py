@@ -2,7 +2,8 @@
 
 Groups of 32 values of a row share a power of two 2^e, the smallest with ``|x| <= 125 * 2^e`` (e >= -126); a value is held as
 ``x / 2^e`` rounded to a whole number, half to even, in a signed byte. 127, -127 and -128 are +inf, -inf and NaN, so what is not finite
-stays what it is and does not touch its neighbours. 33 bytes hold 32 values, and a value is off by at most half a 2^e. The
+stays what it is and does not touch its neighbours. 33 bytes hold 32 values, and a value is off by at most half a 2^e (up to a whole one beyond
+63.5 * 2^122, the largest floats). A group has the precision of its largest: values that mark something are best infinite, a finite 1e30 leaves its neighbours none. The
 reference has no counterpart: it keeps float32 between the passes.
 
 :func:`pack_activations` / :func:`unpack_activations` are the two directions; :func:`keep_packed` has the norms, scans, steps and loops of this

@@ -174,10 +174,13 @@ def gated_scan(gate: torch.Tensor, value: torch.Tensor, state: torch.Tensor | No
 
     A step whose s(-gate) is 0 (gate = inf) holds the state and does not look at its value, one whose s(gate) is 0
     (gate = -inf) takes its value and does not look at the state. Differentiable once in gate, value and state, backward only: tensors with a
-    tangent of torch.autograd.forward_ad are refused. ``packed``: keep gate and
-    value in 8 bits for the backward pass, which then takes the gradients at the packed copies; default as
-    :func:`keep_packed` says. A step's values have to lie side by side, otherwise they are copied; steps and sequences may lie anywhere, so the
-    halves of a wider projection are read where they are."""
+    tangent of torch.autograd.forward_ad are refused. ``packed``: keep gate and value in 8 bits for the backward pass, which then takes the
+    gradients at the packed copies; default as :func:`keep_packed` says. Groups of 32 neighbouring values of a step share a scale, so gates that
+    hold or reset are best infinite.
+
+    Offsets on the host are copied to the device, which a graph capture does not allow, and refused unless they rise from 0 to the number of
+    rows; those on the device are not looked at, and may leave out rows ahead of the first sequence and behind the last. A step's values have to lie
+    side by side, otherwise they are copied; steps and sequences may lie anywhere, so the halves of a wider projection are read where they are."""
     if offsets is not None and not isinstance(offsets, torch.Tensor):
         offsets = torch.as_tensor(offsets, dtype=torch.int64)
     if not (torch.is_grad_enabled() and (gate.requires_grad or value.requires_grad or (state is not None and state.requires_grad))

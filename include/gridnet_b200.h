@@ -530,7 +530,8 @@ GN_API int gn_gated_loop_backward_f32(const float *weight, const float *bias, co
  * No counterpart in the reference, which keeps nothing but float32 between a forward and a backward pass.
  * Groups of 32 values of a row share a power of two 2^e: e the smallest whole number >= -126 with |x| <= 125 * 2^e for every finite x
  * of the group. codes [rows][cols]: x / 2^e rounded to a whole number (half to even) as a signed byte in [-125, 125]; 127, -127 and -128
- * are +inf, -inf and NaN (at e = 122 codes end at 63: what is finite stays so). scales [rows][ceil(cols / 32)]: e + 127 as a byte. A value is off by at most 2^(e-1). */
+ * are +inf, -inf and NaN. scales [rows][ceil(cols / 32)]: e + 127 as a byte. A value is off by at most 2^(e-1); at e = 122, where codes end at 63 so
+ * that what is finite stays so, by less than 2^122. */
 typedef enum gn_dtype { GN_F32 = 0, GN_BF16 = 1, GN_F16 = 2 } gn_dtype;
 GN_API int gn_pack8(const void *x, void *codes, void *scales, long long rows, long long cols, int dtype, void *stream);
 /* Values are rounded to the type of x. Halves: 65536, where the codes put the largest of them, comes out as 65504; what is beyond is of another
