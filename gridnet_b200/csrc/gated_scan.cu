@@ -21,8 +21,8 @@
 // Steps whose n_t is 0 (gates from about 104 up, and +inf) do not look at their value, which may be NaN; steps whose a_t is 0 do not look
 // at the state. Anything else that is not finite stays in the state. Threads that hold a gate beyond 80 select while they compute the gates,
 // those that hold a reset (a_t = 0) also while they go through the steps; all others have products and sums alone. A run with a reset has the
-// sign bit in A (-0). One without, whose factors' product is too small for a float, has the smallest one there is: off by no more than a
-// product that is rounded, and a state that is infinite stays so, where 0 * inf would be no number.
+// sign bit in A (-0). One without, whose factors' product is too small for a float, has the smallest one there is: off by less
+// than that, as a product of that size is once it is rounded, and a state that is infinite stays so, where 0 * inf would be no number.
 //
 // A thread has two channels, so that a row is read 64 channels at a time and arithmetic is on pairs (f32x2); a warp has a run of steps
 // of its own, no lane has to know another lane's.
