@@ -602,7 +602,8 @@ GN_API int gn_gated_scan_backward(const void *gate, const void *value, const voi
                                   const float *grad_last, void *grad_gate, void *grad_value, float *grad_state, int n, long long steps,
                                   long long total, int width, long long gate_seq, long long gate_step, long long value_seq,
                                   long long value_step, int dtype, void *workspace, size_t workspace_bytes, void *stream);
-/* One step of `rows` sequences: h and out_state [rows][width]; out_state may be state. gate_row, value_row: distance of rows in elements. */
+/* One step of `rows` sequences: h and out_state [rows][width]; out_state may be state, and h and out_state share no other memory with what
+ * is read (not checked here). gate_row, value_row: distance of rows in elements. */
 GN_API int gn_gated_scan_step(const void *gate, const void *value, const float *state, void *h, float *out_state, long long rows, int width,
                               long long gate_row, long long value_row, int dtype, void *stream);
 
